@@ -361,6 +361,48 @@ KK_API kk_status kk_wait_selftest(kk_engine* e, int64_t limit_ns);
 /* Message of the last kk_conv_selftest / kk_attention_selftest / kk_lstm_selftest failure on this thread. */
 KK_API const char* kk_conv_selftest_error(void);
 
+/*
+ * 8-bit operators on device buffers: rows held as e4m3 values with a power-of-two scale for each block
+ * of 128, and the linear layer over them. No counterpart in the reference (its linear layers are f32 and
+ * BF16x, docs/VALIDATION.md:38-45).
+ *
+ * A store is values (e4m3 bytes, rows ldv bytes apart) and exps (E8M0 bytes E, rows lde bytes apart, one
+ * byte per 128 columns): a block stands for value * 2^(E - 127). block_rows is 1 for activations (one
+ * row of exps per row) and 128 for weights (one row of exps per 128 rows). ldv is a multiple of 16 and
+ * lde of 4; values are 16-byte and exps 4-byte aligned. A block's E is the smallest integer >= 0 with
+ * max |x| <= 448 * 2^(E - 127) over its finite values; values are rounded to nearest even; infinities and
+ * NaN are held as NaN, which e4m3 has, and so reach every result that reads them. Nothing but the rows x k
+ * values and their exps is written: not the bytes between k and ldv, nor rows behind the last.
+ *
+ * All pointers are device pointers of device `cuda_ordinal`; `stream` is a cudaStream_t of that device
+ * (NULL: its legacy default stream). The calls only enqueue work (they may be captured into a graph),
+ * allocate nothing, keep nothing, and may run at once on several streams and host threads. The caller's
+ * current device is left as it was. rows / m = 0 is a no-op. Rows, columns and blocks stay below 2^31.
+ */
+typedef enum { KK_FP8_F32 = 0, KK_FP8_BF16 = 1, KK_FP8_E4M3 = 2 } kk_fp8_type;
+typedef enum { KK_FP8_ACT_NONE = 0, KK_FP8_ACT_GELU = 1 /* gelu_new, kernels/kokoro.cu:84-90 */ } kk_fp8_act;
+/* x [rows][k] of `type` (KK_FP8_F32 / KK_FP8_BF16), ldx elements apart, into a store. */
+KK_API kk_status kk_fp8_quantize(int cuda_ordinal, void* stream, const void* x, int type, int64_t rows, int64_t k,
+                                 int64_t ldx, int block_rows, uint8_t* values, int64_t ldv, uint8_t* exps,
+                                 int64_t lde);
+/* The values that a store stands for, into y [rows][k] of `type`, ldy elements apart. */
+KK_API kk_status kk_fp8_dequantize(int cuda_ordinal, void* stream, const uint8_t* values, int64_t ldv,
+                                   const uint8_t* exps, int64_t lde, int block_rows, int64_t rows, int64_t k, void* y,
+                                   int type, int64_t ldy);
+/*
+ * y = act(x w^T + bias) + residual: x a store of m rows (block_rows 1), w a store of n rows (block_rows
+ * 128), both of k columns; bias [n] or NULL; sums in 32 bits. y_type KK_FP8_F32 / KK_FP8_BF16: y [m][n],
+ * ldy elements apart, residual of the same type (ldr elements apart; NULL: none; it may be y itself).
+ * y_type KK_FP8_E4M3: y / ldy and y_exps / ldye are a store (block_rows 1) that the result is quantised
+ * into, without a residual. y may not overlap x or w.
+ */
+KK_API kk_status kk_fp8_linear(int cuda_ordinal, void* stream, int64_t m, int64_t n, int64_t k, const uint8_t* x,
+                               int64_t ldx, const uint8_t* x_exps, int64_t ldxe, const uint8_t* w, int64_t ldw,
+                               const uint8_t* w_exps, int64_t ldwe, const float* bias, int act, const void* residual,
+                               int64_t ldr, int y_type, void* y, int64_t ldy, uint8_t* y_exps, int64_t ldye);
+/* Message of the last kk_fp8_* failure on this thread. */
+KK_API const char* kk_fp8_error(void);
+
 /* Bytes of device memory the engine currently holds (weights + arena). */
 KK_API int64_t kk_device_bytes(const kk_engine* e);
 

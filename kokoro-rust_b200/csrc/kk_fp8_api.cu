@@ -1,0 +1,168 @@
+// C entries of the 8-bit operators: argument checks, the caller's device and stream, status codes.
+#include <cuda_runtime.h>
+#include <stdio.h>
+#include <exception>
+#include <string>
+
+#include "../../include/kokoro_b200.h"
+#include "kk_fp8.h"
+#include "kk_tc.h"
+
+namespace {
+
+thread_local std::string g_fp8_error;
+
+kk_status fail(kk_status s, const std::string& m) {
+  g_fp8_error = m;
+  return s;
+}
+
+// Makes the call's device current and puts the caller's back.
+struct DeviceGuard {
+  int prev = -1;
+  cudaError_t err = cudaSuccess;
+  explicit DeviceGuard(int dev) {
+    int cur = -1;
+    err = cudaGetDevice(&cur);
+    if (err == cudaSuccess && cur != dev) {
+      err = cudaSetDevice(dev);
+      if (err == cudaSuccess) prev = cur;
+    }
+  }
+  ~DeviceGuard() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+
+bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+constexpr int64_t MAX_DIM = (int64_t)1 << 31;  // rows, columns and strides stay below
+
+// A store of `rows` x `k` values: what is wrong with it, or null.
+const char* bad_store(const void* v, int64_t ldv, const void* e, int64_t lde, int64_t k) {
+  if (!v || !e) return "null store pointer";
+  if (ldv < k || ldv % 16 != 0 || ldv >= MAX_DIM) return "value rows must be a multiple of 16 bytes apart and hold every column";
+  if (lde < (k + 127) / 128 || lde % 4 != 0 || lde >= MAX_DIM)
+    return "exponent rows must be a multiple of 4 bytes apart and hold one byte per 128 columns";
+  if (!aligned(v, 16)) return "values must be 16-byte aligned";
+  if (!aligned(e, 4)) return "exponents must be 4-byte aligned";
+  return nullptr;
+}
+
+const char* bad_rows(const void* x, int type, int64_t k, int64_t ld) {
+  if (!x) return "null row pointer";
+  if (type != KK_FP8_F32 && type != KK_FP8_BF16) return "rows are f32 or bf16";
+  if (ld < k || ld >= MAX_DIM) return "row stride below the row's columns";
+  if (!aligned(x, type == KK_FP8_F32 ? 4 : 2)) return "rows must be aligned to their element";
+  return nullptr;
+}
+
+const char* bad_extent(int64_t rows, int64_t k) {
+  if (rows < 0 || rows >= MAX_DIM) return "row count out of range";
+  if (k < 1 || k >= MAX_DIM / 2) return "column count out of range";
+  if (rows > 0 && (k + 127) / 128 > (MAX_DIM - 1) / rows) return "more than 2^31 blocks";
+  return nullptr;
+}
+
+kk_status run(int ordinal, const char* what, cudaError_t (*f)(const void*, cudaStream_t), const void* arg, void* stream) {
+  try {
+    int n = 0;
+    cudaError_t e = cudaGetDeviceCount(&n);
+    if (e != cudaSuccess || ordinal < 0 || ordinal >= n)
+      return fail(e != cudaSuccess ? KK_ERR_CUDA : KK_ERR_INVALID_ARG, "CUDA device ordinal out of range");
+    DeviceGuard g(ordinal);
+    if (g.err != cudaSuccess) return fail(KK_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(g.err));
+    if (!kk::tc_available()) return fail(KK_ERR_CUDA, "device is not compute capability 10.x (sm_100a)");
+    e = f(arg, (cudaStream_t)stream);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return fail(e == cudaErrorMemoryAllocation ? KK_ERR_OOM : KK_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+    }
+    return KK_OK;
+  } catch (const std::exception& x) {
+    return fail(KK_ERR_CUDA, x.what());
+  }
+}
+
+struct QuantArgs {
+  const void* x;
+  int type;
+  long rows, k, ld;
+  int block_rows;
+  kk::Fp8Store q;
+};
+
+}  // namespace
+
+extern "C" {
+
+const char* kk_fp8_error(void) { return g_fp8_error.c_str(); }
+
+kk_status kk_fp8_quantize(int cuda_ordinal, void* stream, const void* x, int type, int64_t rows, int64_t k, int64_t ldx,
+                          int block_rows, uint8_t* values, int64_t ldv, uint8_t* exps, int64_t lde) {
+  if (const char* m = bad_extent(rows, k)) return fail(KK_ERR_INVALID_ARG, m);
+  if (block_rows != 1 && block_rows != 128) return fail(KK_ERR_INVALID_ARG, "block_rows must be 1 or 128");
+  if (rows == 0) return KK_OK;
+  if (const char* m = bad_rows(x, type, k, ldx)) return fail(KK_ERR_INVALID_ARG, m);
+  if (const char* m = bad_store(values, ldv, exps, lde, k)) return fail(KK_ERR_INVALID_ARG, m);
+  QuantArgs a{x, type, (long)rows, (long)k, (long)ldx, block_rows, {values, (long)ldv, exps, (long)lde}};
+  return run(cuda_ordinal, "kk_fp8_quantize", [](const void* p, cudaStream_t st) {
+    const QuantArgs& a = *(const QuantArgs*)p;
+    return kk::launch_fp8_quantize(a.x, a.type, a.rows, a.k, a.ld, a.block_rows, a.q, st);
+  }, &a, stream);
+}
+
+kk_status kk_fp8_dequantize(int cuda_ordinal, void* stream, const uint8_t* values, int64_t ldv, const uint8_t* exps,
+                            int64_t lde, int block_rows, int64_t rows, int64_t k, void* y, int type, int64_t ldy) {
+  if (const char* m = bad_extent(rows, k)) return fail(KK_ERR_INVALID_ARG, m);
+  if (block_rows != 1 && block_rows != 128) return fail(KK_ERR_INVALID_ARG, "block_rows must be 1 or 128");
+  if (rows == 0) return KK_OK;
+  if (const char* m = bad_rows(y, type, k, ldy)) return fail(KK_ERR_INVALID_ARG, m);
+  if (const char* m = bad_store(values, ldv, exps, lde, k)) return fail(KK_ERR_INVALID_ARG, m);
+  QuantArgs a{y, type, (long)rows, (long)k, (long)ldy, block_rows,
+              {const_cast<uint8_t*>(values), (long)ldv, const_cast<uint8_t*>(exps), (long)lde}};
+  return run(cuda_ordinal, "kk_fp8_dequantize", [](const void* p, cudaStream_t st) {
+    const QuantArgs& a = *(const QuantArgs*)p;
+    return kk::launch_fp8_dequantize(a.q, a.rows, a.k, a.block_rows, const_cast<void*>(a.x), a.type, a.ld, st);
+  }, &a, stream);
+}
+
+kk_status kk_fp8_linear(int cuda_ordinal, void* stream, int64_t m, int64_t n, int64_t k, const uint8_t* x, int64_t ldx,
+                        const uint8_t* x_exps, int64_t ldxe, const uint8_t* w, int64_t ldw, const uint8_t* w_exps,
+                        int64_t ldwe, const float* bias, int act, const void* residual, int64_t ldr, int y_type, void* y,
+                        int64_t ldy, uint8_t* y_exps, int64_t ldye) {
+  if (const char* s = bad_extent(m, k)) return fail(KK_ERR_INVALID_ARG, s);
+  if (const char* s = bad_extent(m, n)) return fail(KK_ERR_INVALID_ARG, s);
+  if (const char* s = bad_extent(n, k)) return fail(KK_ERR_INVALID_ARG, s);
+  if (act != KK_FP8_ACT_NONE && act != KK_FP8_ACT_GELU) return fail(KK_ERR_INVALID_ARG, "unknown activation");
+  if (y_type != KK_FP8_F32 && y_type != KK_FP8_BF16 && y_type != KK_FP8_E4M3)
+    return fail(KK_ERR_INVALID_ARG, "unknown output type");
+  if (m == 0) return KK_OK;
+  if (const char* s = bad_store(x, ldx, x_exps, ldxe, k)) return fail(KK_ERR_INVALID_ARG, std::string("x: ") + s);
+  if (const char* s = bad_store(w, ldw, w_exps, ldwe, k)) return fail(KK_ERR_INVALID_ARG, std::string("w: ") + s);
+  if (!aligned(bias, 4)) return fail(KK_ERR_INVALID_ARG, "bias must be 4-byte aligned");
+  if (y_type == KK_FP8_E4M3) {
+    if (residual) return fail(KK_ERR_INVALID_ARG, "an e4m3 result takes no residual");
+    if (const char* s = bad_store(y, ldy, y_exps, ldye, n)) return fail(KK_ERR_INVALID_ARG, std::string("y: ") + s);
+  } else {
+    if (const char* s = bad_rows(y, y_type, n, ldy)) return fail(KK_ERR_INVALID_ARG, std::string("y: ") + s);
+    if (residual)
+      if (const char* s = bad_rows(residual, y_type, n, ldr)) return fail(KK_ERR_INVALID_ARG, std::string("residual: ") + s);
+  }
+  struct Args {
+    kk::Fp8Linear a;
+  } g{};
+  g.a.m = (long)m, g.a.n = (long)n, g.a.k = (long)k;
+  g.a.x = {const_cast<uint8_t*>(x), (long)ldx, const_cast<uint8_t*>(x_exps), (long)ldxe};
+  g.a.w = {const_cast<uint8_t*>(w), (long)ldw, const_cast<uint8_t*>(w_exps), (long)ldwe};
+  g.a.bias = bias, g.a.gelu = act == KK_FP8_ACT_GELU, g.a.res = residual, g.a.ldr = (long)ldr, g.a.y_type = y_type;
+  if (y_type == KK_FP8_E4M3)
+    g.a.q = {(uint8_t*)y, (long)ldy, y_exps, (long)ldye};
+  else
+    g.a.y = y, g.a.ldy = (long)ldy;
+  return run(cuda_ordinal, "kk_fp8_linear", [](const void* p, cudaStream_t st) {
+    return kk::launch_fp8_linear(((const Args*)p)->a, nullptr, st);
+  }, &g, stream);
+}
+
+}  // extern "C"

@@ -78,6 +78,15 @@ _SIGS = {
     "kk_pth_data": (ctypes.c_void_p, [_P, ctypes.c_int]),
     "kk_pth_close": (None, [_P]),
     "kk_pth_error": (ctypes.c_char_p, []),
+    "kk_fp8_quantize": (ctypes.c_int, [ctypes.c_int, _P, _P, ctypes.c_int, ctypes.c_int64, ctypes.c_int64,
+                                       ctypes.c_int64, ctypes.c_int, _P, ctypes.c_int64, _P, ctypes.c_int64]),
+    "kk_fp8_dequantize": (ctypes.c_int, [ctypes.c_int, _P, _P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int,
+                                         ctypes.c_int64, ctypes.c_int64, _P, ctypes.c_int, ctypes.c_int64]),
+    "kk_fp8_linear": (ctypes.c_int, [ctypes.c_int, _P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _P,
+                                     ctypes.c_int64, _P, ctypes.c_int64, _P, ctypes.c_int64, _P, ctypes.c_int64, _P,
+                                     ctypes.c_int, _P, ctypes.c_int64, ctypes.c_int, _P, ctypes.c_int64, _P,
+                                     ctypes.c_int64]),
+    "kk_fp8_error": (ctypes.c_char_p, []),
     "kk_device_memory": (ctypes.c_int, [ctypes.c_int, _P, _P]),
 }
 

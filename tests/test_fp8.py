@@ -1,0 +1,135 @@
+"""The 8-bit operators on the CPU: the reference forms against each other, and every refusal of the C
+entries and of the torch entries that needs no GPU."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import fp8_ref as ref
+
+
+def test_codes_against_torch_conversion():
+    rng = np.random.default_rng(0)
+    v = np.concatenate([rng.uniform(-448, 448, 4000), rng.standard_normal(4000), rng.standard_normal(4000) * 2.0 ** -8,
+                        (ref._POS[1:] + ref._POS[:-1]) / 2, -(ref._POS[1:] + ref._POS[:-1]) / 2, ref._POS, -ref._POS])
+    v = v.astype(np.float32)
+    want = torch.from_numpy(v).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    assert np.array_equal(ref.e4m3_code(v.astype(np.float64)), want)
+    assert np.array_equal(ref.TABLE[:127], torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy())
+
+
+def test_scale_is_the_smallest_that_holds_the_block():
+    for a in (0.0, 1e-45, 2.0 ** -126, 1.0, 447.9, 448.0, 448.0001, 449.0, 896.0, 897.0, 3.4e38):
+        e = ref.block_exp(a)
+        assert a <= 448.0 * 2.0 ** (e - 127)
+        assert e == 0 or a > 448.0 * 2.0 ** (e - 128)
+
+
+def test_quantize_keeps_half_a_step():
+    rng = np.random.default_rng(1)
+    x = rng.standard_normal((7, 300)) * np.exp(rng.uniform(-20, 20, (7, 1)))
+    code, E = ref.quantize(x)
+    back = ref.dequantize(code, E)
+    amax = np.repeat([[np.abs(r[b * 128:(b + 1) * 128]).max() for b in range(3)] for r in x], 128, 1)[:, :300]
+    # half a step of the value, or half of the smallest step (2^-9) at a scale below amax / 224
+    assert (np.abs(back - x) <= 2.0 ** -4 * np.abs(x) + 2.0 ** -10 * amax / 224).all()
+
+
+# ---- refusals of the C entries (nothing is launched; the pointers are never followed)
+
+P = 1 << 12  # an aligned address
+
+
+def q_args(**kw):
+    a = dict(dev=0, st=None, x=P, type=0, rows=4, k=256, ldx=256, br=1, v=P, ldv=256, e=P, lde=4)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("kw, word", [
+    (dict(rows=-1), "row count"), (dict(rows=1 << 31), "row count"), (dict(k=0), "column count"),
+    (dict(k=1 << 31), "column count"), (dict(rows=1 << 30, k=1024, ldx=1024, ldv=1024, lde=8), "blocks"),
+    (dict(br=2), "block_rows"), (dict(br=0), "block_rows"), (dict(x=None), "null"), (dict(type=2), "f32 or bf16"),
+    (dict(type=-1), "f32 or bf16"), (dict(ldx=255), "row stride"), (dict(x=P + 2), "aligned"),
+    (dict(v=None), "null"), (dict(e=None), "null"), (dict(ldv=255), "16 bytes"), (dict(ldv=240), "16 bytes"),
+    (dict(ldv=264), "16 bytes"), (dict(lde=2), "4 bytes"), (dict(lde=5), "4 bytes"), (dict(v=P + 8), "16-byte"),
+    (dict(e=P + 1), "4-byte"),
+])
+def test_quantize_refusals(kk, kw, word):
+    lib = kk.load_library()
+    assert lib.kk_fp8_quantize(*q_args(**kw)) == kk.engine.KK_ERR_INVALID_ARG
+    assert word in lib.kk_fp8_error().decode()
+    a = q_args(**kw)
+    if "x" in kw or "ldx" in kw or "type" in kw:  # the same rows on the way back
+        a = [a[0], a[1], a[8], a[9], a[10], a[11], a[7], a[4], a[5], a[2], a[3], a[6]]
+        assert lib.kk_fp8_dequantize(*a) == kk.engine.KK_ERR_INVALID_ARG
+        assert word in lib.kk_fp8_error().decode()
+
+
+def l_args(**kw):
+    a = dict(dev=0, st=None, m=4, n=256, k=128, x=P, ldx=128, xe=P, ldxe=4, w=P, ldw=128, we=P, ldwe=4, bias=None, act=0,
+             res=None, ldr=256, yt=0, y=P, ldy=256, ye=None, ldye=0)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("kw, word", [
+    (dict(m=-1), "row count"), (dict(n=0), "column count"), (dict(k=0), "column count"), (dict(n=-5), "column count"),
+    (dict(act=2), "activation"), (dict(yt=3), "output type"), (dict(x=None), "x: null"), (dict(w=None), "w: null"),
+    (dict(x=P + 4), "x: values"), (dict(w=P + 4), "w: values"), (dict(ldx=100), "x: value rows"),
+    (dict(ldxe=1), "x: exponent rows"), (dict(bias=P + 2), "bias"), (dict(y=None), "y: null"), (dict(ldy=255), "y: row stride"),
+    (dict(res=P, ldr=200), "residual: row stride"), (dict(res=P + 1), "residual: rows"),
+    (dict(yt=2, ldy=256, ye=P, ldye=4, res=P), "no residual"), (dict(yt=2, ldy=256, ye=None, ldye=4), "y: null"),
+    (dict(yt=2, ldy=250, ye=P, ldye=4), "y: value rows"), (dict(yt=1, y=P + 1), "y: rows"),
+])
+def test_linear_refusals(kk, kw, word):
+    lib = kk.load_library()
+    assert lib.kk_fp8_linear(*l_args(**kw)) == kk.engine.KK_ERR_INVALID_ARG
+    assert word in lib.kk_fp8_error().decode()
+
+
+def test_no_rows_is_a_no_op(kk):
+    lib = kk.load_library()
+    assert lib.kk_fp8_quantize(*q_args(rows=0, x=None, v=None, e=None)) == kk.engine.KK_OK
+    assert lib.kk_fp8_linear(*l_args(m=0, x=None, xe=None, y=None)) == kk.engine.KK_OK
+
+
+def test_bad_ordinal_is_a_status(kk):
+    lib = kk.load_library()
+    assert lib.kk_fp8_quantize(*q_args(dev=99)) in (kk.engine.KK_ERR_INVALID_ARG, kk.engine.KK_ERR_CUDA)
+    assert lib.kk_fp8_error()
+
+
+# ---- refusals of the torch entries
+
+
+def refused(kk, f, *a, **kw):
+    with pytest.raises(kk.KokoroError) as e:
+        f(*a, **kw)
+    assert e.value.status == kk.engine.KK_ERR_INVALID_ARG
+    return str(e.value)
+
+
+def test_torch_refusals(kk):
+    fp8 = kk.fp8
+    assert "CUDA tensor" in refused(kk, fp8.quantize, torch.zeros(4, 128))
+    assert "float32" in refused(kk, fp8.quantize, torch.zeros(4, 128, dtype=torch.float16))
+    assert "rows are wanted" in refused(kk, fp8.quantize, torch.zeros(128))
+    assert "adjacent" in refused(kk, fp8.quantize, torch.zeros(128, 4).t())
+    assert "store is wanted" in refused(kk, fp8.dequantize, torch.zeros(4, 128))
+    assert "block_rows 1" in refused(kk, fp8.linear, torch.zeros(4, 128), torch.zeros(4, 128))
+    v = torch.zeros(4, 128, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    assert "CUDA tensor" in refused(kk, fp8.Fp8Tensor, v, torch.zeros(4, 1, dtype=torch.uint8))
+    assert "values" in refused(kk, fp8.Fp8Tensor, v.view(torch.uint8), torch.zeros(4, 1, dtype=torch.uint8))
+
+
+def test_fp8_error_is_per_thread(kk):
+    import threading
+    lib = kk.load_library()
+    assert lib.kk_fp8_quantize(*q_args(k=0)) != 0
+    got = []
+    t = threading.Thread(target=lambda: got.append(ctypes.string_at(lib.kk_fp8_error())))
+    t.start()
+    t.join()
+    assert lib.kk_fp8_error() and got == [b""]

@@ -1,0 +1,357 @@
+"""The 8-bit operators on the GPU against their definition in 64 bits (tests/fp8_ref.py).
+
+Tolerances, derived: quantising is exact (the same codes and exponents). In the linear layer the
+products of two e4m3 values are exact in 32 bits, so an element is off by the additions alone. Each
+of at most K + 2 additions is off by at most one step of a partial sum, 2^-23 of it, and a partial sum
+is at most S = sum |x w| + |bias| + |residual|: |error| <= (K + 4) 2^-23 S for any order. Over a whole
+result the rounded partial sums have the size of the result, and an accumulator takes 32 products at a
+time: norm(error) <= 4 (K / 32 + 8) 2^-23 norm(sqrt(x^2 w^2 sums)). GELU has slope at most 1.13 and is
+evaluated to 2^-20. A bf16 result adds half a step, 2^-8 |y| at most, an e4m3 one 2^-4 |y| or half of
+its smallest step, 2^-10 of a scale that is at most amax / 224."""
+import numpy as np
+import pytest
+import torch
+
+import fp8_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+E4M3 = torch.float8_e4m3fn
+
+
+def hard_rows(rng, rows, k):
+    """Rows of very different sizes, with blocks of zeros, exact ties and values at the scale's border."""
+    x = rng.standard_normal((rows, k)) * np.exp(rng.uniform(-30, 30, (rows, 1)))
+    x[rows // 2] = 0.0
+    x[rows // 3] = rng.integers(-64, 65, k) * 0.5  # ties of the 4-bit grid
+    x[-1] = np.where(rng.random(k) < 0.5, 448.0, rng.integers(-448, 449, k))
+    x[0, : k // 2] *= 1e-8
+    return x.astype(np.float32)
+
+
+def bits(t):
+    return t.contiguous().view(torch.uint8).cpu().numpy()
+
+
+def check_store(q, code, E):
+    got = bits(q.values)
+    nan = (code & 127) == 127
+    assert np.array_equal((got & 127) == 127, nan)
+    assert np.array_equal(got[~nan], code[~nan])
+    assert np.array_equal(q.exps.cpu().numpy(), E)
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows, k, pad, off", [(1, 1, 0, 0), (1, 768, 0, 0), (3, 127, 0, 0), (5, 128, 1, 0), (130, 129, 3, 1),
+                                               (257, 514, 2, 0), (64, 2048, 8, 0), (128, 256, 0, 3), (9, 1000, 4, 2)])
+def test_quantize_and_read_back(kk, block_rows, dtype, rows, k, pad, off):
+    rng = np.random.default_rng(rows * 1000 + k)
+    buf = torch.zeros(rows * (k + pad) + off + 4, device="cuda", dtype=dtype)
+    x = buf[off:off + rows * (k + pad)].view(rows, k + pad)[:, :k]  # strided, at any offset of its elements
+    x.copy_(torch.from_numpy(hard_rows(rng, rows, k)))
+    x64 = x.double().cpu().numpy()
+    code, E = ref.quantize(x64, block_rows)
+    q = kk.fp8.quantize(x, block_rows=block_rows)
+    check_store(q, code, E)
+    assert np.array_equal(x.double().cpu().numpy(), x64)
+    back = ref.dequantize(code, E, block_rows)
+    got = kk.fp8.dequantize(q)
+    assert got.dtype == torch.float32 and np.array_equal(got.double().cpu().numpy(), back.astype(np.float32).astype(np.float64))
+    b16 = kk.fp8.dequantize(q, torch.bfloat16)
+    assert torch.equal(b16, torch.from_numpy(back.astype(np.float32)).to(torch.bfloat16).cuda())
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_infinities_and_nan(kk, block_rows):
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((140, 300)).astype(np.float32)
+    x[0, 3], x[1, 130], x[2, 299], x[139, 0] = np.inf, -np.inf, np.nan, np.nan
+    x[4, :128] = np.nan  # nothing finite in the block
+    x[5, 128:256] = np.inf
+    code, E = ref.quantize(x.astype(np.float64), block_rows)
+    q = kk.fp8.quantize(torch.from_numpy(x).cuda(), block_rows=block_rows)
+    check_store(q, code, E)
+    back = kk.fp8.dequantize(q).cpu().numpy()
+    assert np.array_equal(np.isnan(back), ~np.isfinite(x))
+
+
+def test_quantize_ends_of_the_range(kk):
+    x = np.zeros((6, 128), np.float32)
+    x[0, :4] = [3.4e38, -1e30, 1e25, 0]
+    x[1, :4] = [1e-45, -1e-42, 0, 0]
+    x[2, :2] = [2.0 ** -118, 2.0 ** -126]
+    x[3, :3] = [448 * 2.0 ** -127, 2.0 ** -127, 2.0 ** -136]
+    x[4, :2] = [-0.0, 0.0]
+    x[5, :2] = [np.nextafter(np.float32(448), np.float32(500)), 1]
+    code, E = ref.quantize(x.astype(np.float64))
+    q = kk.fp8.quantize(torch.from_numpy(x).cuda())
+    check_store(q, code, E)
+
+
+def test_store_is_written_within_its_rows_and_columns(kk):
+    fp8 = kk.fp8
+    vals = torch.full((40, 320), 0x55, device="cuda", dtype=torch.uint8)
+    exps = torch.full((40, 8), 0x66, device="cuda", dtype=torch.uint8)
+    store = fp8.Fp8Tensor(vals.view(E4M3)[:, :300], exps[:, :3])
+    x = torch.randn(7, 300, device="cuda")
+    fp8.quantize(x, out=store[11:18])
+    code, E = ref.quantize(x.double().cpu().numpy())
+    check_store(store[11:18], code, E)
+    v, e = vals.cpu().numpy(), exps.cpu().numpy()
+    assert (v[:11] == 0x55).all() and (v[18:] == 0x55).all() and (v[:, 300:] == 0x55).all()
+    assert (e[:11] == 0x66).all() and (e[18:] == 0x66).all() and (e[:, 3:] == 0x66).all()
+
+
+def make(rng, m, n, k, fp8, wild=False):
+    x = rng.standard_normal((m, k))
+    if wild:
+        x *= np.exp(rng.uniform(-8, 8, (m, 1)))
+        x[:, : min(k, 128)] *= (rng.random((m, 1)) < 0.7)  # some rows' first block is all zeros
+    w = rng.uniform(-1, 1, (n, k)) / np.sqrt(k)
+    xq = fp8.quantize(torch.from_numpy(x.astype(np.float32)).cuda())
+    wq = fp8.quantize(torch.from_numpy(w.astype(np.float32)).cuda(), block_rows=128)
+    xd = ref.dequantize(bits(xq.values), xq.exps.cpu().numpy())
+    wd = ref.dequantize(bits(wq.values), wq.exps.cpu().numpy(), 128)
+    return xq, wq, xd, wd
+
+
+def check_linear(got, y, S, rms, K, act, dtype):
+    """got against y: element by element, and as a whole (32-bit results)."""
+    tol = (K + 4) * 2.0 ** -23 * S * (1.13 if act else 1.0) + (2.0 ** -20 * np.abs(y) if act else 0.0)
+    if dtype == E4M3:
+        back = ref.dequantize(bits(got.values), got.exps.cpu().numpy())
+        n = y.shape[1]
+        amax = np.stack([np.abs(y[:, b:b + 128]).max(1) for b in range(0, n, 128)], 1)
+        amax = np.repeat(amax, 128, 1)[:, :n]
+        tol = tol * 1.07 + 2.0 ** -4 * np.abs(y) + 2.0 ** -10 * amax * (1 + 1e-3) / 224 + 1e-300
+        err = np.abs(back - y)
+    else:
+        g = got.double().cpu().numpy()
+        err = np.abs(g - y)
+        if dtype == torch.bfloat16:
+            tol = tol * 1.01 + 2.0 ** -8 * np.abs(y)
+        else:
+            tol = tol + 2.0 ** -24 * np.abs(y)
+            whole = 4 * (K / 32 + 8) * 2.0 ** -23 * (1.13 if act else 1.0) + 2.0 ** -20 * (act is not None) + 2.0 ** -23
+            assert np.linalg.norm(g - y) <= whole * np.linalg.norm(rms)
+    bad = np.argwhere(~(err <= tol))
+    assert len(bad) == 0, (len(bad), bad[:5].tolist(), err.max())
+
+
+SIZES = [(1, 1, 1), (1, 16, 128), (1, 768, 768), (2, 130, 100), (7, 128, 129), (16, 2304, 768), (17, 50, 512), (33, 257, 300),
+         (64, 512, 768), (65, 96, 640), (66, 2048, 768), (128, 768, 2048), (129, 255, 16), (200, 1090, 514), (300, 769, 1100),
+         (512, 768, 2048), (700, 640, 520)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, E4M3])
+@pytest.mark.parametrize("m, n, k", SIZES)
+def test_linear(kk, m, n, k, dtype):
+    rng = np.random.default_rng(m * 7 + n * 3 + k)
+    fp8 = kk.fp8
+    xq, wq, xd, wd = make(rng, m, n, k, fp8, wild=True)
+    bias = rng.standard_normal(n).astype(np.float32) * 0.1
+    bias_d = torch.from_numpy(bias).cuda()
+    res = None if dtype == E4M3 else torch.from_numpy(rng.standard_normal((m, n)).astype(np.float32)).cuda().to(dtype)
+    for act, r, b in ((None, None, bias_d), ("gelu", None, bias_d), (None, res, bias_d), ("gelu", res, None)):
+        y, S = ref.linear(xd, wd, None if b is None else bias, act, None if r is None else r.double().cpu().numpy())
+        got = fp8.linear(xq, wq, b, act=act, residual=r, out_dtype=dtype)
+        rms = np.sqrt((xd ** 2) @ (wd ** 2).T + y ** 2)
+        check_linear(got, y, S, rms, k, act, dtype)
+
+
+def test_linear_nan_reaches_its_row_only(kk):
+    rng = np.random.default_rng(3)
+    for m in (5, 200):
+        x = rng.standard_normal((m, 300)).astype(np.float32)
+        x[3, 140] = np.inf
+        w = torch.from_numpy(rng.standard_normal((150, 300)).astype(np.float32)).cuda()
+        y = kk.fp8.linear(kk.fp8.quantize(torch.from_numpy(x).cuda()), kk.fp8.quantize(w, block_rows=128))
+        assert y[3].isnan().all() and not y[:3].isnan().any() and not y[4:].isnan().any()
+
+
+def test_linear_far_apart_scales(kk):
+    """Rows of zeros, of 1e-30 and of 1e30 in one tile: each keeps its own relative accuracy."""
+    rng = np.random.default_rng(4)
+    for m in (6, 140):
+        x = rng.standard_normal((m, 256))
+        x[0], x[1], x[2] = 0.0, x[1] * 1e-30, x[2] * 1e30
+        w = rng.standard_normal((200, 256)).astype(np.float32)
+        w[:128] *= 1e-4
+        xq = kk.fp8.quantize(torch.from_numpy(x.astype(np.float32)).cuda())
+        wq = kk.fp8.quantize(torch.from_numpy(w).cuda(), block_rows=128)
+        xd = ref.dequantize(bits(xq.values), xq.exps.cpu().numpy())
+        wd = ref.dequantize(bits(wq.values), wq.exps.cpu().numpy(), 128)
+        y, S = ref.linear(xd, wd)
+        got = kk.fp8.linear(xq, wq).double().cpu().numpy()
+        assert (np.abs(got - y) <= (256 + 4) * 2.0 ** -23 * S).all()
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 130, 200), (20, 300, 514), (150, 300, 514)])
+@pytest.mark.parametrize("ldy_pad, off", [(1, 0), (2, 1), (4, 4), (8, 0), (0, 3)])
+def test_linear_any_strides_and_offsets(kk, m, n, k, ldy_pad, off):
+    """Result and residual rows at strides and offsets of every alignment; nothing is written beside them."""
+    rng = np.random.default_rng(m + n + ldy_pad)
+    fp8 = kk.fp8
+    xq, wq, xd, wd = make(rng, m, n, k, fp8)
+    for dtype in (torch.float32, torch.bfloat16):
+        buf = torch.full((off + (m + 2) * (n + ldy_pad),), 7.0, device="cuda", dtype=dtype)
+        y = buf[off:off + m * (n + ldy_pad)].view(m, n + ldy_pad)[:, :n]
+        rbuf = torch.randn(off + m * (n + ldy_pad + 1), device="cuda").to(dtype)
+        r = rbuf[off:].view(m, n + ldy_pad + 1)[:, :n]
+        got = fp8.linear(xq, wq, residual=r, out_dtype=dtype, out=y)
+        assert got.data_ptr() == y.data_ptr()
+        want, S = ref.linear(xd, wd, residual=r.double().cpu().numpy())
+        check_linear(y, want, S, np.sqrt((xd ** 2) @ (wd ** 2).T + want ** 2), k, None, dtype)
+        rest = buf.clone()
+        rest[off:off + m * (n + ldy_pad)].view(m, n + ldy_pad)[:, :n] = 7.0
+        assert (rest == 7.0).all()
+
+
+def test_linear_onto_its_residual(kk):
+    rng = np.random.default_rng(8)
+    for m in (3, 300):
+        xq, wq, xd, wd = make(rng, m, 768, 256, kk.fp8)
+        y = torch.randn(m, 768, device="cuda")
+        want = kk.fp8.linear(xq, wq, residual=y.clone())
+        kk.fp8.linear(xq, wq, residual=y, out=y)
+        assert torch.equal(y, want)
+
+
+def test_linear_result_store_within_a_larger_one(kk):
+    rng = np.random.default_rng(9)
+    fp8 = kk.fp8
+    for m in (5, 140):
+        xq, wq, xd, wd = make(rng, m, 300, 256, fp8)
+        vals = torch.full((m + 6, 336), 0x55, device="cuda", dtype=torch.uint8)
+        exps = torch.full((m + 6, 4), 0x66, device="cuda", dtype=torch.uint8)
+        store = fp8.Fp8Tensor(vals.view(E4M3)[:, :300], exps[:, :3])
+        fp8.linear(xq, wq, out_dtype=E4M3, out=store[2:m + 2])
+        want = fp8.linear(xq, wq, out_dtype=E4M3)
+        assert np.array_equal(bits(store[2:m + 2].values), bits(want.values))
+        assert torch.equal(store[2:m + 2].exps, want.exps)
+        v, e = vals.cpu().numpy(), exps.cpu().numpy()
+        assert (v[:2] == 0x55).all() and (v[m + 2:] == 0x55).all() and (v[:, 300:] == 0x55).all()
+        assert (e[:2] == 0x66).all() and (e[m + 2:] == 0x66).all() and (e[:, 3:] == 0x66).all()
+
+
+def test_rows_do_not_depend_on_the_batch_they_are_in(kk):
+    """Same inputs, same bits; and twice the same."""
+    rng = np.random.default_rng(10)
+    xq, wq, _, _ = make(rng, 700, 768, 2048, kk.fp8)
+    a, b = kk.fp8.linear(xq, wq), kk.fp8.linear(xq, wq)
+    assert torch.equal(a, b)
+
+
+def feed_forward(fp8, x, w1, b1, w2, b2, residual):
+    h = fp8.linear(fp8.quantize(x), w1, b1, act="gelu", out_dtype=E4M3)
+    return fp8.linear(h, w2, b2, residual=residual)
+
+
+@pytest.mark.parametrize("m", [1, 66, 513])
+def test_feed_forward_block(kk, m):
+    """The operators as they are used together; the middle store may round an element to the neighbouring
+    code where 32 and 64 bits fall on two sides of a border: at most one step of 2^-3 for each such element."""
+    rng = np.random.default_rng(m)
+    fp8 = kk.fp8
+    x = torch.from_numpy(rng.standard_normal((m, 768)).astype(np.float32)).cuda()
+    W = [(rng.uniform(-1, 1, s) / np.sqrt(s[1])).astype(np.float32) for s in ((2048, 768), (768, 2048))]
+    B = [(rng.uniform(-1, 1, s) * 0.03).astype(np.float32) for s in (2048, 768)]
+    w1, w2 = (fp8.quantize(torch.from_numpy(w).cuda(), block_rows=128) for w in W)
+    b1, b2 = (torch.from_numpy(b).cuda() for b in B)
+    got = feed_forward(fp8, x, w1, b1, w2, b2, x).double().cpu().numpy()
+    d1, d2 = (ref.dequantize(bits(w.values), w.exps.cpu().numpy(), 128) for w in (w1, w2))
+    x64 = x.double().cpu().numpy()
+    h, S = ref.linear(ref.dequantize(*ref.quantize(x64)), d1, B[0], "gelu")
+    hd = ref.dequantize(*ref.quantize(h))
+    y, S2 = ref.linear(hd, d2, B[1], None, x64)
+    # elements whose 32-bit value may lie across a border: within the layer's tolerance of a border
+    tol = (768 + 4) * 2.0 ** -23 * S * 1.13 + 2.0 ** -20 * np.abs(h)
+    step = np.maximum(2.0 ** -3 * np.abs(hd), 2.0 ** -9 * np.abs(h).max() / 224)
+    near = np.abs(np.abs(h - hd) - step / 2) <= tol + step / 4  # generous: a quarter of a step around each border
+    slack = (near * step * 1.5) @ np.abs(d2).T
+    assert (np.abs(got - y) <= (2048 + 4) * 2.0 ** -23 * S2 + slack + 2.0 ** -24 * np.abs(y)).all()
+    assert np.linalg.norm(got - y) <= 2e-3 * np.linalg.norm(y - x64)
+
+
+def test_streams_and_graphs(kk):
+    fp8 = kk.fp8
+    torch.manual_seed(0)
+    x = torch.randn(300, 768, device="cuda")
+    w1, w2 = (fp8.quantize(torch.randn(s, device="cuda") / 30, block_rows=128) for s in ((2048, 768), (768, 2048)))
+    b1, b2 = torch.randn(2048, device="cuda"), torch.randn(768, device="cuda")
+    want = feed_forward(fp8, x, w1, b1, w2, b2, x)
+    want_small = feed_forward(fp8, x[:5], w1, b1, w2, b2, x[:5])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for i, s in enumerate(streams * 3):  # calls at once on several streams
+        with torch.cuda.stream(s):
+            n = 5 if i % 2 else 300
+            got.append((n, feed_forward(fp8, x[:n], w1, b1, w2, b2, x[:n])))
+    torch.cuda.synchronize()
+    for n, y in got:
+        assert torch.equal(y, want if n == 300 else want_small)
+    # two captured graphs of the same operators, replayed on new inputs, at once on two streams
+    xs = [x.clone(), x.clone()]
+    graphs, outs = [], []
+    for xi in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(feed_forward(fp8, xi, w1, b1, w2, b2, xi))
+        graphs.append(g)
+    x2 = torch.randn(300, 768, device="cuda")
+    xs[1].copy_(x2)
+    want2 = feed_forward(fp8, x2, w1, b1, w2, b2, x2)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want2)
+
+
+def test_gpu_refusals(kk):
+    fp8 = kk.fp8
+    x = fp8.quantize(torch.randn(4, 256, device="cuda"))
+    w = fp8.quantize(torch.randn(130, 256, device="cuda"), block_rows=128)
+
+    def refused(f, *a, **k):
+        with pytest.raises(kk.KokoroError) as e:
+            f(*a, **k)
+        assert e.value.status == kk.engine.KK_ERR_INVALID_ARG
+        return str(e.value)
+
+    assert "block_rows 128" in refused(fp8.linear, x, x)
+    assert "block_rows 1 " in refused(fp8.linear, w, w)
+    w3 = fp8.quantize(torch.randn(130, 128, device="cuda"), block_rows=128)
+    assert "columns" in refused(fp8.linear, x, w3)
+    assert "act" in refused(fp8.linear, x, w, act="relu")
+    assert "bias" in refused(fp8.linear, x, w, torch.zeros(131, device="cuda"))
+    assert "bias" in refused(fp8.linear, x, w, torch.zeros(130, device="cuda", dtype=torch.bfloat16))
+    assert "one device" in refused(fp8.linear, x, w, torch.zeros(130))
+    assert "residual" in refused(fp8.linear, x, w, residual=torch.zeros(4, 129, device="cuda"))
+    assert "residual" in refused(fp8.linear, x, w, residual=torch.zeros(4, 130, device="cuda", dtype=torch.bfloat16))
+    assert "no residual" in refused(fp8.linear, x, w, residual=torch.zeros(4, 130, device="cuda"), out_dtype=E4M3)
+    assert "out_dtype" in refused(fp8.linear, x, w, out_dtype=torch.float16)
+    assert "out" in refused(fp8.linear, x, w, out=torch.zeros(4, 131, device="cuda"))
+    assert "out" in refused(fp8.linear, x, w, out=torch.zeros(4, 130, device="cuda"), out_dtype=torch.bfloat16)
+    assert "gradient" in refused(fp8.quantize, torch.zeros(4, 128, device="cuda", requires_grad=True))
+    assert "dtype" in refused(fp8.dequantize, x, torch.float16)
+    assert "block_rows" in refused(fp8.quantize, torch.zeros(4, 128, device="cuda"), block_rows=64)
+    assert "slice" in refused(w.__getitem__, slice(0, 1))
+    assert "exps" in refused(fp8.Fp8Tensor, x.values, x.exps[:3])
+    v = torch.zeros(4, 100, device="cuda", dtype=torch.uint8).view(E4M3)  # rows 100 bytes apart
+    assert "16 bytes" in refused(fp8.dequantize, fp8.Fp8Tensor(v, torch.zeros(4, 4, device="cuda", dtype=torch.uint8)[:, :1]))
+    with torch.no_grad():
+        fp8.quantize(torch.zeros(4, 128, device="cuda", requires_grad=True))
+
+
+def test_no_rows(kk):
+    fp8 = kk.fp8
+    q = fp8.quantize(torch.empty(0, 256, device="cuda"))
+    w = fp8.quantize(torch.randn(130, 256, device="cuda"), block_rows=128)
+    assert fp8.linear(q, w).shape == (0, 130)
+    assert fp8.linear(q, w, out_dtype=E4M3).shape == (0, 130)
+    assert fp8.dequantize(q).shape == (0, 256)
