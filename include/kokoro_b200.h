@@ -400,6 +400,12 @@ KK_API kk_status kk_fp8_linear(int cuda_ordinal, void* stream, int64_t m, int64_
                                int64_t ldx, const uint8_t* x_exps, int64_t ldxe, const uint8_t* w, int64_t ldw,
                                const uint8_t* w_exps, int64_t ldwe, const float* bias, int act, const void* residual,
                                int64_t ldr, int y_type, void* y, int64_t ldy, uint8_t* y_exps, int64_t ldye);
+/*
+ * Waits for the stream and reports (KK_ERR_TIMEOUT, once) whether a bounded in-kernel wait of a
+ * kk_fp8_linear on this device gave up since the last check; its results are then not valid. Not inside
+ * a capture.
+ */
+KK_API kk_status kk_fp8_check(int cuda_ordinal, void* stream);
 /* Message of the last kk_fp8_* failure on this thread. */
 KK_API const char* kk_fp8_error(void);
 

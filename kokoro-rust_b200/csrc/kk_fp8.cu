@@ -1,5 +1,5 @@
-// 8-bit operators on device buffers: quantising rows and weights to e4m3 with a power-of-two scale for
-// each block of 128, reading them back, and the linear layer over them (layout in kk_fp8.h).
+// 8-bit operators: quantising rows and weights to e4m3 with a power-of-two scale for each block of 128, and
+// reading them back (layout in kk_fp8.h).
 //
 // Block of 128 columns of one row (activations) or 128 x 128 (weights), a = max |x| over its finite
 // values: E is the smallest integer >= 0 with a <= 448 * 2^(E - 127) (448 is e4m3's largest value), and
@@ -7,56 +7,10 @@
 // NaN. A power of two scales exactly, so a value is rounded once and does not depend on the order or
 // precision of anything; against a * 2^-.. / 448 it gives up at most one binade of e4m3's range (15
 // binades of normal numbers), and it is the scale format the tensor core applies by itself.
-#include <cuda_bf16.h>
-#include <cuda_fp8.h>
-#include <string.h>
-
-#include "kk_common.cuh"
 #include "kk_fp8.h"
+#include "kk_fp8_math.cuh"
 
 namespace kk {
-
-// E of a block whose largest finite magnitude has these bits: 448 = 1.75 * 2^8, so with
-// a = m * 2^p, 1 <= m < 2, E - 127 is p - 8, and one more where m > 1.75.
-__device__ __forceinline__ int fp8_exp(uint32_t amax_bits) {
-  const int e = (int)(amax_bits >> 23) - 8 + ((amax_bits & 0x7FFFFF) > 0x600000 ? 1 : 0);
-  return e > 0 ? e : 0;
-}
-// 2^(127 - E), E in [0, 254]
-__device__ __forceinline__ float fp8_inv_scale(int e) {
-  return e == 254 ? __uint_as_float(1u << 22) : __uint_as_float((uint32_t)(254 - e) << 23);
-}
-// 2^(E - 127); 2^-127 is subnormal; E = 255 is E8M0's NaN
-__device__ __forceinline__ float fp8_scale(int e) {
-  return e == 0 ? __uint_as_float(1u << 22) : __uint_as_float(e == 255 ? 0x7FC00000u : (uint32_t)e << 23);
-}
-// Magnitude bits of a finite value, 0 for infinities and NaN: they order like the magnitudes.
-__device__ __forceinline__ uint32_t finite_bits(float v) {
-  const uint32_t u = __float_as_uint(v) & 0x7FFFFFFFu;
-  return u < 0x7F800000u ? u : 0u;
-}
-// four scaled values to e4m3, infinities (which the conversion would saturate) as NaN
-__device__ __forceinline__ uint32_t e4m3x4(const float* v, float inv) {
-  float s[4];
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    s[i] = v[i] * inv;
-    if (fabsf(v[i]) == INFINITY) s[i] = NAN;
-  }
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(s[0], s[1]), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(s[2], s[3]), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
-}
-__device__ __forceinline__ void e4m3x4_to_f32(uint32_t u, float* v) {
-#pragma unroll
-  for (int h = 0; h < 2; h++) {
-    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u >> (16 * h)), __NV_E4M3);
-    __half2 p;
-    memcpy(&p, &r, 4);
-    const float2 f = __half22float2(p);
-    v[2 * h] = f.x, v[2 * h + 1] = f.y;
-  }
-}
 
 // columns c .. c + 3 of a row (nothing past k: 0); VEC: one aligned load of the four
 template <typename T, bool VEC>
@@ -101,7 +55,7 @@ __global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const T* x, long ld
   uint32_t m = max(max(finite_bits(v[0]), finite_bits(v[1])), max(finite_bits(v[2]), finite_bits(v[3])));
   m = __reduce_max_sync(0xFFFFFFFFu, m);
   const int e = fp8_exp(m);
-  store_e4m3x4(q.v + r * q.ldv, c, k, e4m3x4(v, fp8_inv_scale(e)));
+  store_e4m3x4(q.v + r * q.ldv, c, k, e4m3x4(v[0], v[1], v[2], v[3], fp8_inv_scale(e)));
   if (lane == 0) q.e[r * q.lde + b] = (uint8_t)e;
 }
 
@@ -136,7 +90,7 @@ __global__ void __launch_bounds__(256) fp8_quant_blocks_kernel(const T* x, long 
   const float inv = fp8_inv_scale(e);
 #pragma unroll
   for (int i = 0; i < 16; i++)
-    if (r0 + i < rows) store_e4m3x4(q.v + (r0 + i) * q.ldv, c, k, e4m3x4(v[i], inv));
+    if (r0 + i < rows) store_e4m3x4(q.v + (r0 + i) * q.ldv, c, k, e4m3x4(v[i][0], v[i][1], v[i][2], v[i][3], inv));
   if (threadIdx.x == 0) q.e[rb * q.lde + b] = (uint8_t)e;
 }
 
@@ -164,85 +118,6 @@ __global__ void __launch_bounds__(256) fp8_dequant_kernel(Fp8Store q, long k, in
 #pragma unroll
   for (int j = 0; j < 4; j++)
     if (c + j < k) yr[c + j] = (T)(v[j] * s);
-}
-
-// ---- linear layer: y = act(x W^T + bias) + residual
-constexpr int LT = 32;  // tile edge of the plain kernel
-
-// The sum over a block of 128 columns is taken in 32 bits and scaled once by both blocks' powers of two.
-__global__ void __launch_bounds__(256) fp8_linear_plain_kernel(Fp8Linear a) {
-  __shared__ float xs[LT][33], ws[128][33], outs[LT][129];
-  const long m0 = (long)blockIdx.x * LT, n0 = (long)blockIdx.y * 128;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  float acc[4][4] = {};  // rows ty * 4 + i, columns tx + 32 * j
-  const int kb = (int)((a.k + 127) / 128);
-  for (int b = 0; b < kb; b++) {
-    float part[4][4] = {};
-    for (int k0 = b * 128; k0 < b * 128 + 128 && k0 < a.k; k0 += 32) {
-      for (int i = threadIdx.x; i < (LT + 128) * 32; i += 256) {
-        const int r = i / 32, c = i % 32;
-        const bool isx = r < LT;
-        const long row = isx ? m0 + r : n0 + r - LT;
-        const Fp8Store& s = isx ? a.x : a.w;
-        float v[4] = {0, 0, 0, 0};
-        if (row < (isx ? a.m : a.n) && k0 + c < a.k) e4m3x4_to_f32(s.v[row * s.ldv + k0 + c], v);
-        if (isx)
-          xs[r][c] = v[0];
-        else
-          ws[r - LT][c] = v[0];
-      }
-      __syncthreads();
-      for (int c = 0; c < 32; c++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) part[i][j] = fmaf(xs[ty * 4 + i][c], ws[tx + 32 * j][c], part[i][j]);
-      __syncthreads();
-    }
-    const float sw = fp8_scale(a.w.e[blockIdx.y * a.w.lde + b]);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const long m = m0 + ty * 4 + i;
-      const float s = m < a.m ? fp8_scale(a.x.e[m * a.x.lde + b]) * sw : 0.0f;
-#pragma unroll
-      for (int j = 0; j < 4; j++) acc[i][j] = fmaf(part[i][j], s, acc[i][j]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const long m = m0 + ty * 4 + i, n = n0 + tx + 32 * j;
-      float v = acc[i][j];
-      if (m < a.m && n < a.n) {
-        if (a.bias) v += a.bias[n];
-        if (a.gelu) v = gelu_new(v);
-        if (a.y_type == FP8_F32) {
-          if (a.res) v += ((const float*)a.res)[m * a.ldr + n];
-          ((float*)a.y)[m * a.ldy + n] = v;
-        } else if (a.y_type == FP8_BF16) {
-          if (a.res) v += (float)((const __nv_bfloat16*)a.res)[m * a.ldr + n];
-          ((__nv_bfloat16*)a.y)[m * a.ldy + n] = __float2bfloat16(v);
-        }
-      } else {
-        v = 0.0f;
-      }
-      outs[ty * 4 + i][tx + 32 * j] = v;
-    }
-  if (a.y_type != FP8_E4M3) return;
-  __syncwarp();
-  for (int i = 0; i < 4; i++) {
-    const long m = m0 + ty * 4 + i;
-    if (m >= a.m) return;
-    float v[4];
-    for (int j = 0; j < 4; j++) v[j] = outs[ty * 4 + i][4 * tx + j];
-    uint32_t mx = 0;
-    for (int j = 0; j < 4; j++) mx = max(mx, finite_bits(v[j]));
-    mx = __reduce_max_sync(0xFFFFFFFFu, mx);
-    const int e = fp8_exp(mx);
-    store_e4m3x4(a.q.v + m * a.q.ldv, n0 + 4 * tx, a.n, e4m3x4(v, fp8_inv_scale(e)));
-    if (tx == 0) a.q.e[m * a.q.lde + blockIdx.y] = (uint8_t)e;
-  }
 }
 
 template <typename T>
@@ -284,13 +159,6 @@ cudaError_t launch_fp8_dequantize(Fp8Store q, long rows, long k, int block_rows,
   else
     fp8_dequant_kernel<__nv_bfloat16, true><<<grid, 256, 0, st>>>(q, k, quads, total, block_rows, (__nv_bfloat16*)y,
                                                                   ldy);
-  return cudaGetLastError();
-}
-
-cudaError_t launch_fp8_linear(const Fp8Linear& a, int* err, cudaStream_t st) {
-  if (a.m == 0) return cudaSuccess;
-  const dim3 grid((unsigned)((a.m + LT - 1) / LT), (unsigned)((a.n + 127) / 128));
-  fp8_linear_plain_kernel<<<grid, 256, 0, st>>>(a);
   return cudaGetLastError();
 }
 

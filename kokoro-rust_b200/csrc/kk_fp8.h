@@ -39,7 +39,9 @@ cudaError_t launch_fp8_quantize(const void* x, int type, long rows, long k, long
                                 cudaStream_t st);
 cudaError_t launch_fp8_dequantize(Fp8Store q, long rows, long k, int block_rows, void* y, int type, long ldy,
                                   cudaStream_t st);
-// err receives 2 if a bounded pipeline wait expires
+// err receives 2 if a bounded pipeline wait expires; null: the device's own flag, for fp8_take_wait_error
 cudaError_t launch_fp8_linear(const Fp8Linear& a, int* err, cudaStream_t st);
+// Waits for the stream; *flag = the current device's flag, which is cleared.
+cudaError_t fp8_take_wait_error(int* flag, cudaStream_t st);
 
 }  // namespace kk

@@ -165,4 +165,14 @@ kk_status kk_fp8_linear(int cuda_ordinal, void* stream, int64_t m, int64_t n, in
   }, &g, stream);
 }
 
+kk_status kk_fp8_check(int cuda_ordinal, void* stream) {
+  int flag = 0;
+  int* const out = &flag;
+  const kk_status s = run(cuda_ordinal, "kk_fp8_check", [](const void* p, cudaStream_t st) {
+    return kk::fp8_take_wait_error(*(int* const*)p, st);
+  }, &out, stream);
+  if (s == KK_OK && flag) return fail(KK_ERR_TIMEOUT, "a bounded wait of kk_fp8_linear expired (code " + std::to_string(flag) + ")");
+  return s;
+}
+
 }  // extern "C"

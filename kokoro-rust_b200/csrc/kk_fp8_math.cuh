@@ -1,0 +1,69 @@
+// Device helpers of the 8-bit operators: block scales, e4m3 conversions, the GELU of their epilogues.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+#include <string.h>
+
+namespace kk {
+
+// E of a block whose largest finite magnitude has these bits: 448 = 1.75 * 2^8, so with
+// a = m * 2^p, 1 <= m < 2, E - 127 is p - 8, and one more where m > 1.75. At most 247.
+__device__ __forceinline__ int fp8_exp(uint32_t amax_bits) {
+  const int e = (int)(amax_bits >> 23) - 8 + ((amax_bits & 0x7FFFFF) > 0x600000 ? 1 : 0);
+  return e > 0 ? e : 0;
+}
+// 2^(127 - E), E in [0, 247]
+__device__ __forceinline__ float fp8_inv_scale(int e) { return __uint_as_float((uint32_t)(254 - e) << 23); }
+// 2^(E - 127); 2^-127 is subnormal; E = 255 is E8M0's NaN
+__device__ __forceinline__ float fp8_scale(int e) {
+  return __uint_as_float(e == 0 ? 1u << 22 : (e == 255 ? 0x7FC00000u : (uint32_t)e << 23));
+}
+// Magnitude bits of a finite value, 0 for infinities and NaN: they order like the magnitudes.
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t u = __float_as_uint(v) & 0x7FFFFFFFu;
+  return u < 0x7F800000u ? u : 0u;
+}
+// four scaled values to e4m3, infinities (which the conversion would saturate) as NaN
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d, float inv) {
+  const float s[4] = {a * inv, b * inv, c * inv, d * inv};
+  uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(s[0], s[1]), __NV_SATFINITE, __NV_E4M3);
+  uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(s[2], s[3]), __NV_SATFINITE, __NV_E4M3);
+  uint32_t u = lo | (hi << 16);
+  // a finite value of the block is at most 448 once scaled: only an infinity is still one
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (fabsf(s[i]) == INFINITY) u |= 0x7Fu << (8 * i);
+  return u;
+}
+__device__ __forceinline__ void e4m3x4_to_f32(uint32_t u, float* v) {
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u >> (16 * h)), __NV_E4M3);
+    __half2 p;
+    memcpy(&p, &r, 4);
+    const float2 f = __half22float2(p);
+    v[2 * h] = f.x, v[2 * h + 1] = f.y;
+  }
+}
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+  uint32_t u;
+  memcpy(&u, &p, 4);
+  return u;
+}
+
+// gelu_new(x) = x / 2 (1 + tanh(u)) = x / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3), with the
+// hardware exponential and reciprocal: about 2^-21 relative near 0 and above. (The bf16 layers use the
+// hardware tanh, 2^-11; here the result may be kept in 32 bits, or be rounded to e4m3, where an error of
+// 2^-11 moves one value in a hundred to the neighbouring code.)
+__device__ __forceinline__ float gelu_fast(float x) {
+  constexpr float c = -2.0f * 0.797884560802865355f * 1.44269504088896341f;  // -2 sqrt(2 / pi) log2(e)
+  const float z = c * fmaf(0.044715f * x * x, x, x);
+  float t, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(z));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + t));
+  return x * r;
+}
+
+}  // namespace kk

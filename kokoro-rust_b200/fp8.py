@@ -195,3 +195,10 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
                                       *y))
     return out
 
+
+def check(device=None) -> None:
+    """Waits for the current stream and raises if a bounded in-kernel wait of a linear layer on this
+    device gave up since the last check (its results are then not valid)."""
+    dev = torch.device("cuda") if device is None else torch.device(device)
+    idx = torch.cuda.current_device() if dev.index is None else dev.index
+    _run(load_library().kk_fp8_check(idx, torch.cuda.current_stream(idx).cuda_stream))
