@@ -45,53 +45,118 @@ __device__ __forceinline__ void mma_mxf8(uint32_t tmem_d, uint64_t a, uint64_t b
 __device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint32_t saddr) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc(saddr, 128, 128)) : "memory");
 }
+
+// ---- the same over a pair of CTAs (cta_group::2): the MMA is issued by the pair's first CTA and reads both
+// CTAs' shared memory at the same offsets; each CTA holds its own 128 rows of the accumulator
+__device__ __forceinline__ void mma_mxf8_pair(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+                                              uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_cp_scales_pair(uint32_t taddr, uint32_t saddr) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc(saddr, 128, 128)) : "memory");
+}
+// arrives on the barrier at this offset in both CTAs once the pair's MMAs so far are done
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((unsigned short)3)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// the address of this CTA's shared-memory location in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// a load into this CTA's shared memory whose bytes complete on a barrier of either CTA of the pair
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// mbar_wait on a barrier that the other CTA of the cluster arrives on
+__device__ __forceinline__ bool mbar_try_cluster(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(b)), "r"(parity), "r"(500000u)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* b, uint32_t parity, volatile int* abort_flag, int* err) {
+  if (mbar_try_cluster(b, parity)) return true;
+  const unsigned long long t0 = tc_now();
+  while (true) {
+    if (mbar_try_cluster(b, parity)) return true;
+    if (*abort_flag) return false;
+    if (tc_now() - t0 > KK_WAIT_TIMEOUT_NS) {
+      *abort_flag = 1;
+      atomicExch(err, 2);
+      return false;
+    }
+  }
+}
 // Waits, at most KK_WAIT_TIMEOUT_NS, for a phase that work already in flight completes.
 __device__ __forceinline__ void mbar_drain(uint64_t* b, uint32_t parity) {
   const unsigned long long t0 = tc_now();
   while (!mbar_try_sleep(b, parity) && tc_now() - t0 < KK_WAIT_TIMEOUT_NS) {
   }
 }
-__device__ __forceinline__ void ldg_v8(const void* p, uint32_t* r) {
-  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "l"(p)
-               : "memory");
-}
-__device__ __forceinline__ void stg_v8(void* p, const uint32_t* r) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
-               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
-
 struct TcFp8Args {
   Fp8Linear a;
   int* err;
-  int kb;             // blocks of 128 columns of K
+  int kb;              // blocks of 128 columns of K
   int m_tiles, n_tiles;
-  int vec_y, vec_res; // rows of y / residual start on 32-byte boundaries
+  int tma_y;           // y (and the residual) can be stored (loaded) by TMA: 16-byte aligned rows
+  int tma_edge;        // so can their last columns: TMA writes whole 16-byte units, so n has to end on one
 };
 
-constexpr int TM = 128;       // rows of x of a tile
-constexpr int SF_RING = 2;    // scale groups (4 blocks of K each) in shared memory and TMEM
+// ---- large layers: a pair of CTAs per tile of 256 rows x 256 columns
+//
+// Bound by the tensor cores from about K = 1000 on, by HBM below. One CTA with a 128 x 256 tile reads 96 bytes of
+// L2 per SM and clock at the full MMA rate, more than L2 gives; a pair shares the 256 rows of W (each CTA loads
+// and holds half of them), which takes 64.
+constexpr int TM = 128, TN = 256;  // a CTA's rows, the pair's columns
+constexpr int SF_RING = 2;         // scale groups (4 blocks of K each) in shared memory and TMEM
+constexpr int EPI_WARPS = 8;       // two per TMEM lane quarter, 128 columns each
+constexpr int PAIR_THREADS = 32 * (4 + EPI_WARPS);
+constexpr int BOX = 4096;          // 32 rows of 128 bytes: what an epilogue warp stores (or loads) at once
 
-template <int NT>
-struct TcShape {
-  static constexpr int EPI = NT == 256 ? 8 : 4;                  // epilogue warps
-  static constexpr int COLS = NT / (EPI / 4);                    // columns of an epilogue thread
-  static constexpr int THREADS = 32 * (4 + EPI);
-  static constexpr int NB = (NT + 127) / 128;                    // 128-row scale tiles of W
-  static constexpr int A_BYTES = TM * 128, B_BYTES = NT * 128;
-  static constexpr int STAGES = NT == 256 ? 4 : (NT == 128 ? 6 : 8);
-  static constexpr int SF_BYTES = 512 * (1 + NB);
-  // TMEM columns: two accumulators (for NT = 256 they share columns 224..255, see the epilogue), then scales
-  static constexpr int D1 = NT == 256 ? 224 : NT;
-  static constexpr int SF_COL = D1 + NT;
-  static constexpr int SF_COLS = 4 * (1 + NB);
-  static constexpr int TMEM_COLS = SF_COL + SF_RING * SF_COLS <= 256 ? 256 : 512;
-  static constexpr int OFF_B = STAGES * A_BYTES, OFF_SF = OFF_B + STAGES * B_BYTES;
-  static constexpr int OFF_BIAS = OFF_SF + SF_RING * SF_BYTES, OFF_BAR = OFF_BIAS + EPI * COLS * 4;
-  static constexpr int SMEM = OFF_BAR + 256 + 1024;              // 1024: alignment of the first stage
-  static_assert(SF_COL + SF_RING * SF_COLS <= TMEM_COLS, "TMEM columns");
+template <int OUT, bool RES>
+struct PairShape {
+  static constexpr int STAGES = RES ? 4 : 5;
+  static constexpr int NBUF = RES ? 2 : 1;  // boxes of an epilogue warp; two, so that a residual is loaded ahead
+  static constexpr int A_BYTES = TM * 128, B_BYTES = TN / 2 * 128;
+  static constexpr int SF_BYTES = 512 * 3;
+  // TMEM columns: the two accumulators share columns 224..255 (see the epilogue); scales behind them
+  static constexpr int D1 = 224, SF_COL = D1 + TN, SF_COLS = 12;
+  static constexpr int OFF_B = STAGES * A_BYTES, OFF_BOX = OFF_B + STAGES * B_BYTES;
+  static constexpr int OFF_SF = OFF_BOX + EPI_WARPS * NBUF * BOX, OFF_BIAS = OFF_SF + SF_RING * SF_BYTES;
+  static constexpr int OFF_BAR = OFF_BIAS + EPI_WARPS * 128 * 4;
+  static constexpr int SMEM = OFF_BAR + 512 + 1024;  // 1024: alignment of the first stage
+  static_assert(SF_COL + SF_RING * SF_COLS <= 512, "TMEM columns");
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
@@ -112,46 +177,12 @@ __device__ __forceinline__ void warp_transpose(float* v, int lane) {
   }
 }
 
-// 32 columns from c of the 32 rows from r0 (lane = row): residual added, stored as T. Rows on 32-byte boundaries
-// are read and written as whole sectors by the lane that holds them; otherwise (any stride or offset, the last
-// columns) the warp transposes the square and reads and writes a row's 32 columns together.
+// Rows at strides or offsets that TMA does not take: 32 columns from c of the 32 rows from r0 (lane = row). The
+// warp transposes the square and reads and writes a row's 32 columns together.
 template <typename T>
-__device__ __forceinline__ void store_chunk(const TcFp8Args& p, float* v, long r0, long c, int lane) {
-  const Fp8Linear& a = p.a;
+__device__ __forceinline__ void store_any(const Fp8Linear& a, float* v, long r0, long c, int lane) {
   T* y = (T*)a.y;
   const T* res = (const T*)a.res;
-  if (p.vec_y && (!res || p.vec_res) && c + 32 <= a.n) {
-    if (r0 + lane >= a.m) return;
-    constexpr int PER = 32 / sizeof(T);  // elements of a sector
-    T* yr = y + (r0 + lane) * a.ldy + c;
-    const T* rr = res + (r0 + lane) * a.ldr + c;
-#pragma unroll
-    for (int q = 0; q < 32 / PER; q++) {
-      uint32_t u[8];
-      if (sizeof(T) == 4) {
-        if (res) {
-          ldg_v8(rr + q * PER, u);
-#pragma unroll
-          for (int i = 0; i < 8; i++) v[q * PER + i] += __uint_as_float(u[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) u[i] = __float_as_uint(v[q * PER + i]);
-      } else {
-        if (res) {
-          ldg_v8(rr + q * PER, u);
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            v[q * PER + 2 * i] += __uint_as_float(u[i] << 16);
-            v[q * PER + 2 * i + 1] += __uint_as_float(u[i] & 0xFFFF0000u);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) u[i] = bf16x2(v[q * PER + 2 * i], v[q * PER + 2 * i + 1]);
-      }
-      stg_v8(yr + q * PER, u);
-    }
-    return;
-  }
   warp_transpose(v, lane);
   if (c + lane >= a.n) return;
 #pragma unroll
@@ -163,133 +194,160 @@ __device__ __forceinline__ void store_chunk(const TcFp8Args& p, float* v, long r
   }
 }
 
-// A thread's 128 columns from c of its row, quantised as one block and stored.
-__device__ __forceinline__ void store_block(const Fp8Linear& a, const float* v, long r, long c) {
-  if (r >= a.m || c >= a.n) return;
-  uint32_t m = 0;
+// A block of 128 columns of a thread's row: its scale's E, and the values as e4m3, four to a word.
+__device__ __forceinline__ int quantize_block(const float* v, uint32_t* u) {
+  float m = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 128; i++)
-    if (c + 128 <= a.n || c + i < a.n) m = max(m, finite_bits(v[i]));
-  const int e = fp8_exp(m);
+  for (int i = 0; i < 128; i++) m = fmaxf(m, fabsf(v[i]));  // (a NaN is passed over)
+  uint32_t mb = __float_as_uint(m);
+  if (mb < 0x7F800000u) {
+    const int e = fp8_exp(mb);
+    const float inv = fp8_inv_scale(e);
+#pragma unroll
+    for (int i = 0; i < 32; i++) u[i] = e4m3x4_finite(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv);
+    return e;
+  }
+  mb = 0;
+#pragma unroll
+  for (int i = 0; i < 128; i++) mb = max(mb, finite_bits(v[i]));
+  const int e = fp8_exp(mb);
   const float inv = fp8_inv_scale(e);
-  uint8_t* row = a.q.v + r * a.q.ldv + c;
-  a.q.e[r * a.q.lde + (c >> 7)] = (uint8_t)e;
 #pragma unroll
-  for (int q = 0; q < 8; q++) {
-    uint4 u;
-    u.x = e4m3x4(v[16 * q], v[16 * q + 1], v[16 * q + 2], v[16 * q + 3], inv);
-    u.y = e4m3x4(v[16 * q + 4], v[16 * q + 5], v[16 * q + 6], v[16 * q + 7], inv);
-    u.z = e4m3x4(v[16 * q + 8], v[16 * q + 9], v[16 * q + 10], v[16 * q + 11], inv);
-    u.w = e4m3x4(v[16 * q + 12], v[16 * q + 13], v[16 * q + 14], v[16 * q + 15], inv);
-    if (c + 16 * q + 16 <= a.n) {
-      *reinterpret_cast<uint4*>(row + 16 * q) = u;
-    } else {
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  for (int i = 0; i < 32; i++) u[i] = e4m3x4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv);
+  return e;
+}
+
+__device__ __forceinline__ void add_bias32(float* v, const float* bias_s) {
 #pragma unroll
-      for (int i = 0; i < 16; i++)
-        if (c + 16 * q + i < a.n) row[16 * q + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
-    }
+  for (int j = 0; j < 32; j += 4) {
+    const float4 b = *reinterpret_cast<const float4*>(bias_s + j);
+    v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
   }
 }
 
-// Persistent CTAs over tiles of 128 rows x NT columns, columns fastest (the tiles of one row tile run together
-// and share its rows of x through L2). Warp 0: TMA loads of x and W boxes (128 bytes x rows, 128-byte swizzle)
-// into a ring of stages; warp 1: MMAs; warp 2: scales, four blocks of K at a time, into shared memory in the
-// layout of the TMEM copy; the last warps: epilogue (a thread holds COLS columns of one row).
-template <int NT, int OUT>
-__global__ void __launch_bounds__(TcShape<NT>::THREADS, 1)
-    fp8_linear_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
-                         const __grid_constant__ TcFp8Args p) {
-  using S = TcShape<NT>;
+// Tiles in the order in which the pairs take them: columns fastest within groups of 8 row tiles (down the group
+// first), so that the tiles of a wave share few rows of x and of W in L2.
+__device__ __forceinline__ void tile_at(const TcFp8Args& p, int t, int* mt, int* nt) {
+  constexpr int G = 8;
+  const int per = G * p.n_tiles, g = t / per, r = t - g * per;
+  const int h = min(G, p.m_tiles - g * G);
+  *nt = r / h;
+  *mt = g * G + (r - *nt * h);
+}
+
+// Persistent pairs. In each CTA warp 0 loads its boxes of x and W (128 bytes x 128 rows, 128-byte swizzle) into a
+// ring of stages, warp 2 brings the scales, four blocks of K at a time, into shared memory in the layout of the
+// TMEM copy, warps 4..11 are the epilogue (a thread holds 128 columns of one row); warp 1 of the first CTA issues
+// the pair's MMAs. Barriers that the MMA warp waits on live in the first CTA; those it commits to, in both.
+template <int OUT, bool RES>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+    fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
+                           const __grid_constant__ CUtensorMap ymap, const __grid_constant__ CUtensorMap rmap,
+                           const __grid_constant__ TcFp8Args p) {
+  using S = PairShape<OUT, RES>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint64_t* full = (uint64_t*)(smem + S::OFF_BAR);
   uint64_t *empty = full + S::STAGES, *sf_full = empty + S::STAGES, *sf_empty = sf_full + SF_RING;
   uint64_t *acc_full = sf_empty + SF_RING, *acc_free = acc_full + 1;
-  uint32_t* tmem_slot = (uint32_t*)(acc_free + 1);
+  uint64_t* res_full = acc_free + 1;  // [EPI_WARPS][NBUF]
+  uint32_t* tmem_slot = (uint32_t*)(res_full + EPI_WARPS * 2);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cta_rank();
   const Fp8Linear& a = p.a;
   int* err = p.err ? p.err : &g_fp8_wait_error;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::STAGES; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
-    for (int i = 0; i < SF_RING; i++) mbar_init(sf_full + i, 1), mbar_init(sf_empty + i, 1);
+    for (int i = 0; i < SF_RING; i++) mbar_init(sf_full + i, 2), mbar_init(sf_empty + i, 1);
     mbar_init(acc_full, 1);
-    mbar_init(acc_free, S::EPI);
+    mbar_init(acc_free, 2 * EPI_WARPS);
+    for (int i = 0; i < EPI_WARPS * 2; i++) mbar_init(res_full + i, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "n"(S::TMEM_COLS)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int tiles = p.m_tiles * p.n_tiles, kb = p.kb;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
   if (warp == 0) {
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-        const int m0 = t / p.n_tiles * TM, n0 = t % p.n_tiles * NT;
+      for (int t = first; ok && t < tiles; t += step) {
+        int mt, nt;
+        tile_at(p, t, &mt, &nt);
+        const int m0 = mt * 2 * TM + (int)rank * TM, n0 = nt * TN + (int)rank * (TN / 2);
         for (int b = 0; b < kb; b++, it++) {
           const uint32_t s = it % S::STAGES;
           if (it >= S::STAGES && !mbar_wait(empty + s, (it / S::STAGES + 1) & 1, abort_flag, err)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(full + s, S::A_BYTES + S::B_BYTES);
-          tma_load_2d(smem + s * S::A_BYTES, &xmap, b * 128, m0, full + s);
-          tma_load_2d(smem + S::OFF_B + s * S::B_BYTES, &wmap, b * 128, n0, full + s);
+          if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * (S::A_BYTES + S::B_BYTES));
+          const uint32_t bar = map_rank(full + s, 0);
+          tma_load_2d_pair(smem + s * S::A_BYTES, &xmap, b * 128, m0, bar);
+          tma_load_2d_pair(smem + S::OFF_B + s * S::B_BYTES, &wmap, b * 128, n0, bar);
         }
       }
-      if (!ok)  // loads still in flight land before the block's shared memory goes
-        for (uint32_t i = it > S::STAGES ? it - S::STAGES : 0; i < it; i++)
-          mbar_drain(full + i % S::STAGES, (i / S::STAGES) & 1);
+      // After an expired wait, loads still in flight land before the shared memory goes: the first CTA sees them
+      // complete, the second, whose loads complete there, waits far longer than a load takes.
+      if (!ok) {
+        if (rank == 0) {
+          for (uint32_t i = it > S::STAGES ? it - S::STAGES : 0; i < it; i++)
+            mbar_drain(full + i % S::STAGES, (i / S::STAGES) & 1);
+        } else {
+          const unsigned long long t0 = tc_now();
+          while (tc_now() - t0 < 1000000ull) __nanosleep(1000);
+        }
+      }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       uint32_t it = 0, g = 0, tile_n = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, tile_n++) {
-        if (tile_n > 0 && !mbar_wait(acc_free, (tile_n - 1) & 1, abort_flag, err)) break;
+      for (int t = first; ok && t < tiles; t += step, tile_n++) {
+        if (tile_n > 0 && !mbar_wait_cluster(acc_free, (tile_n - 1) & 1, abort_flag, err)) break;
         tc_fence_after();
         const uint32_t d = tmem + (tile_n & 1) * S::D1;
         for (int b = 0; b < kb; b++, it++) {
           const uint32_t slot = g % SF_RING, sfa = tmem + S::SF_COL + slot * S::SF_COLS, sfb = sfa + 4;
           if ((b & 3) == 0) {
-            if (!mbar_wait(sf_full + slot, (g / SF_RING) & 1, abort_flag, err)) {
+            if (!mbar_wait_cluster(sf_full + slot, (g / SF_RING) & 1, abort_flag, err)) {
               ok = false;
               break;
             }
             const uint32_t sf = smem_u32(smem + S::OFF_SF + slot * S::SF_BYTES);
-            tmem_cp_scales(sfa, sf);
-#pragma unroll
-            for (int i = 0; i < S::NB; i++) tmem_cp_scales(sfb + 4 * i, sf + 512 * (1 + i));
+            tmem_cp_scales_pair(sfa, sf);
+            tmem_cp_scales_pair(sfb, sf + 512);
+            tmem_cp_scales_pair(sfb + 4, sf + 1024);
           }
           const uint32_t s = it % S::STAGES;
-          if (!mbar_wait(full + s, (it / S::STAGES) & 1, abort_flag, err)) {
+          if (!mbar_wait_cluster(full + s, (it / S::STAGES) & 1, abort_flag, err)) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint64_t da = sdesc_sw128(smem_u32(smem + s * S::A_BYTES));
           const uint64_t db = sdesc_sw128(smem_u32(smem + S::OFF_B + s * S::B_BYTES));
-          const uint32_t id = idesc_mxf8(TM, NT, b & 3);
+          const uint32_t id = idesc_mxf8(2 * TM, TN, b & 3);
 #pragma unroll
-          for (int k = 0; k < 4; k++) mma_mxf8(d, da + 2 * k, db + 2 * k, id, sfa, sfb, b > 0 || k > 0);
-          mma_commit(empty + s);
+          for (int k = 0; k < 4; k++) mma_mxf8_pair(d, da + 2 * k, db + 2 * k, id, sfa, sfb, b > 0 || k > 0);
+          mma_commit_pair(empty + s);
           if ((b & 3) == 3 || b == kb - 1) {
-            mma_commit(sf_empty + slot);
+            mma_commit_pair(sf_empty + slot);
             g++;
           }
         }
-        if (ok) mma_commit(acc_full);
+        if (ok) mma_commit_pair(acc_full);
       }
       if (*abort_flag && it > 0)  // MMAs still in flight end before their operands and TMEM go
         mbar_drain(empty + (it - 1) % S::STAGES, ((it - 1) / S::STAGES) & 1);
@@ -297,19 +355,21 @@ __global__ void __launch_bounds__(TcShape<NT>::THREADS, 1)
   } else if (warp == 2) {
     uint32_t g = 0;
     bool ok = true;
-    for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-      const long m0 = (long)(t / p.n_tiles) * TM, n0 = (long)(t % p.n_tiles) * NT;
+    for (int t = first; ok && t < tiles; t += step) {
+      int mt, nt;
+      tile_at(p, t, &mt, &nt);
+      const long m0 = (long)mt * 2 * TM + rank * TM, n0 = (long)nt * TN;
       for (int b = 0; b < kb; b += 4, g++) {
-        uint32_t wx[4], ww[S::NB][4];
+        uint32_t wx[4], ww[2];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const long r = m0 + 32 * i + lane;
           wx[i] = r < a.m ? *reinterpret_cast<const uint32_t*>(a.x.e + r * a.x.lde + b) : 0u;
+        }
 #pragma unroll
-          for (int j = 0; j < S::NB; j++) {
-            const long c = n0 + 128 * j + 32 * i;
-            ww[j][i] = c < a.n ? *reinterpret_cast<const uint32_t*>(a.w.e + (c >> 7) * a.w.lde + b) : 0u;
-          }
+        for (int j = 0; j < 2; j++) {
+          const long c = n0 + 128 * j;
+          ww[j] = c < a.n ? *reinterpret_cast<const uint32_t*>(a.w.e + (c >> 7) * a.w.lde + b) : 0u;
         }
         const uint32_t slot = g % SF_RING;
         if (g >= SF_RING) {
@@ -318,87 +378,215 @@ __global__ void __launch_bounds__(TcShape<NT>::THREADS, 1)
         }
         const uint32_t sf = smem_u32(smem + S::OFF_SF + slot * S::SF_BYTES) + lane * 16;
         sts_u4(sf, make_uint4(wx[0], wx[1], wx[2], wx[3]));
-#pragma unroll
-        for (int j = 0; j < S::NB; j++) sts_u4(sf + 512 * (1 + j), make_uint4(ww[j][0], ww[j][1], ww[j][2], ww[j][3]));
+        sts_u4(sf + 512, make_uint4(ww[0], ww[0], ww[0], ww[0]));
+        sts_u4(sf + 1024, make_uint4(ww[1], ww[1], ww[1], ww[1]));
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(sf_full + slot);
+        if (lane == 0) mbar_arrive_cluster(map_rank(sf_full + slot, 0));
       }
     }
   } else if (warp >= 4) {
     const int ew = warp - 4, half = ew >> 2;
-    float* bias_s = (float*)(smem + S::OFF_BIAS) + ew * S::COLS;
-    uint32_t tile_n = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, tile_n++) {
-      const long r0 = (long)(t / p.n_tiles) * TM + (ew & 3) * 32;
-      const long c0 = (long)(t % p.n_tiles) * NT + half * S::COLS;
+    float* bias_s = (float*)(smem + S::OFF_BIAS) + ew * 128;
+    uint8_t* box = smem + S::OFF_BOX + ew * S::NBUF * BOX;
+    const uint32_t row_s = smem_u32(box) + lane * 128;  // this thread's row of the box; 16-byte units swizzled by row
+    const uint32_t acc_free0 = map_rank(acc_free, 0);
+    constexpr int BC = OUT == FP8_F32 ? 32 : (OUT == FP8_BF16 ? 64 : 128);  // columns of a box
+    constexpr int NCH = 128 / BC;
+    uint32_t tile_n = 0, nres = 0;
+    bool ok = true;
+    for (int t = first; ok && t < tiles; t += step, tile_n++) {
+      int mt, nt;
+      tile_at(p, t, &mt, &nt);
+      const long r0 = (long)mt * 2 * TM + rank * TM + (ew & 3) * 32;
+      const long c0 = (long)nt * TN + half * 128;
+      // The next tile's accumulator may be written once the columns that it shares with this one are read: the last
+      // 32 of the first accumulator are the first 32 of the second; the half that holds them reads them first. (The
+      // tile after next reuses all of this accumulator: it waits for the next tile's arrivals, which come after all
+      // of this tile's reads.)
+      const bool shares = half == (int)(1 - (tile_n & 1));
+      const int ch0 = shares && half == 1 ? NCH - 1 : 0;
+      // boxes with columns, and how many of them go by TMA
+      const int live = r0 < a.m && c0 < a.n ? (int)min((long)NCH, (a.n - c0 + BC - 1) / BC) : 0;
+      const int boxes = !p.tma_y || live == 0 ? 0 : (p.tma_edge ? live : (int)min((long)live, (a.n - c0) / BC));
+      // the boxes in the order of their use: ch0, then the others from 0 (NCH 2 or 4, ch0 0 or NCH - 1)
+      if constexpr (RES) {
+        // the first boxes' residuals, while the tile's MMAs run; a box is free once its last store has read it
+        if (boxes > 0 && lane == 0) {
+          bulk_wait_all_read();
+          int q = 0;
+          for (int i = 0; i < NCH && q < 2; i++) {
+            const int ch = (i + ch0) % NCH;
+            if (ch >= boxes) continue;
+            const uint32_t n = nres + q, bf = n & 1;
+            mbar_arrive_expect_tx(res_full + ew * 2 + bf, BOX);
+            tma_load_2d(box + bf * BOX, &rmap, (int)c0 + ch * BC, (int)r0, res_full + ew * 2 + bf);
+            q++;
+          }
+        }
+      }
       __syncwarp();
-      for (int i = lane; i < S::COLS; i += 32) bias_s[i] = a.bias && c0 + i < a.n ? a.bias[c0 + i] : 0.0f;
+      for (int i = lane; i < 128; i += 32) bias_s[i] = a.bias && c0 + i < a.n ? a.bias[c0 + i] : 0.0f;
       __syncwarp();
-      if (!__all_sync(0xFFFFFFFFu, mbar_wait(acc_full, tile_n & 1, abort_flag, err))) break;
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(acc_full, tile_n & 1, abort_flag, err));
+      if (!ok) break;
       tc_fence_after();
-      const uint32_t d = tmem + ((uint32_t)(ew & 3) << 21) + (tile_n & 1) * S::D1 + half * S::COLS;
-      // The next tile's accumulator may be written once the columns that it shares with this one are read: with
-      // NT = 256 the last 32 of the first accumulator, which are the first 32 of the second; the half that holds
-      // them reads them first. (The tile after next reuses all of this accumulator; it waits for the next tile's
-      // arrivals, which come after all of this tile's reads.)
-      const bool shares = NT == 256 && half == (int)(1 - (tile_n & 1));
-      const int first = shares && half == 1 ? S::COLS / 32 - 1 : 0;
-      if (!shares && lane == 0) mbar_arrive(acc_free);
+      const uint32_t d = tmem + ((uint32_t)(ew & 3) << 21) + (tile_n & 1) * S::D1 + half * 128;
+      if (!shares && lane == 0) mbar_arrive_cluster(acc_free0);
       if constexpr (OUT == FP8_E4M3) {
-        float v[S::COLS];
-        // all columns are read before any is stored: the block's scale needs them
+        float v[128];
         tmem_ld64(d, v);
         tmem_ld64(d + 64, v + 64);
-        tc_fence_before();
-        __syncwarp();
-        if (shares && lane == 0) mbar_arrive(acc_free);
-#pragma unroll
-        for (int i = 0; i < S::COLS; i += 4) {
-          const float4 bv = *reinterpret_cast<const float4*>(bias_s + i);
-          v[i] += bv.x, v[i + 1] += bv.y, v[i + 2] += bv.z, v[i + 3] += bv.w;
+        if (shares) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(acc_free0);
         }
+#pragma unroll
+        for (int i = 0; i < 4; i++) add_bias32(v + 32 * i, bias_s + 32 * i);
         if (a.gelu) {
 #pragma unroll
-          for (int i = 0; i < S::COLS; i++) v[i] = gelu_fast(v[i]);
+          for (int i = 0; i < 128; i++) v[i] = gelu_fast(v[i]);
         }
-        store_block(a, v, r0 + lane, c0);
-      } else {
-#pragma unroll 1
-        for (int i = 0; i < S::COLS / 32; i++) {
-          const int ch = (i + first) % (S::COLS / 32);
-          float v[32];
-          tmem_ld32(d + 32 * ch, v);
-          if (i == 0 && shares) {
-            tc_fence_before();
+        if (live) {
+          uint32_t u[32];
+          const int e = quantize_block(v, u);
+          if (r0 + lane < a.m) a.q.e[(r0 + lane) * a.q.lde + (c0 >> 7)] = (uint8_t)e;
+          if (boxes) {
+            if (lane == 0) bulk_wait_all_read();
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_free);
+#pragma unroll
+            for (int q = 0; q < 8; q++)
+              sts_u4(row_s + ((q ^ (lane & 7)) << 4), make_uint4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]));
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&ymap, (int)c0, (int)r0, box);
+              bulk_commit();
+            }
+          } else if (r0 + lane < a.m) {  // the last columns
+            uint8_t* row = a.q.v + (r0 + lane) * a.q.ldv + c0;
+#pragma unroll
+            for (int i = 0; i < 128; i++)
+              if (c0 + i < a.n) row[i] = (uint8_t)(u[i >> 2] >> (8 * (i & 3)));
+          }
+        }
+      } else {
+        int used = 0;
+#pragma unroll 1
+        for (int i = 0; i < NCH; i++) {
+          const int ch = (i + ch0) % NCH;
+          const uint32_t bf = RES ? (nres & 1) : 0;
+          const uint32_t row_b = row_s + bf * BOX;
+          const bool on = ch < live, tma = ch < boxes;
+          if (tma) {
+            if constexpr (RES) {
+              ok = __all_sync(0xFFFFFFFFu, mbar_wait(res_full + ew * 2 + bf, (nres >> 1) & 1, abort_flag, err));
+              if (!ok) break;
+            } else {
+              if (lane == 0) bulk_wait_all_read();
+              __syncwarp();
+            }
           }
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 bv = *reinterpret_cast<const float4*>(bias_s + 32 * ch + j);
-            v[j] += bv.x, v[j + 1] += bv.y, v[j + 2] += bv.z, v[j + 3] += bv.w;
-          }
-          if (a.gelu) {
+          for (int h = 0; h < BC / 32; h++) {
+            // (the shared columns are the last 32 of this box when it is read out of order: read the box backwards)
+            const int hh = ch0 != 0 ? BC / 32 - 1 - h : h;
+            const int c = ch * BC + 32 * hh;
+            float v[32];
+            tmem_ld32(d + c, v);
+            if (shares && i == 0 && h == 0) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster(acc_free0);
+            }
+            if (!on) continue;
+            add_bias32(v, bias_s + c);
+            if (a.gelu) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = gelu_fast(v[j]);
+              for (int j = 0; j < 32; j++) v[j] = gelu_fast(v[j]);
+            }
+            if (!tma) {
+              if (c0 + c < a.n) {
+                if constexpr (OUT == FP8_F32)
+                  store_any<float>(a, v, r0, c0 + c, lane);
+                else
+                  store_any<__nv_bfloat16>(a, v, r0, c0 + c, lane);
+              }
+              continue;
+            }
+            if constexpr (OUT == FP8_F32) {
+#pragma unroll
+              for (int q = 0; q < 8; q++) {
+                const uint32_t at = row_b + ((q ^ (lane & 7)) << 4);
+                float4 o = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                if constexpr (RES) {
+                  const float4 r = lds_f4(at);
+                  o.x += r.x, o.y += r.y, o.z += r.z, o.w += r.w;
+                }
+                sts_u4(at, make_uint4(__float_as_uint(o.x), __float_as_uint(o.y), __float_as_uint(o.z), __float_as_uint(o.w)));
+              }
+            } else {
+#pragma unroll
+              for (int q = 0; q < 4; q++) {
+                const uint32_t at = row_b + (((4 * hh + q) ^ (lane & 7)) << 4);
+                if constexpr (RES) {
+                  const float4 r = lds_f4(at);
+                  const uint32_t u[4] = {__float_as_uint(r.x), __float_as_uint(r.y), __float_as_uint(r.z), __float_as_uint(r.w)};
+#pragma unroll
+                  for (int k = 0; k < 4; k++) {
+                    v[8 * q + 2 * k] += __uint_as_float(u[k] << 16);
+                    v[8 * q + 2 * k + 1] += __uint_as_float(u[k] & 0xFFFF0000u);
+                  }
+                }
+                sts_u4(at, make_uint4(bf16x2(v[8 * q], v[8 * q + 1]), bf16x2(v[8 * q + 2], v[8 * q + 3]),
+                                      bf16x2(v[8 * q + 4], v[8 * q + 5]), bf16x2(v[8 * q + 6], v[8 * q + 7])));
+              }
+            }
           }
-          if (r0 >= a.m || c0 + 32 * ch >= a.n) continue;
-          if constexpr (OUT == FP8_F32)
-            store_chunk<float>(p, v, r0, c0 + 32 * ch, lane);
-          else
-            store_chunk<__nv_bfloat16>(p, v, r0, c0 + 32 * ch, lane);
+          if (!tma) continue;
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&ymap, (int)c0 + ch * BC, (int)r0, box + bf * BOX);
+            bulk_commit();
+          }
+          nres++;
+          used++;
+          if constexpr (RES) {
+            // the box of this store takes the residual after next, if the tile has one (boxes in use order)
+            if (used + 1 < boxes && lane == 0) {
+              int seen = 0, nx = 0;
+              for (int k = 0; k < NCH; k++) {
+                const int cc = (k + ch0) % NCH;
+                if (cc >= boxes) continue;
+                if (seen == used + 1) nx = cc;
+                seen++;
+              }
+              bulk_wait_all_read();
+              mbar_arrive_expect_tx(res_full + ew * 2 + bf, BOX);
+              tma_load_2d(box + bf * BOX, &rmap, (int)c0 + nx * BC, (int)r0, res_full + ew * 2 + bf);
+            }
+          }
         }
       }
       tc_fence_before();  // this tile's TMEM reads before the arrivals of the next
+    }
+    if (lane == 0) {
+      if (!ok && RES) {  // residual boxes still in flight land before the shared memory goes
+        const unsigned long long t0 = tc_now();
+        while (tc_now() - t0 < 1000000ull) __nanosleep(1000);
+      }
+      bulk_wait_all();
     }
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  cluster_sync();
   if (warp == 0) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::TMEM_COLS));
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
 }
 
@@ -422,16 +610,18 @@ static EncodeTiledFn encode_tiled() {
   return fn;
 }
 
-// Boxes of 128 bytes x box_rows of [rows][k] values, 128-byte swizzle; what lies outside reads as zero, so
-// neither K nor the rows need to be padded.
-static bool make_map(CUtensorMap* m, const Fp8Store& s, long rows, long k, int box_rows) {
+// Boxes of 128 bytes x box_rows of [rows][cols] elements of es bytes, rows ld elements apart, 128-byte swizzle; what
+// lies outside reads as zero and is not written, so no edge needs to be padded.
+static bool make_map(CUtensorMap* m, const void* base, int es, long rows, long cols, long ld, int box_rows) {
   const EncodeTiledFn fn = encode_tiled();
   if (!fn) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)s.ldv};
-  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * es};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, s.v, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const CUtensorMapDataType t = es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                        : (es == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8);
+  return fn(m, t, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
          CUDA_SUCCESS;
 }
@@ -448,46 +638,43 @@ static int num_sms() {
   return n;
 }
 
-template <int NT, int OUT>
-static cudaError_t launch_tc(const Fp8Linear& a, int* err, cudaStream_t st) {
-  using S = TcShape<NT>;
+template <int OUT, bool RES>
+static cudaError_t launch_pair(const Fp8Linear& a, int* err, cudaStream_t st) {
+  using S = PairShape<OUT, RES>;
+  constexpr int es = OUT == FP8_F32 ? 4 : (OUT == FP8_BF16 ? 2 : 1);
   TcFp8Args p;
   p.a = a;
   p.err = err;
   p.kb = (int)((a.k + 127) / 128);
-  p.m_tiles = (int)((a.m + TM - 1) / TM);
-  p.n_tiles = (int)((a.n + NT - 1) / NT);
-  const size_t es = a.y_type == FP8_F32 ? 4 : 2;
-  p.vec_y = ((uintptr_t)a.y | (a.ldy * es)) % 32 == 0;
-  p.vec_res = ((uintptr_t)a.res | (a.ldr * es)) % 32 == 0;
-  CUtensorMap xm, wm;
-  if (!make_map(&xm, a.x, a.m, a.k, TM) || !make_map(&wm, a.w, a.n, a.k, NT)) return cudaErrorInvalidValue;
-  const auto kernel = fp8_linear_tc_kernel<NT, OUT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+  p.m_tiles = (int)((a.m + 2 * TM - 1) / (2 * TM));
+  p.n_tiles = (int)((a.n + TN - 1) / TN);
+  CUtensorMap xm, wm, ym, rm;
+  if (!make_map(&xm, a.x.v, 1, a.m, a.k, a.x.ldv, TM) || !make_map(&wm, a.w.v, 1, a.n, a.k, a.w.ldv, TN / 2))
+    return cudaErrorInvalidValue;
+  const void* y = OUT == FP8_E4M3 ? a.q.v : a.y;
+  const long ldy = OUT == FP8_E4M3 ? a.q.ldv : a.ldy;
+  p.tma_y = ((uintptr_t)y | (size_t)ldy * es) % 16 == 0 && (!RES || ((uintptr_t)a.res | (size_t)a.ldr * es) % 16 == 0);
+  p.tma_edge = (size_t)a.n * es % 16 == 0;
+  if (p.tma_y) {
+    if (!make_map(&ym, y, es, a.m, a.n, ldy, 32)) return cudaErrorInvalidValue;
+    if (RES && !make_map(&rm, a.res, es, a.m, a.n, a.ldr, 32)) return cudaErrorInvalidValue;
+  }
+  const auto kernel = fp8_linear_pair_kernel<OUT, RES>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
   if (e != cudaSuccess) return e;
   const long tiles = (long)p.m_tiles * p.n_tiles;
-  const int sms = num_sms();
-  if (sms <= 0) return cudaErrorInvalidDevice;
-  kernel<<<(unsigned)(tiles < sms ? tiles : sms), S::THREADS, S::SMEM, st>>>(xm, wm, p);
+  const int pairs = num_sms() / 2;
+  if (pairs <= 0) return cudaErrorInvalidDevice;
+  kernel<<<2 * (unsigned)(tiles < pairs ? tiles : pairs), PAIR_THREADS, S::SMEM, st>>>(xm, wm, p.tma_y ? ym : xm,
+                                                                                       p.tma_y && RES ? rm : xm, p);
   return cudaGetLastError();
-}
-
-template <int OUT>
-static cudaError_t launch_out(const Fp8Linear& a, int* err, cudaStream_t st) {
-  const long rows = (a.m + TM - 1) / TM;
-  const int sms = num_sms();
-  if (rows * ((a.n + 255) / 256) >= sms) return launch_tc<256, OUT>(a, err, st);
-  if constexpr (OUT != FP8_E4M3) {
-    if (rows * ((a.n + 127) / 128) < sms / 2) return launch_tc<64, OUT>(a, err, st);
-  }
-  return launch_tc<128, OUT>(a, err, st);
 }
 
 cudaError_t launch_fp8_linear(const Fp8Linear& a, int* err, cudaStream_t st) {
   if (a.m == 0) return cudaSuccess;
-  if (a.y_type == FP8_F32) return launch_out<FP8_F32>(a, err, st);
-  if (a.y_type == FP8_BF16) return launch_out<FP8_BF16>(a, err, st);
-  return launch_out<FP8_E4M3>(a, err, st);
+  if (a.y_type == FP8_E4M3) return launch_pair<FP8_E4M3, false>(a, err, st);
+  if (a.y_type == FP8_F32) return a.res ? launch_pair<FP8_F32, true>(a, err, st) : launch_pair<FP8_F32, false>(a, err, st);
+  return a.res ? launch_pair<FP8_BF16, true>(a, err, st) : launch_pair<FP8_BF16, false>(a, err, st);
 }
 
 cudaError_t fp8_take_wait_error(int* err, cudaStream_t st) {

@@ -24,7 +24,13 @@ __device__ __forceinline__ uint32_t finite_bits(float v) {
   const uint32_t u = __float_as_uint(v) & 0x7FFFFFFFu;
   return u < 0x7F800000u ? u : 0u;
 }
-// four scaled values to e4m3, infinities (which the conversion would saturate) as NaN
+// four finite or NaN values, scaled, to e4m3
+__device__ __forceinline__ uint32_t e4m3x4_finite(float a, float b, float c, float d, float inv) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * inv, d * inv), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+// the same with infinities (which the conversion would saturate) as NaN
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d, float inv) {
   const float s[4] = {a * inv, b * inv, c * inv, d * inv};
   uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(s[0], s[1]), __NV_SATFINITE, __NV_E4M3);

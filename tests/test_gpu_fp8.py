@@ -188,7 +188,7 @@ def test_linear_far_apart_scales(kk):
 
 
 @pytest.mark.parametrize("m, n, k", [(1, 130, 200), (20, 300, 514), (150, 300, 514)])
-@pytest.mark.parametrize("ldy_pad, off", [(1, 0), (2, 1), (4, 4), (8, 0), (0, 3)])
+@pytest.mark.parametrize("ldy_pad, off", [(1, 0), (2, 1), (4, 4), (8, 0), (0, 3), (6, 0), (4, 0)])
 def test_linear_any_strides_and_offsets(kk, m, n, k, ldy_pad, off):
     """Result and residual rows at strides and offsets of every alignment; nothing is written beside them."""
     rng = np.random.default_rng(m + n + ldy_pad)
