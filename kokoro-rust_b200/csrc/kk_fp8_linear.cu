@@ -57,8 +57,14 @@ __device__ __forceinline__ void mma_mxf8_pair(uint32_t tmem_d, uint64_t a, uint6
       "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tmem_cp_scales_pair(uint32_t taddr, uint32_t saddr) {
-  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc(saddr, 128, 128)) : "memory");
+__device__ __forceinline__ void tmem_cp_scales_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// true on one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 // arrives on the barrier at this offset in both CTAs once the pair's MMAs so far are done
 __device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
@@ -139,7 +145,7 @@ struct TcFp8Args {
 // L2 per SM and clock at the full MMA rate, more than L2 gives; a pair shares the 256 rows of W (each CTA loads
 // and holds half of them), which takes 64.
 constexpr int TM = 128, TN = 256;  // a CTA's rows, the pair's columns
-constexpr int SF_RING = 2;         // scale groups (4 blocks of K each) in shared memory and TMEM
+constexpr int SF_RING = 4;         // scale groups (4 blocks of K each) in shared memory and TMEM
 constexpr int EPI_WARPS = 8;       // two per TMEM lane quarter, 128 columns each
 constexpr int PAIR_THREADS = 32 * (4 + EPI_WARPS);
 constexpr int BOX = 4096;          // 32 rows of 128 bytes: what an epilogue warp stores (or loads) at once
@@ -150,8 +156,8 @@ struct PairShape {
   static constexpr int NBUF = RES ? 2 : 1;  // boxes of an epilogue warp; two, so that a residual is loaded ahead
   static constexpr int A_BYTES = TM * 128, B_BYTES = TN / 2 * 128;
   static constexpr int SF_BYTES = 512 * 3;
-  // TMEM columns: the two accumulators share columns 224..255 (see the epilogue); scales behind them
-  static constexpr int D1 = 224, SF_COL = D1 + TN, SF_COLS = 12;
+  // TMEM columns: the two accumulators share columns 192..255 (see the epilogue); scales behind them
+  static constexpr int D1 = 192, SF_COL = D1 + TN, SF_COLS = 12;
   static constexpr int OFF_B = STAGES * A_BYTES, OFF_BOX = OFF_B + STAGES * B_BYTES;
   static constexpr int OFF_SF = OFF_BOX + EPI_WARPS * NBUF * BOX, OFF_BIAS = OFF_SF + SF_RING * SF_BYTES;
   static constexpr int OFF_BAR = OFF_BIAS + EPI_WARPS * 128 * 4;
@@ -217,6 +223,16 @@ __device__ __forceinline__ int quantize_block(const float* v, uint32_t* u) {
   return e;
 }
 
+__device__ __forceinline__ float4 load_bias(const Fp8Linear& a, long c) {
+  float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (!a.bias) return b;
+  if (c < a.n) b.x = a.bias[c];
+  if (c + 1 < a.n) b.y = a.bias[c + 1];
+  if (c + 2 < a.n) b.z = a.bias[c + 2];
+  if (c + 3 < a.n) b.w = a.bias[c + 3];
+  return b;
+}
+
 __device__ __forceinline__ void add_bias32(float* v, const float* bias_s) {
 #pragma unroll
   for (int j = 0; j < 32; j += 4) {
@@ -229,9 +245,9 @@ __device__ __forceinline__ void add_bias32(float* v, const float* bias_s) {
 // first), so that the tiles of a wave share few rows of x and of W in L2.
 __device__ __forceinline__ void tile_at(const TcFp8Args& p, int t, int* mt, int* nt) {
   constexpr int G = 8;
-  const int per = G * p.n_tiles, g = t / per, r = t - g * per;
-  const int h = min(G, p.m_tiles - g * G);
-  *nt = r / h;
+  const unsigned per = G * p.n_tiles, g = (unsigned)t / per, r = t - g * per;
+  const unsigned h = min(G, p.m_tiles - (int)g * G);
+  *nt = h == G ? r / G : r / h;
   *mt = g * G + (r - *nt * h);
 }
 
@@ -280,15 +296,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      uint32_t it = 0;
+      uint32_t it = 0, s = 0, ph = 1;  // ph: of the wait for the stage's last use
       bool ok = true;
       for (int t = first; ok && t < tiles; t += step) {
         int mt, nt;
         tile_at(p, t, &mt, &nt);
         const int m0 = mt * 2 * TM + (int)rank * TM, n0 = nt * TN + (int)rank * (TN / 2);
         for (int b = 0; b < kb; b++, it++) {
-          const uint32_t s = it % S::STAGES;
-          if (it >= S::STAGES && !mbar_wait(empty + s, (it / S::STAGES + 1) & 1, abort_flag, err)) {
+          if (it >= S::STAGES && !mbar_wait(empty + s, ph, abort_flag, err)) {
             ok = false;
             break;
           }
@@ -296,6 +311,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
           const uint32_t bar = map_rank(full + s, 0);
           tma_load_2d_pair(smem + s * S::A_BYTES, &xmap, b * 128, m0, bar);
           tma_load_2d_pair(smem + S::OFF_B + s * S::B_BYTES, &wmap, b * 128, n0, bar);
+          if (++s == S::STAGES) s = 0, ph ^= 1;
         }
       }
       // After an expired wait, loads still in flight land before the shared memory goes: the first CTA sees them
@@ -311,46 +327,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      uint32_t it = 0, g = 0, tile_n = 0;
-      bool ok = true;
+    if (rank == 0) {
+      // The whole warp runs this loop, so that its control flow and addresses stay uniform, and one elected lane
+      // issues. What the loop does for each block of K (a wait, four MMAs, a commit) has to take less than the
+      // block's 512 MMA cycles: with one divergent lane it took 870.
+      const bool lead = elect_one();
+      const uint64_t da0 = sdesc_sw128(smem_u32(smem)), db0 = sdesc_sw128(smem_u32(smem + S::OFF_B));
+      const uint64_t dsf0 = sdesc(smem_u32(smem + S::OFF_SF), 128, 128);
+      uint32_t s = 0, ph = 0, slot = 0, sph = 0, tile_n = 0, last = 0, last_ph = 0;
+      bool ok = true, issued = false;
       for (int t = first; ok && t < tiles; t += step, tile_n++) {
         if (tile_n > 0 && !mbar_wait_cluster(acc_free, (tile_n - 1) & 1, abort_flag, err)) break;
         tc_fence_after();
         const uint32_t d = tmem + (tile_n & 1) * S::D1;
-        for (int b = 0; b < kb; b++, it++) {
-          const uint32_t slot = g % SF_RING, sfa = tmem + S::SF_COL + slot * S::SF_COLS, sfb = sfa + 4;
-          if ((b & 3) == 0) {
-            if (!mbar_wait_cluster(sf_full + slot, (g / SF_RING) & 1, abort_flag, err)) {
-              ok = false;
-              break;
-            }
-            const uint32_t sf = smem_u32(smem + S::OFF_SF + slot * S::SF_BYTES);
-            tmem_cp_scales_pair(sfa, sf);
-            tmem_cp_scales_pair(sfb, sf + 512);
-            tmem_cp_scales_pair(sfb + 4, sf + 1024);
+        for (int b0 = 0; ok && b0 < kb; b0 += 4) {
+          const uint32_t sfa = tmem + S::SF_COL + slot * S::SF_COLS;
+          ok = mbar_wait_cluster(sf_full + slot, sph, abort_flag, err);
+          if (!ok) break;
+          if (lead) {
+            const uint64_t dsf = dsf0 + slot * (S::SF_BYTES >> 4);
+            tmem_cp_scales_pair(sfa, dsf);
+            tmem_cp_scales_pair(sfa + 4, dsf + (512 >> 4));
+            tmem_cp_scales_pair(sfa + 8, dsf + (1024 >> 4));
           }
-          const uint32_t s = it % S::STAGES;
-          if (!mbar_wait_cluster(full + s, (it / S::STAGES) & 1, abort_flag, err)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint64_t da = sdesc_sw128(smem_u32(smem + s * S::A_BYTES));
-          const uint64_t db = sdesc_sw128(smem_u32(smem + S::OFF_B + s * S::B_BYTES));
-          const uint32_t id = idesc_mxf8(2 * TM, TN, b & 3);
 #pragma unroll
-          for (int k = 0; k < 4; k++) mma_mxf8_pair(d, da + 2 * k, db + 2 * k, id, sfa, sfb, b > 0 || k > 0);
-          mma_commit_pair(empty + s);
-          if ((b & 3) == 3 || b == kb - 1) {
-            mma_commit_pair(sf_empty + slot);
-            g++;
+          for (int j = 0; j < 4; j++) {
+            if (b0 + j >= kb) break;
+            ok = mbar_wait_cluster(full + s, ph, abort_flag, err);
+            if (!ok) break;
+            tc_fence_after();
+            if (lead) {
+              const uint64_t da = da0 + s * (S::A_BYTES >> 4), db = db0 + s * (S::B_BYTES >> 4);
+#pragma unroll
+              for (int k = 0; k < 4; k++)
+                mma_mxf8_pair(d, da + 2 * k, db + 2 * k, idesc_mxf8(2 * TM, TN, j), sfa, sfa + 4, j > 0 || k > 0 || b0 > 0);
+              mma_commit_pair(empty + s);
+            }
+            issued = true, last = s, last_ph = ph;
+            if (++s == S::STAGES) s = 0, ph ^= 1;
           }
+          if (ok && lead) mma_commit_pair(sf_empty + slot);
+          if (++slot == SF_RING) slot = 0, sph ^= 1;
         }
-        if (ok) mma_commit_pair(acc_full);
+        if (ok && lead) mma_commit_pair(acc_full);
       }
-      if (*abort_flag && it > 0)  // MMAs still in flight end before their operands and TMEM go
-        mbar_drain(empty + (it - 1) % S::STAGES, ((it - 1) / S::STAGES) & 1);
+      if (*abort_flag && issued) mbar_drain(empty + last, last_ph);  // MMAs in flight end before their operands and TMEM go
     }
   } else if (warp == 2) {
     uint32_t g = 0;
@@ -395,21 +416,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     constexpr int NCH = 128 / BC;
     uint32_t tile_n = 0, nres = 0;
     bool ok = true;
+    float4 bias_r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (first < tiles) {
+      int mt, nt;
+      tile_at(p, first, &mt, &nt);
+      bias_r = load_bias(a, (long)nt * TN + half * 128 + 4 * lane);
+    }
     for (int t = first; ok && t < tiles; t += step, tile_n++) {
       int mt, nt;
       tile_at(p, t, &mt, &nt);
       const long r0 = (long)mt * 2 * TM + rank * TM + (ew & 3) * 32;
       const long c0 = (long)nt * TN + half * 128;
       // The next tile's accumulator may be written once the columns that it shares with this one are read: the last
-      // 32 of the first accumulator are the first 32 of the second; the half that holds them reads them first. (The
+      // 64 of the first accumulator are the first 64 of the second; the half that holds them reads them first. (The
       // tile after next reuses all of this accumulator: it waits for the next tile's arrivals, which come after all
       // of this tile's reads.)
       const bool shares = half == (int)(1 - (tile_n & 1));
-      const int ch0 = shares && half == 1 ? NCH - 1 : 0;
+      const int ch0 = !shares || half == 0 ? 0 : (BC == 32 ? 2 : NCH - 1);
       // boxes with columns, and how many of them go by TMA
       const int live = r0 < a.m && c0 < a.n ? (int)min((long)NCH, (a.n - c0 + BC - 1) / BC) : 0;
       const int boxes = !p.tma_y || live == 0 ? 0 : (p.tma_edge ? live : (int)min((long)live, (a.n - c0) / BC));
-      // the boxes in the order of their use: ch0, then the others from 0 (NCH 2 or 4, ch0 0 or NCH - 1)
+      // (boxes are used in the order ch0, ch0 + 1, .. round to ch0 - 1)
       if constexpr (RES) {
         // the first boxes' residuals, while the tile's MMAs run; a box is free once its last store has read it
         if (boxes > 0 && lane == 0) {
@@ -426,8 +453,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         }
       }
       __syncwarp();
-      for (int i = lane; i < 128; i += 32) bias_s[i] = a.bias && c0 + i < a.n ? a.bias[c0 + i] : 0.0f;
+      *reinterpret_cast<float4*>(bias_s + 4 * lane) = bias_r;
       __syncwarp();
+      if (t + step < tiles) {  // the next tile's, which arrives during this one
+        int mt1, nt1;
+        tile_at(p, t + step, &mt1, &nt1);
+        bias_r = load_bias(a, (long)nt1 * TN + half * 128 + 4 * lane);
+      }
       ok = __all_sync(0xFFFFFFFFu, mbar_wait(acc_full, tile_n & 1, abort_flag, err));
       if (!ok) break;
       tc_fence_after();
@@ -490,12 +522,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
           }
 #pragma unroll
           for (int h = 0; h < BC / 32; h++) {
-            // (the shared columns are the last 32 of this box when it is read out of order: read the box backwards)
-            const int hh = ch0 != 0 ? BC / 32 - 1 - h : h;
-            const int c = ch * BC + 32 * hh;
+            const int c = ch * BC + 32 * h;
             float v[32];
             tmem_ld32(d + c, v);
-            if (shares && i == 0 && h == 0) {
+            if (shares && (BC == 32 ? i == 1 : i == 0 && h == 1)) {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive_cluster(acc_free0);
@@ -529,7 +559,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             } else {
 #pragma unroll
               for (int q = 0; q < 4; q++) {
-                const uint32_t at = row_b + (((4 * hh + q) ^ (lane & 7)) << 4);
+                const uint32_t at = row_b + (((4 * h + q) ^ (lane & 7)) << 4);
                 if constexpr (RES) {
                   const float4 r = lds_f4(at);
                   const uint32_t u[4] = {__float_as_uint(r.x), __float_as_uint(r.y), __float_as_uint(r.z), __float_as_uint(r.w)};
