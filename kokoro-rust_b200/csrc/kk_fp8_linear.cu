@@ -42,8 +42,8 @@ __device__ __forceinline__ void mma_mxf8(uint32_t tmem_d, uint64_t a, uint64_t b
 }
 // 32 lanes x 16 bytes of shared memory (512 contiguous bytes) to four TMEM columns, in all four lane quarters:
 // word w of lane l is the scale word of row 32 w + l.
-__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint32_t saddr) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc(saddr, 128, 128)) : "memory");
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 // ---- the same over a pair of CTAs (cta_group::2): the MMA is issued by the pair's first CTA and reads both
@@ -620,6 +620,289 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
   }
 }
 
+// ---- small layers: one CTA per tile of 128 rows x NT columns and share of K
+//
+// With few rows the weights are all there is to read, and what counts is that every SM reads some of them and that
+// nothing is waited for twice: K is split over the CTAs of a cluster until the tiles fill the machine, each CTA
+// starts its loads before anything else, and the shares are summed through the cluster's shared memory (in the
+// order of the shares, so the result does not vary).
+constexpr int SPLIT_THREADS = 256;
+constexpr int SPLIT_RING = 8;          // scale groups held
+constexpr int SPLIT_STAGES = 8;        // at most
+constexpr int SPLIT_BUDGET = 96 << 10; // shared memory for the stages: two CTAs fit an SM
+
+struct SplitArgs {
+  Fp8Linear a;
+  int* err;
+  int kb, n_tiles;
+  int splits;       // CTAs of a cluster
+  int stages;
+  int box_rows;     // rows of x of a tile that are loaded (a multiple of 8)
+  int vec_y, vec_res;
+};
+
+template <int NT>
+struct SplitShape {
+  static constexpr int NB = (NT + 127) / 128;
+  static constexpr int SF_BYTES = 512 * (1 + NB);
+  static constexpr int SF_COLS = 4 * (1 + NB);
+  static constexpr int TMEM_COLS = NT + SPLIT_RING * SF_COLS <= 128 ? 128 : 256;
+  static constexpr int PITCH = NT + 4;  // of a partial row, in floats: a warp's 16-byte stores hit every bank once
+  static_assert(NT + SPLIT_RING * SF_COLS <= TMEM_COLS, "TMEM columns");
+};
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+
+template <int NT, int OUT>
+__global__ void __launch_bounds__(SPLIT_THREADS, 2)
+    fp8_linear_split_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
+                            const __grid_constant__ SplitArgs p) {
+  using S = SplitShape<NT>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full[SPLIT_STAGES], empty[SPLIT_STAGES], sf_full[SPLIT_RING], sf_empty[SPLIT_RING], acc_full;
+  __shared__ __align__(16) uint8_t sf_s[SPLIT_RING * S::SF_BYTES];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_s;
+  volatile int* abort_flag = &abort_s;
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const Fp8Linear& a = p.a;
+  int* err = p.err ? p.err : &g_fp8_wait_error;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int splits = p.splits, share = blockIdx.x % splits, tile = blockIdx.x / splits;
+  const long m0 = (long)(tile / p.n_tiles) * TM, n0 = (long)(tile % p.n_tiles) * NT;
+  const int b_lo = (int)((long)p.kb * share / splits), b_hi = (int)((long)p.kb * (share + 1) / splits);
+  const int a_bytes = p.box_rows * 128, stage = a_bytes + NT * 128;
+  const int rows = (int)min((long)TM, a.m - m0);
+
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < SPLIT_STAGES; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
+    for (int i = 0; i < SPLIT_RING; i++) mbar_init(sf_full + i, 1), mbar_init(sf_empty + i, 1);
+    mbar_init(&acc_full, 1);
+    abort_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    // the first stages' loads are under way while the rest is set up
+    for (int b = b_lo; b < b_hi && b - b_lo < p.stages; b++) {
+      const int s = b - b_lo;
+      mbar_arrive_expect_tx(full + s, stage);
+      tma_load_2d(smem + s * stage + a_bytes, &wmap, b * 128, (int)n0, full + s);
+      tma_load_2d(smem + s * stage, &xmap, b * 128, (int)m0, full + s);
+    }
+  } else if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                 "n"(S::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  // what the epilogue adds, on its way while the MMAs run: a thread's units of 4 columns all lie in the same columns
+  constexpr int UNITS = NT / 4;
+  const int c = (int)(threadIdx.x % UNITS) * 4;
+  float bias_r[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) bias_r[i] = a.bias && n0 + c + i < a.n ? a.bias[n0 + c + i] : 0.0f;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      int b = b_lo + p.stages, s = 0, ph = 0;
+      for (; b < b_hi; b++) {
+        if (!mbar_wait(empty + s, ph, abort_flag, err)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(full + s, stage);
+        tma_load_2d(smem + s * stage + a_bytes, &wmap, b * 128, (int)n0, full + s);
+        tma_load_2d(smem + s * stage, &xmap, b * 128, (int)m0, full + s);
+        if (++s == p.stages) s = 0, ph ^= 1;
+      }
+      if (!ok)  // loads in flight land before the shared memory goes
+        for (int i = max(b_lo, b - p.stages); i < b; i++)
+          mbar_drain(full + (i - b_lo) % p.stages, ((i - b_lo) / p.stages) & 1);
+    }
+  } else if (warp == 1) {
+    const bool lead = elect_one();
+    const uint64_t d0 = sdesc_sw128(smem_u32(smem)), dsf0 = sdesc(smem_u32(sf_s), 128, 128);
+    int s = 0, ph = 0, slot = -1, sph = 0, last = -1, last_ph = 0;
+    bool ok = true;
+    uint32_t sfa = 0;
+    for (int b = b_lo; b < b_hi; b++) {
+      if ((b & 3) == 0 || b == b_lo) {
+        if (slot >= 0 && lead) mma_commit(sf_empty + slot);
+        if (++slot == SPLIT_RING) slot = 0, sph ^= 1;
+        ok = mbar_wait(sf_full + slot, sph, abort_flag, err);
+        if (!ok) break;
+        sfa = tmem + NT + slot * S::SF_COLS;
+        if (lead) {
+#pragma unroll
+          for (int i = 0; i < 1 + S::NB; i++)
+            tmem_cp_scales(sfa + 4 * i, dsf0 + ((slot * S::SF_BYTES + 512 * i) >> 4));
+        }
+      }
+      ok = mbar_wait(full + s, ph, abort_flag, err);
+      if (!ok) break;
+      tc_fence_after();
+      if (lead) {
+        const uint64_t da = d0 + ((s * stage) >> 4), db = da + (a_bytes >> 4);
+        const uint32_t id = idesc_mxf8(TM, NT, 0) | ((uint32_t)(b & 3) << 4) | ((uint32_t)(b & 3) << 29);
+#pragma unroll
+        for (int k = 0; k < 4; k++) mma_mxf8(tmem, da + 2 * k, db + 2 * k, id, sfa, sfa + 4, b > b_lo || k > 0);
+        mma_commit(empty + s);
+      }
+      last = s, last_ph = ph;
+      if (++s == p.stages) s = 0, ph ^= 1;
+    }
+    if (ok && lead) mma_commit(&acc_full);
+    if (!ok && last >= 0) mbar_drain(empty + last, last_ph);  // MMAs in flight end before their operands and TMEM go
+  } else if (warp == 2) {
+    int slot = 0, ph = 1, n = 0;
+    for (int b = b_lo & ~3; b < b_hi; b += 4, n++) {
+      uint32_t wx[4], ww[S::NB][4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int r = 32 * i + lane;
+        wx[i] = r < rows ? *reinterpret_cast<const uint32_t*>(a.x.e + (m0 + r) * a.x.lde + b) : 0u;
+#pragma unroll
+        for (int j = 0; j < S::NB; j++) {
+          const long cc = n0 + 128 * j + 32 * i;
+          ww[j][i] = cc < a.n ? *reinterpret_cast<const uint32_t*>(a.w.e + (cc >> 7) * a.w.lde + b) : 0u;
+        }
+      }
+      if (n >= SPLIT_RING && !__all_sync(0xFFFFFFFFu, mbar_wait(sf_empty + slot, ph, abort_flag, err))) break;
+      const uint32_t sf = smem_u32(sf_s) + slot * S::SF_BYTES + lane * 16;
+      sts_u4(sf, make_uint4(wx[0], wx[1], wx[2], wx[3]));
+#pragma unroll
+      for (int j = 0; j < S::NB; j++) sts_u4(sf + 512 * (1 + j), make_uint4(ww[j][0], ww[j][1], ww[j][2], ww[j][3]));
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sf_full + slot);
+      if (++slot == SPLIT_RING) slot = 0, ph ^= 1;
+    }
+  } else if (warp >= 4) {
+    const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(&acc_full, 0, abort_flag, err));
+    tc_fence_after();
+    const int q = warp & 3, r = 32 * q + lane;
+    if (ok && 32 * q < rows) {  // the stages' memory is free now: the MMAs that read it are done
+      const uint32_t row_s = smem_u32(smem) + r * S::PITCH * 4;
+#pragma unroll
+      for (int i = 0; i < NT / 32; i++) {
+        float v[32];
+        tmem_ld32(tmem + ((uint32_t)q << 21) + 32 * i, v);
+        if (r < rows) {
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            sts_u4(row_s + 128 * i + 16 * j, make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                                                        __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])));
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncwarp();
+  __syncthreads();
+  if (splits > 1) cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::TMEM_COLS));
+  }
+  const bool done = *abort_flag == 0;
+  for (int u = share * SPLIT_THREADS + threadIdx.x; done && u < rows * UNITS; u += splits * SPLIT_THREADS) {
+    const int r = u / UNITS;
+    const long m = m0 + r, n = n0 + c;
+    float res_r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (OUT != FP8_E4M3 && a.res) {
+      if (OUT == FP8_F32) {
+        const float* rr = (const float*)a.res + m * a.ldr + n;
+        if (p.vec_res && n + 4 <= a.n) {
+          const float4 f = *reinterpret_cast<const float4*>(rr);
+          res_r[0] = f.x, res_r[1] = f.y, res_r[2] = f.z, res_r[3] = f.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (n + i < a.n) res_r[i] = rr[i];
+        }
+      } else {
+        const __nv_bfloat16* rr = (const __nv_bfloat16*)a.res + m * a.ldr + n;
+        if (p.vec_res && n + 4 <= a.n) {
+          const uint2 f = *reinterpret_cast<const uint2*>(rr);
+          res_r[0] = __uint_as_float(f.x << 16), res_r[1] = __uint_as_float(f.x & 0xFFFF0000u);
+          res_r[2] = __uint_as_float(f.y << 16), res_r[3] = __uint_as_float(f.y & 0xFFFF0000u);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (n + i < a.n) res_r[i] = (float)rr[i];
+        }
+      }
+    }
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const float* part = (const float*)smem + r * S::PITCH + c;
+    if (splits == 1) {
+      const float4 f = *reinterpret_cast<const float4*>(part);
+      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    } else {
+      float4 f[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (i < splits) f[i] = ld_cluster_f4(map_rank(part, i));
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (i < splits) v[0] += f[i].x, v[1] += f[i].y, v[2] += f[i].z, v[3] += f[i].w;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      v[i] += bias_r[i];
+      if (a.gelu) v[i] = gelu_fast(v[i]);
+      if (OUT != FP8_E4M3) v[i] += res_r[i];
+    }
+    if constexpr (OUT == FP8_F32) {
+      float* y = (float*)a.y + m * a.ldy + n;
+      if (p.vec_y && n + 4 <= a.n) {
+        *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (n + i < a.n) y[i] = v[i];
+      }
+    } else if constexpr (OUT == FP8_BF16) {
+      __nv_bfloat16* y = (__nv_bfloat16*)a.y + m * a.ldy + n;
+      if (p.vec_y && n + 4 <= a.n) {
+        *reinterpret_cast<uint2*>(y) = make_uint2(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (n + i < a.n) y[i] = __float2bfloat16(v[i]);
+      }
+    } else {
+      // a warp holds the 128 columns of a row: one block (columns past n count for nothing and are not stored)
+      uint32_t mx = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (n + i < a.n) mx = max(mx, finite_bits(v[i]));
+      mx = __reduce_max_sync(0xFFFFFFFFu, mx);
+      const int e = fp8_exp(mx);
+      const uint32_t w = e4m3x4(v[0], v[1], v[2], v[3], fp8_inv_scale(e));
+      uint8_t* q = a.q.v + m * a.q.ldv + n;
+      if (n + 4 <= a.n) {
+        *reinterpret_cast<uint32_t*>(q) = w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (n + i < a.n) q[i] = (uint8_t)(w >> (8 * i));
+      }
+      if (lane == 0) a.q.e[m * a.q.lde + (n >> 7)] = (uint8_t)e;
+    }
+  }
+  __syncwarp();
+  if (splits > 1) cluster_sync();  // the others have read this CTA's share
+}
+
 // ---- host side
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -700,11 +983,73 @@ static cudaError_t launch_pair(const Fp8Linear& a, int* err, cudaStream_t st) {
   return cudaGetLastError();
 }
 
+template <int NT, int OUT>
+static cudaError_t launch_split(const Fp8Linear& a, int splits, int* err, cudaStream_t st) {
+  using S = SplitShape<NT>;
+  SplitArgs p;
+  p.a = a;
+  p.err = err;
+  p.kb = (int)((a.k + 127) / 128);
+  p.n_tiles = (int)((a.n + NT - 1) / NT);
+  p.splits = splits;
+  p.box_rows = (int)(a.m < TM ? (a.m + 7) / 8 * 8 : TM);
+  const int stage = (p.box_rows + NT) * 128;
+  const int share = (p.kb + splits - 1) / splits;
+  // an MMA reads 128 rows of x wherever its box starts, so the last stage is followed by what that may take
+  const int tail = stage < TM * 128 ? TM * 128 - stage : 0;
+  p.stages = (SPLIT_BUDGET - tail) / stage;
+  if (p.stages > SPLIT_STAGES) p.stages = SPLIT_STAGES;
+  if (p.stages > share) p.stages = share;
+  const size_t es = OUT == FP8_F32 ? 4 : 2;
+  p.vec_y = ((uintptr_t)a.y | a.ldy * es) % (4 * es) == 0;
+  p.vec_res = ((uintptr_t)a.res | a.ldr * es) % (4 * es) == 0;
+  CUtensorMap xm, wm;
+  if (!make_map(&xm, a.x.v, 1, a.m, a.k, a.x.ldv, p.box_rows) || !make_map(&wm, a.w.v, 1, a.n, a.k, a.w.ldv, NT))
+    return cudaErrorInvalidValue;
+  const int partial = p.box_rows * S::PITCH * 4;  // takes the stages' place
+  int smem = p.stages * stage + tail;
+  if (smem < partial) smem = partial;
+  smem += 1024;
+  const auto kernel = fp8_linear_split_kernel<NT, OUT>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SPLIT_BUDGET + 1024);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((a.m + TM - 1) / TM * p.n_tiles * splits));
+  cfg.blockDim = dim3(SPLIT_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = splits, at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, xm, wm, p);
+}
+
+template <int OUT>
+static cudaError_t launch_out(const Fp8Linear& a, int* err, cudaStream_t st) {
+  const int sms = num_sms();
+  if (sms <= 0) return cudaErrorInvalidDevice;
+  const long rows = (a.m + TM - 1) / TM, t128 = rows * ((a.n + 127) / 128);
+  if (t128 <= 2 * sms) {
+    const int kb = (int)((a.k + 127) / 128);
+    const long t64 = rows * ((a.n + 63) / 64);
+    const bool narrow = OUT != FP8_E4M3 && t64 <= sms;
+    const long tiles = narrow ? t64 : t128;
+    int splits = 1;
+    while (splits < 8 && 2 * splits <= kb && tiles * 2 * splits <= 2 * sms) splits *= 2;
+    if constexpr (OUT != FP8_E4M3)
+      if (narrow) return launch_split<64, OUT>(a, splits, err, st);
+    return launch_split<128, OUT>(a, splits, err, st);
+  }
+  if constexpr (OUT == FP8_E4M3) return launch_pair<OUT, false>(a, err, st);
+  return a.res ? launch_pair<OUT, OUT != FP8_E4M3>(a, err, st) : launch_pair<OUT, false>(a, err, st);
+}
+
 cudaError_t launch_fp8_linear(const Fp8Linear& a, int* err, cudaStream_t st) {
   if (a.m == 0) return cudaSuccess;
-  if (a.y_type == FP8_E4M3) return launch_pair<FP8_E4M3, false>(a, err, st);
-  if (a.y_type == FP8_F32) return a.res ? launch_pair<FP8_F32, true>(a, err, st) : launch_pair<FP8_F32, false>(a, err, st);
-  return a.res ? launch_pair<FP8_BF16, true>(a, err, st) : launch_pair<FP8_BF16, false>(a, err, st);
+  if (a.y_type == FP8_E4M3) return launch_out<FP8_E4M3>(a, err, st);
+  return a.y_type == FP8_F32 ? launch_out<FP8_F32>(a, err, st) : launch_out<FP8_BF16>(a, err, st);
 }
 
 cudaError_t fp8_take_wait_error(int* err, cudaStream_t st) {

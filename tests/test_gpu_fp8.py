@@ -141,7 +141,8 @@ def check_linear(got, y, S, rms, K, act, dtype):
 
 SIZES = [(1, 1, 1), (1, 16, 128), (1, 768, 768), (2, 130, 100), (7, 128, 129), (16, 2304, 768), (17, 50, 512), (33, 257, 300),
          (64, 512, 768), (65, 96, 640), (66, 2048, 768), (128, 768, 2048), (129, 255, 16), (200, 1090, 514), (300, 769, 1100),
-         (512, 768, 2048), (700, 640, 520), (4800, 1000, 384), (9501, 513, 640), (2600, 2304, 768)]
+         (512, 768, 2048), (700, 640, 520), (4800, 1000, 384), (9501, 513, 640), (2600, 2304, 768),
+         (3, 20000, 4700), (140, 1000, 2500)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, E4M3])
