@@ -3,136 +3,287 @@
 //
 // Block of 128 columns of one row (activations) or 128 x 128 (weights), a = max |x| over its finite
 // values: E is the smallest integer >= 0 with a <= 448 * 2^(E - 127) (448 is e4m3's largest value), and
-// the block is held as e4m3(x * 2^(127 - E)), rounded to nearest even; infinities and NaN are held as
-// NaN. A power of two scales exactly, so a value is rounded once and does not depend on the order or
-// precision of anything; against a * 2^-.. / 448 it gives up at most one binade of e4m3's range (15
-// binades of normal numbers), and it is the scale format the tensor core applies by itself.
+// the block is held as e4m3(x * 2^(127 - E)), rounded to nearest even (off by at most 2^-4 of the value);
+// infinities and NaN are held as NaN. A power of two scales exactly, so a value is rounded once and does not
+// depend on the order or precision of anything; against a scale of a / 448 it gives up at most one binade of
+// e4m3's 17, and it is the scale format the tensor core applies by itself.
+//
+// All of it is bound by HBM: each kernel reads and writes each byte once, 16 bytes a lane on its 16- or 32-bit
+// side, with several loads in flight before the first is used.
 #include "kk_fp8.h"
 #include "kk_fp8_math.cuh"
 
 namespace kk {
 
-// columns c .. c + 3 of a row (nothing past k: 0); VEC: one aligned load of the four
+// A lane's part of a row. The quantisers take 8 columns a lane, 16 lanes a block, whatever the type (their work
+// per block, the maximum and the scale, weighs more than the loads do); the read-back 16 bytes of the result.
+constexpr int QCOLS = 8, QLANES = 128 / QCOLS;
+template <typename T>
+struct Lane {
+  static constexpr int COLS = 16 / (int)sizeof(T);
+  static constexpr int LANES = 128 / COLS;
+};
+template <typename T>
+struct Raw {
+  static constexpr int WORDS = QCOLS * (int)sizeof(T) / 4;
+  uint32_t w[WORDS];
+};
+
+__device__ __forceinline__ void widen(const Raw<float>& u, float (&v)[QCOLS]) {
+#pragma unroll
+  for (int i = 0; i < QCOLS; i++) v[i] = __uint_as_float(u.w[i]);
+}
+__device__ __forceinline__ void widen(const Raw<__nv_bfloat16>& u, float (&v)[QCOLS]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    v[2 * i] = __uint_as_float(u.w[i] << 16), v[2 * i + 1] = __uint_as_float(u.w[i] & 0xFFFF0000u);
+}
+__device__ __forceinline__ uint32_t bits_of(float v) { return __float_as_uint(v); }
+__device__ __forceinline__ uint32_t bits_of(__nv_bfloat16 v) { return (uint32_t)__bfloat16_as_ushort(v); }
+
+// columns c .. c + 7 of a row as raw bits, zeros from column k on; VEC: rows are 16-byte aligned
 template <typename T, bool VEC>
-__device__ __forceinline__ void load4(const T* row, long c, long k, float* v) {
-  if (VEC && c + 4 <= k) {
-    if (sizeof(T) == 4) {
-      const float4 f = *reinterpret_cast<const float4*>(row + c);
-      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(row + c);
-      v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xFFFF0000u);
-      v[2] = __uint_as_float(u.y << 16), v[3] = __uint_as_float(u.y & 0xFFFF0000u);
+__device__ __forceinline__ void load_lane(Raw<T>& u, const T* row, long c, long k) {
+  if (VEC && c + QCOLS <= k) {
+#pragma unroll
+    for (int i = 0; i < Raw<T>::WORDS; i += 4) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(row + c) + i / 4);
+      u.w[i] = q.x, u.w[i + 1] = q.y, u.w[i + 2] = q.z, u.w[i + 3] = q.w;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = c + i < k ? (float)row[c + i] : 0.0f;
+    return;
   }
-}
-// four held values to columns c .. c + 3 (c a multiple of 4), nothing at or past column k
-__device__ __forceinline__ void store_e4m3x4(uint8_t* row, long c, long k, uint32_t u) {
-  if (c + 4 <= k) {
-    *reinterpret_cast<uint32_t*>(row + c) = u;
-  } else {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (c + i < k) row[c + i] = (uint8_t)(u >> (8 * i));
-  }
-}
-
-// One warp per (row, block): a lane holds four columns, the block's maximum is one integer reduction.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const T* x, long ldx, long k, int kb, int units,
-                                                             Fp8Store q) {
-  const int lane = threadIdx.x & 31;
-  const int u = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (u >= units) return;
-  const long r = u / kb;
-  const int b = u - (int)r * kb;
-  const long c = (long)b * 128 + 4 * lane;
-  float v[4];
-  load4<T, VEC>(x + r * ldx, c, k, v);
-  uint32_t m = max(max(finite_bits(v[0]), finite_bits(v[1])), max(finite_bits(v[2]), finite_bits(v[3])));
-  m = __reduce_max_sync(0xFFFFFFFFu, m);
-  const int e = fp8_exp(m);
-  store_e4m3x4(q.v + r * q.ldv, c, k, e4m3x4(v[0], v[1], v[2], v[3], fp8_inv_scale(e)));
-  if (lane == 0) q.e[r * q.lde + b] = (uint8_t)e;
-}
-
-// One CTA per 128 x 128 block, the block in registers between the maximum and the conversion.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) fp8_quant_blocks_kernel(const T* x, long ldx, long rows, long k, int kb,
-                                                               Fp8Store q) {
-  __shared__ uint32_t wmax[8];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long rb = blockIdx.x / kb;
-  const int b = (int)(blockIdx.x - rb * kb);
-  const long r0 = rb * 128 + warp * 16, c = (long)b * 128 + 4 * lane;
-  float v[16][4];
+  for (int i = 0; i < Raw<T>::WORDS; i++) u.w[i] = 0;
 #pragma unroll
-  for (int i = 0; i < 16; i++) {
-    if (r0 + i < rows)
-      load4<T, VEC>(x + (r0 + i) * ldx, c, k, v[i]);
-    else
-      v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.0f;
-  }
+  for (int i = 0; i < QCOLS; i++)
+    if (c + i < k) u.w[i * sizeof(T) / 4] |= bits_of(row[c + i]) << (8 * (i * sizeof(T) % 4));
+}
+template <typename T>
+__device__ __forceinline__ void clear(Raw<T>& u) {
+#pragma unroll
+  for (int i = 0; i < Raw<T>::WORDS; i++) u.w[i] = 0;
+}
+// the largest magnitude of a lane's values as bits, and whether one is infinite (a NaN is passed over)
+template <int N>
+__device__ __forceinline__ uint32_t amax_bits(const float (&v)[N]) {
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; i++) m = fmaxf(m, fabsf(v[i]));
+  return __float_as_uint(m);
+}
+template <int N>
+__device__ __forceinline__ uint32_t amax_finite_bits(const float (&v)[N]) {
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 16; i++)
+  for (int i = 0; i < N; i++) m = max(m, finite_bits(v[i]));
+  return m;
+}
+// maximum over the half warp that holds a block
+__device__ __forceinline__ uint32_t block_max(uint32_t m) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) m = max(m, finite_bits(v[i][j]));
+  for (int o = QLANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  return m;
+}
+// A lane's values held as e4m3, stored at column c, nothing at or past column k.
+template <int N>
+__device__ __forceinline__ void store_lane(uint8_t* row, long c, long k, const float (&v)[N], float inv, bool infinite) {
+  uint32_t u[N / 4];
+#pragma unroll
+  for (int i = 0; i < N / 4; i++)
+    u[i] = infinite ? e4m3x4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv)
+                    : e4m3x4_finite(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv);
+  if (c + N <= k) {
+    if constexpr (N == 4)
+      *reinterpret_cast<uint32_t*>(row + c) = u[0];
+    else
+      *reinterpret_cast<uint2*>(row + c) = make_uint2(u[0], u[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      if (c + i < k) row[c + i] = (uint8_t)(u[i >> 2] >> (8 * (i & 3)));
+  }
+}
+
+// Rows: half a warp per (row, block), U blocks a lane, whose loads are all under way before the first is used.
+template <typename T, bool VEC, int U>
+__global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const T* __restrict__ x, long ldx, long k, unsigned kb,
+                                                             unsigned units, Fp8Store q) {
+  const int lane = threadIdx.x & 31, in = lane % QLANES;
+  const unsigned u0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * (2 * U) + lane / QLANES;
+  Raw<T> raw[U];
+  unsigned r = u0 / kb, b = u0 - r * kb;
+  const unsigned r0 = r, b0 = b;
+#pragma unroll
+  for (int i = 0; i < U; i++) {
+    if (u0 + 2 * i < units)
+      load_lane<T, VEC>(raw[i], x + r * ldx, (long)b * 128 + QCOLS * in, k);
+    else
+      clear(raw[i]);
+    for (b += 2; b >= kb; b -= kb) r++;
+  }
+  r = r0, b = b0;
+#pragma unroll
+  for (int i = 0; i < U; i++) {
+    float v[QCOLS];
+    widen(raw[i], v);
+    uint32_t m = block_max(amax_bits(v));
+    const bool infinite = m == 0x7F800000u;
+    if (__any_sync(0xFFFFFFFFu, infinite)) m = block_max(amax_finite_bits(v));
+    const int e = fp8_exp(m);
+    if (u0 + 2 * i < units) {
+      store_lane<QCOLS>(q.v + r * q.ldv, (long)b * 128 + QCOLS * in, k, v, fp8_inv_scale(e), infinite);
+      if (in == 0) q.e[r * q.lde + b] = (uint8_t)e;
+    }
+    for (b += 2; b >= kb; b -= kb) r++;
+  }
+}
+
+// Weights: one CTA per 128 x 128 block, the block in registers between the maximum and the conversion.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) fp8_quant_blocks_kernel(const T* __restrict__ x, long ldx, long rows, long k,
+                                                               unsigned kb, Fp8Store q) {
+  constexpr int U = 8;  // rows of a lane: 16 to a warp, two at once
+  __shared__ uint32_t wmax[8], wfin[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned rb = blockIdx.x / kb, b = blockIdx.x - rb * kb;
+  const long r0 = (long)rb * 128 + warp * 16 + lane / QLANES, c = (long)b * 128 + QCOLS * (lane % QLANES);
+  Raw<T> raw[U];
+  if (VEC && (long)rb * 128 + 128 <= rows && (long)b * 128 + 128 <= k) {
+#pragma unroll
+    for (int i = 0; i < U; i++) load_lane<T, VEC>(raw[i], x + (r0 + 2 * i) * ldx, c, c + QCOLS);
+  } else {
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+      if (r0 + 2 * i < rows)
+        load_lane<T, VEC>(raw[i], x + (r0 + 2 * i) * ldx, c, k);
+      else
+        clear(raw[i]);
+    }
+  }
+  uint32_t m = 0, f = 0;
+#pragma unroll
+  for (int i = 0; i < U; i++) {
+    float v[QCOLS];
+    widen(raw[i], v);
+    m = max(m, amax_bits(v));
+  }
   m = __reduce_max_sync(0xFFFFFFFFu, m);
   if (lane == 0) wmax[warp] = m;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; i++) m = max(m, wmax[i]);
+  const bool infinite = m == 0x7F800000u;  // the same for the whole CTA
+  if (infinite) {
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+      float v[QCOLS];
+      widen(raw[i], v);
+      f = max(f, amax_finite_bits(v));
+    }
+    f = __reduce_max_sync(0xFFFFFFFFu, f);
+    if (lane == 0) wfin[warp] = f;
+    __syncthreads();
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = max(m, wfin[i]);
+  }
   const int e = fp8_exp(m);
   const float inv = fp8_inv_scale(e);
 #pragma unroll
-  for (int i = 0; i < 16; i++)
-    if (r0 + i < rows) store_e4m3x4(q.v + (r0 + i) * q.ldv, c, k, e4m3x4(v[i][0], v[i][1], v[i][2], v[i][3], inv));
-  if (threadIdx.x == 0) q.e[rb * q.lde + b] = (uint8_t)e;
+  for (int i = 0; i < U; i++) {
+    float v[QCOLS];
+    widen(raw[i], v);
+    if (r0 + 2 * i < rows) store_lane<QCOLS>(q.v + (r0 + 2 * i) * q.ldv, c, k, v, inv, infinite);
+  }
+  if (threadIdx.x == 0) q.e[(long)rb * q.lde + b] = (uint8_t)e;
 }
 
-// One thread per 4 columns: value * 2^(E - 127). The product is exact in 32 bits (4 significant bits);
-// bf16 keeps it exactly too unless it falls below bf16's normal numbers.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) fp8_dequant_kernel(Fp8Store q, long k, int quads, long total, int block_rows,
-                                                          T* y, long ldy) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  const long r = i / quads;
-  const long c = (i - r * quads) * 4;
-  const uint8_t* row = q.v + r * q.ldv;
-  const float s = fp8_scale(q.e[r / block_rows * q.lde + c / 128]);
-  uint32_t u = 0;
-  if (c + 4 <= k) {
-    u = *reinterpret_cast<const uint32_t*>(row + c);
-  } else {
-    for (int j = 0; j < 4; j++)
-      if (c + j < k) u |= (uint32_t)row[c + j] << (8 * j);
-  }
-  float v[4];
-  e4m3x4_to_f32(u, v);
-  T* yr = y + r * ldy;
+// Reading back: value * 2^(E - 127), LANES lanes per block of a row, U blocks a lane. The product is exact in 32 bits
+// (a value has 4 significant bits); bf16 keeps it exactly too unless it falls below bf16's normal numbers.
+template <typename T, bool VEC, int U>
+__global__ void __launch_bounds__(256) fp8_dequant_kernel(Fp8Store q, long k, unsigned kb, unsigned units, int block_shift,
+                                                          T* __restrict__ y, long ldy) {
+  constexpr int N = Lane<T>::COLS, LANES = Lane<T>::LANES, PER = 32 / LANES;
+  const int lane = threadIdx.x & 31, in = lane % LANES;
+  const unsigned u0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * (U * PER) + lane / LANES;
+  uint32_t raw[U][N / 4];
+  int e[U];
+  unsigned r = u0 / kb, b = u0 - r * kb;
+  const unsigned r0 = r, b0 = b;
 #pragma unroll
-  for (int j = 0; j < 4; j++)
-    if (c + j < k) yr[c + j] = (T)(v[j] * s);
+  for (int i = 0; i < U; i++) {
+    e[i] = 0;
+#pragma unroll
+    for (int j = 0; j < N / 4; j++) raw[i][j] = 0;
+    const uint8_t* row = q.v + r * q.ldv;
+    const long c = (long)b * 128 + N * in;
+    const bool on = u0 + i * PER < units;
+    if (on) e[i] = q.e[(long)(r >> block_shift) * q.lde + b];
+    for (b += PER; b >= kb; b -= kb) r++;
+    if (!on) continue;
+    if (c + N <= k) {
+      if constexpr (N == 4) {
+        raw[i][0] = __ldg(reinterpret_cast<const uint32_t*>(row + c));
+      } else {
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(row + c));
+        raw[i][0] = w.x, raw[i][1] = w.y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; j++)
+        if (c + j < k) raw[i][j >> 2] |= (uint32_t)row[c + j] << (8 * (j & 3));
+    }
+  }
+  r = r0, b = b0;
+#pragma unroll
+  for (int i = 0; i < U; i++) {
+    if (u0 + i * PER >= units) break;
+    const long c = (long)b * 128 + N * in;
+    const float s = fp8_scale(e[i]);
+    float v[N];
+#pragma unroll
+    for (int j = 0; j < N / 4; j++) e4m3x4_to_f32(raw[i][j], v + 4 * j);
+#pragma unroll
+    for (int j = 0; j < N; j++) v[j] *= s;
+    T* yr = y + r * ldy;
+    for (b += PER; b >= kb; b -= kb) r++;
+    if (VEC && c + N <= k) {
+      uint4 w;
+      if constexpr (N == 4)
+        w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      else
+        w = make_uint4(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]), bf16x2(v[4], v[5]), bf16x2(v[6], v[7]));
+      *reinterpret_cast<uint4*>(yr + c) = w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; j++)
+        if (c + j < k) yr[c + j] = (T)v[j];
+    }
+  }
 }
+
+// Blocks a lane takes: four, so that enough loads are in flight to fill HBM, but one while the blocks do not give
+// every SM a few warps of four.
+static constexpr unsigned MANY_UNITS = 1u << 15;
 
 template <typename T>
 static cudaError_t quantize_t(const T* x, long rows, long k, long ldx, int block_rows, Fp8Store q, cudaStream_t st) {
-  const int kb = (int)((k + 127) / 128);
-  const bool vec = ldx % 4 == 0 && (uintptr_t)x % (4 * sizeof(T)) == 0;
+  const unsigned kb = (unsigned)((k + 127) / 128);
+  const bool vec = ldx * sizeof(T) % 16 == 0 && (uintptr_t)x % 16 == 0;
   if (block_rows == 1) {
-    const int units = (int)(rows * kb);
-    const int grid = (units + 7) / 8;
-    if (vec)
-      fp8_quant_rows_kernel<T, true><<<grid, 256, 0, st>>>(x, ldx, k, kb, units, q);
+    const unsigned units = (unsigned)(rows * kb);
+    const bool many = units >= MANY_UNITS;
+    const unsigned per = 8 * 2 * (many ? 4 : 1), grid = (unsigned)(((uint64_t)units + per - 1) / per);
+    if (vec && many)
+      fp8_quant_rows_kernel<T, true, 4><<<grid, 256, 0, st>>>(x, ldx, k, kb, units, q);
+    else if (vec)
+      fp8_quant_rows_kernel<T, true, 1><<<grid, 256, 0, st>>>(x, ldx, k, kb, units, q);
+    else if (many)
+      fp8_quant_rows_kernel<T, false, 4><<<grid, 256, 0, st>>>(x, ldx, k, kb, units, q);
     else
-      fp8_quant_rows_kernel<T, false><<<grid, 256, 0, st>>>(x, ldx, k, kb, units, q);
+      fp8_quant_rows_kernel<T, false, 1><<<grid, 256, 0, st>>>(x, ldx, k, kb, units, q);
   } else {
-    const int grid = (int)((rows + 127) / 128 * kb);
+    const unsigned grid = (unsigned)((rows + 127) / 128 * kb);
     if (vec)
       fp8_quant_blocks_kernel<T, true><<<grid, 256, 0, st>>>(x, ldx, rows, k, kb, q);
     else
@@ -148,18 +299,29 @@ cudaError_t launch_fp8_quantize(const void* x, int type, long rows, long k, long
   return quantize_t((const __nv_bfloat16*)x, rows, k, ldx, block_rows, q, st);
 }
 
+template <typename T>
+static cudaError_t dequantize_t(Fp8Store q, long rows, long k, int block_rows, T* y, long ldy, cudaStream_t st) {
+  constexpr unsigned PER = 32 / Lane<T>::LANES;
+  const unsigned kb = (unsigned)((k + 127) / 128), units = (unsigned)(rows * kb);
+  const bool vec = ldy * sizeof(T) % 16 == 0 && (uintptr_t)y % 16 == 0, many = units >= MANY_UNITS;
+  const unsigned per = 8 * PER * (many ? 4 : 1), grid = (unsigned)(((uint64_t)units + per - 1) / per);
+  const int shift = block_rows == 1 ? 0 : 7;
+  if (vec && many)
+    fp8_dequant_kernel<T, true, 4><<<grid, 256, 0, st>>>(q, k, kb, units, shift, y, ldy);
+  else if (vec)
+    fp8_dequant_kernel<T, true, 1><<<grid, 256, 0, st>>>(q, k, kb, units, shift, y, ldy);
+  else if (many)
+    fp8_dequant_kernel<T, false, 4><<<grid, 256, 0, st>>>(q, k, kb, units, shift, y, ldy);
+  else
+    fp8_dequant_kernel<T, false, 1><<<grid, 256, 0, st>>>(q, k, kb, units, shift, y, ldy);
+  return cudaGetLastError();
+}
+
 cudaError_t launch_fp8_dequantize(Fp8Store q, long rows, long k, int block_rows, void* y, int type, long ldy,
                                   cudaStream_t st) {
   if (rows == 0) return cudaSuccess;
-  const int quads = (int)((k + 3) / 4);
-  const long total = rows * quads;
-  const unsigned grid = (unsigned)((total + 255) / 256);
-  if (type == FP8_F32)
-    fp8_dequant_kernel<float, true><<<grid, 256, 0, st>>>(q, k, quads, total, block_rows, (float*)y, ldy);
-  else
-    fp8_dequant_kernel<__nv_bfloat16, true><<<grid, 256, 0, st>>>(q, k, quads, total, block_rows, (__nv_bfloat16*)y,
-                                                                  ldy);
-  return cudaGetLastError();
+  if (type == FP8_F32) return dequantize_t(q, rows, k, block_rows, (float*)y, ldy, st);
+  return dequantize_t(q, rows, k, block_rows, (__nv_bfloat16*)y, ldy, st);
 }
 
 }  // namespace kk

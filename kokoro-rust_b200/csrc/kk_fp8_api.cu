@@ -1,12 +1,11 @@
 // C entries of the 8-bit operators: argument checks, the caller's device and stream, status codes.
 #include <cuda_runtime.h>
-#include <stdio.h>
+#include <atomic>
 #include <exception>
 #include <string>
 
 #include "../../include/kokoro_b200.h"
 #include "kk_fp8.h"
-#include "kk_tc.h"
 
 namespace {
 
@@ -64,16 +63,32 @@ const char* bad_extent(int64_t rows, int64_t k) {
   return nullptr;
 }
 
+// What a device ordinal is, looked up once: 1 compute capability 10.x, 2 another device, 3 none.
+int device_kind(int ordinal) {
+  static std::atomic<int> cache[64];
+  if (ordinal < 0 || ordinal >= 64) return 3;
+  int kind = cache[ordinal].load(std::memory_order_relaxed);
+  if (kind == 0) {
+    int n = 0, major = 0;
+    if (cudaGetDeviceCount(&n) != cudaSuccess) {
+      cudaGetLastError();
+      return 3;
+    }
+    if (ordinal >= n || cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, ordinal) != cudaSuccess) return 3;
+    kind = major == 10 ? 1 : 2;
+    cache[ordinal].store(kind, std::memory_order_relaxed);
+  }
+  return kind;
+}
+
 kk_status run(int ordinal, const char* what, cudaError_t (*f)(const void*, cudaStream_t), const void* arg, void* stream) {
   try {
-    int n = 0;
-    cudaError_t e = cudaGetDeviceCount(&n);
-    if (e != cudaSuccess || ordinal < 0 || ordinal >= n)
-      return fail(e != cudaSuccess ? KK_ERR_CUDA : KK_ERR_INVALID_ARG, "CUDA device ordinal out of range");
+    const int kind = device_kind(ordinal);
+    if (kind == 3) return fail(KK_ERR_INVALID_ARG, "CUDA device ordinal out of range");
+    if (kind == 2) return fail(KK_ERR_CUDA, "device is not compute capability 10.x (sm_100a)");
     DeviceGuard g(ordinal);
     if (g.err != cudaSuccess) return fail(KK_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(g.err));
-    if (!kk::tc_available()) return fail(KK_ERR_CUDA, "device is not compute capability 10.x (sm_100a)");
-    e = f(arg, (cudaStream_t)stream);
+    const cudaError_t e = f(arg, (cudaStream_t)stream);
     if (e != cudaSuccess) {
       cudaGetLastError();
       return fail(e == cudaErrorMemoryAllocation ? KK_ERR_OOM : KK_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));

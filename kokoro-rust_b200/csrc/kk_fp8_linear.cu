@@ -951,6 +951,18 @@ static int num_sms() {
   return n;
 }
 
+// Raises a kernel's shared-memory limit, once per device.
+template <class K>
+static cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>* done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (e != cudaSuccess || (dev < 64 && (done->load(std::memory_order_relaxed) & bit))) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done->fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 template <int OUT, bool RES>
 static cudaError_t launch_pair(const Fp8Linear& a, int* err, cudaStream_t st) {
   using S = PairShape<OUT, RES>;
@@ -973,7 +985,8 @@ static cudaError_t launch_pair(const Fp8Linear& a, int* err, cudaStream_t st) {
     if (RES && !make_map(&rm, a.res, es, a.m, a.n, a.ldr, 32)) return cudaErrorInvalidValue;
   }
   const auto kernel = fp8_linear_pair_kernel<OUT, RES>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_smem(kernel, S::SMEM, &allowed);
   if (e != cudaSuccess) return e;
   const long tiles = (long)p.m_tiles * p.n_tiles;
   const int pairs = num_sms() / 2;
@@ -1011,7 +1024,8 @@ static cudaError_t launch_split(const Fp8Linear& a, int splits, int* err, cudaSt
   if (smem < partial) smem = partial;
   smem += 1024;
   const auto kernel = fp8_linear_split_kernel<NT, OUT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SPLIT_BUDGET + 1024);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_smem(kernel, SPLIT_BUDGET + 1024, &allowed);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((a.m + TM - 1) / TM * p.n_tiles * splits));

@@ -18,10 +18,11 @@ from typing import Optional, Union
 
 import torch
 
-from .engine import KK_ERR_INVALID_ARG, KK_OK, KokoroError, load_library
+from .engine import KK_ERR_INVALID_ARG, KokoroError, load_library
 
 E4M3 = torch.float8_e4m3fn
-_TYPES = {torch.float32: 0, torch.bfloat16: 1, E4M3: 2}  # kk_fp8_type
+_F32, _BF16 = torch.float32, torch.bfloat16
+_TYPES = {_F32: 0, _BF16: 1, E4M3: 2}  # kk_fp8_type
 _ACTS = {None: 0, "gelu": 1}  # kk_fp8_act
 
 
@@ -29,22 +30,31 @@ def _refuse(msg: str):
     raise KokoroError(KK_ERR_INVALID_ARG, msg)
 
 
-def _ld(t: torch.Tensor, unit: int = 1) -> int:
-    """Row stride; a single row's is whatever holds its columns."""
-    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // unit) * unit
+def _public_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
 
 
-def _check_rows(t: torch.Tensor, name: str, dtypes) -> None:
+# the current stream's handle without the object around it, where torch offers that (2 us of a small call)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
+
+
+def _rows(t: torch.Tensor, name: str, dtypes, unit: int = 1):
+    """(rows, columns, row stride) of a CUDA tensor of rows whose columns are adjacent; a single row's
+    stride is whatever holds its columns."""
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
         _refuse(f"{name}: a tensor of {' or '.join(str(d) for d in dtypes)} is wanted")
-    if t.dim() != 2:
+    shape = t.shape
+    if len(shape) != 2:
         _refuse(f"{name}: rows are wanted, [rows, columns]")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    rows, k = shape
+    ld, inner = t.stride()
+    if inner != 1 and k > 1:
         _refuse(f"{name}: a row's columns must be adjacent")
     if not t.is_cuda:
         _refuse(f"{name}: a CUDA tensor is wanted")
     if t.requires_grad and torch.is_grad_enabled():
         _refuse(f"{name}: the 8-bit operators have no gradient")
+    return rows, k, ld if rows > 1 else -(-k // unit) * unit
 
 
 class Fp8Tensor:
@@ -52,36 +62,55 @@ class Fp8Tensor:
     bytes apart) and ``exps`` (uint8 [ceil(rows / block_rows), ceil(k / 128)], rows a multiple of 4
     bytes apart): a block stands for value * 2^(E - 127). block_rows is 1 (activations) or 128 (weights)."""
 
-    __slots__ = ("values", "exps", "block_rows")
+    __slots__ = ("shape", "block_rows", "device", "_values", "_exps", "_buf", "_args")
 
     def __init__(self, values: torch.Tensor, exps: torch.Tensor, block_rows: int = 1):
-        _check_rows(values, "values", (E4M3,))
-        _check_rows(exps, "exps", (torch.uint8,))
-        if block_rows not in (1, 128):
+        rows, k, ldv = _rows(values, "values", (E4M3,), 16)
+        erows, kb, lde = _rows(exps, "exps", (torch.uint8,), 4)
+        if block_rows != 1 and block_rows != 128:
             _refuse("block_rows must be 1 or 128")
-        rows, k = values.shape
-        if exps.shape[0] != -(-rows // block_rows) or exps.shape[1] != -(-k // 128):
+        if erows != -(-rows // block_rows) or kb != -(-k // 128):
             _refuse(f"exps: [{-(-rows // block_rows)}, {-(-k // 128)}] is wanted for values [{rows}, {k}]")
-        if exps.device != values.device:
+        self.device = values.device
+        if exps.device != self.device:
             _refuse("values and exps must be on one device")
-        self.values, self.exps, self.block_rows = values, exps, block_rows
+        self.shape, self.block_rows, self._values, self._exps, self._buf = values.shape, block_rows, values, exps, None
+        self._args = (values.data_ptr(), ldv, exps.data_ptr(), lde)
 
     @classmethod
     def empty(cls, rows: int, k: int, block_rows: int = 1, device="cuda") -> "Fp8Tensor":
         """A store with its rows padded to the alignment that the operators want; not initialised."""
-        kb = -(-k // 128)
-        v = torch.empty(rows, -(-k // 16) * 16, dtype=E4M3, device=device)
-        e = torch.empty(-(-rows // block_rows) if block_rows in (1, 128) else 0, -(-kb // 4) * 4, dtype=torch.uint8,
-                        device=device)
-        return cls(v[:, :k], e[:, :kb], block_rows)
+        if block_rows != 1 and block_rows != 128:
+            _refuse("block_rows must be 1 or 128")
+        if rows < 0 or k < 0:
+            _refuse("rows and columns must not be negative")
+        ldv, lde = -(-k // 16) * 16, -(-k // 512) * 4
+        self = cls.__new__(cls)
+        # one allocation: the values, then the exponents; the views are made when they are asked for
+        self._buf = torch.empty(rows * ldv + -(-rows // block_rows) * lde, dtype=torch.uint8, device=device)
+        at = self._buf.data_ptr()
+        self.shape, self.block_rows, self.device = torch.Size((rows, k)), block_rows, self._buf.device
+        self._values = self._exps = None
+        self._args = (at, ldv, at + rows * ldv, lde)
+        return self
+
+    def _views(self) -> None:
+        (rows, k), (_, ldv, _, lde) = self.shape, self._args
+        n = rows * ldv
+        self._values = self._buf[:n].view(E4M3).view(rows, ldv)[:, :k]
+        self._exps = self._buf[n:].view(-(-rows // self.block_rows), lde)[:, : -(-k // 128)]
 
     @property
-    def shape(self) -> torch.Size:
-        return self.values.shape
+    def values(self) -> torch.Tensor:
+        if self._values is None:
+            self._views()
+        return self._values
 
     @property
-    def device(self) -> torch.device:
-        return self.values.device
+    def exps(self) -> torch.Tensor:
+        if self._exps is None:
+            self._views()
+        return self._exps
 
     def __getitem__(self, rows: slice) -> "Fp8Tensor":
         """A view of some of an activation store's rows (to read them, or to quantise into them)."""
@@ -89,33 +118,29 @@ class Fp8Tensor:
             _refuse("a store is cut by a slice of rows, and only with block_rows 1")
         return Fp8Tensor(self.values[rows], self.exps[rows])
 
-    def _args(self):
-        v, e = self.values, self.exps
-        return v.data_ptr(), _ld(v, 16), e.data_ptr(), _ld(e, 4)
-
 
 def _run(status: int) -> None:
-    if status != KK_OK:
+    if status != 0:
         raise KokoroError(status, load_library().kk_fp8_error().decode())
 
 
-def _same_device(dev: torch.device, *tensors) -> None:
-    for t in tensors:
-        if t is not None and t.device != dev:
-            _refuse(f"tensors on {dev} and {t.device}: one device is wanted")
+def _one_device(dev: torch.device, other: torch.device) -> None:
+    if other != dev:
+        _refuse(f"tensors on {dev} and {other}: one device is wanted")
 
 
 def quantize(x: torch.Tensor, block_rows: int = 1, out: Optional[Fp8Tensor] = None) -> Fp8Tensor:
     """x [rows, k] (float32 or bfloat16) as a store; into ``out`` when given (its other rows are left)."""
-    _check_rows(x, "x", (torch.float32, torch.bfloat16))
+    rows, k, ld = _rows(x, "x", (_F32, _BF16))
+    dev = x.device
     if out is None:
-        out = Fp8Tensor.empty(x.shape[0], x.shape[1], block_rows, x.device)
+        out = Fp8Tensor.empty(rows, k, block_rows, dev)
     elif not isinstance(out, Fp8Tensor) or out.shape != x.shape or out.block_rows != block_rows:
         _refuse("out: a store of x's shape and of the same block_rows is wanted")
-    dev = x.device
-    _same_device(dev, out.values)
-    _run(load_library().kk_fp8_quantize(dev.index, torch.cuda.current_stream(dev).cuda_stream, x.data_ptr(),
-                                        _TYPES[x.dtype], x.shape[0], x.shape[1], _ld(x), block_rows, *out._args()))
+    elif out.device != dev:
+        _one_device(dev, out.device)
+    _run(load_library().kk_fp8_quantize(dev.index, _stream(dev.index), x.data_ptr(), _TYPES[x.dtype], rows, k, ld,
+                                        block_rows, *out._args))
     return out
 
 
@@ -124,19 +149,18 @@ def dequantize(q: Fp8Tensor, dtype: torch.dtype = torch.float32, out: Optional[t
     but for bfloat16 below its normal numbers)."""
     if not isinstance(q, Fp8Tensor):
         _refuse("q: a store is wanted")
+    if dtype is not _F32 and dtype is not _BF16:
+        _refuse("dtype: float32 or bfloat16 is wanted")
+    (rows, k), dev = q.shape, q.device
     if out is None:
-        if dtype not in (torch.float32, torch.bfloat16):
-            _refuse("dtype: float32 or bfloat16 is wanted")
-        out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        out, ld = torch.empty((rows, k), dtype=dtype, device=dev), k
     else:
-        _check_rows(out, "out", (dtype,) if dtype in (torch.float32, torch.bfloat16) else (torch.float32,))
+        ld = _rows(out, "out", (dtype,))[2]
         if out.shape != q.shape:
             _refuse("out: the store's shape is wanted")
-    dev = q.device
-    _same_device(dev, out)
-    _run(load_library().kk_fp8_dequantize(dev.index, torch.cuda.current_stream(dev).cuda_stream, *q._args(),
-                                          q.block_rows, q.shape[0], q.shape[1], out.data_ptr(), _TYPES[out.dtype],
-                                          _ld(out)))
+        _one_device(dev, out.device)
+    _run(load_library().kk_fp8_dequantize(dev.index, _stream(dev.index), *q._args, q.block_rows, rows, k, out.data_ptr(),
+                                          _TYPES[dtype], ld))
     return out
 
 
@@ -151,48 +175,54 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
         _refuse("x: a store with block_rows 1 is wanted")
     if not isinstance(w, Fp8Tensor) or w.block_rows != 128:
         _refuse("w: a store with block_rows 128 is wanted")
-    m, k = x.values.shape
-    n = w.values.shape[0]
-    if w.values.shape[1] != k:
-        _refuse(f"x has {k} columns and w {w.values.shape[1]}")
+    m, k = x.shape
+    n, kw = w.shape
+    if kw != k:
+        _refuse(f"x has {k} columns and w {kw}")
     if act not in _ACTS:
         _refuse("act: None or 'gelu' is wanted")
+    if out_dtype not in _TYPES:
+        _refuse("out_dtype: float32, bfloat16 or float8_e4m3fn is wanted")
+    dev = x.device
+    if w.device != dev:
+        _one_device(dev, w.device)
+    b = None
     if bias is not None:
-        if bias.dtype != torch.float32 or bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
+        if bias.dtype is not _F32 or bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
             _refuse(f"bias: adjacent float32 [{n}] is wanted")
         if bias.requires_grad and torch.is_grad_enabled():
             _refuse("bias: the 8-bit operators have no gradient")
-    dev = x.values.device
-    if out is None:
-        if out_dtype == E4M3:
-            out = Fp8Tensor.empty(m, n, 1, dev)
-        elif out_dtype in (torch.float32, torch.bfloat16):
-            out = torch.empty((m, n), dtype=out_dtype, device=dev)
-        else:
-            _refuse("out_dtype: float32, bfloat16 or float8_e4m3fn is wanted")
-    if isinstance(out, Fp8Tensor):
-        if out.block_rows != 1 or out.shape != (m, n) or out_dtype != E4M3:
-            _refuse(f"out: a store [{m}, {n}] with block_rows 1 goes with out_dtype float8_e4m3fn")
-        if residual is not None:
+        if bias.device != dev:
+            _one_device(dev, bias.device)
+        b = bias.data_ptr()
+    res, ldr = None, 0
+    if residual is not None:
+        if out_dtype is E4M3:
             _refuse("an e4m3 result takes no residual")
-        y_type, y = 2, out._args()
-        _same_device(dev, w.values, bias, out.values)
-        r = (None, 0)
+        ldr = _rows(residual, "residual", (out_dtype,))[2]
+        if residual.shape != (m, n):
+            _refuse(f"residual: [{m}, {n}] is wanted")
+        if residual.device != dev:
+            _one_device(dev, residual.device)
+        res = residual.data_ptr()
+    if out_dtype is E4M3:
+        if out is None:
+            out = Fp8Tensor.empty(m, n, 1, dev)
+        elif not isinstance(out, Fp8Tensor) or out.block_rows != 1 or out.shape != (m, n):
+            _refuse(f"out: a store [{m}, {n}] with block_rows 1 is wanted")
+        y = out._args
+    elif out is None:
+        out = torch.empty((m, n), dtype=out_dtype, device=dev)
+        y = (out.data_ptr(), n, None, 0)
     else:
-        _check_rows(out, "out", (out_dtype,) if out_dtype in (torch.float32, torch.bfloat16) else ())
+        ldy = _rows(out, "out", (out_dtype,))[2]
         if out.shape != (m, n):
             _refuse(f"out: [{m}, {n}] is wanted")
-        y_type, y = _TYPES[out_dtype], (out.data_ptr(), _ld(out), None, 0)
-        _same_device(dev, w.values, bias, out, residual)
-        r = (None, 0)
-        if residual is not None:
-            _check_rows(residual, "residual", (out_dtype,))
-            if residual.shape != (m, n):
-                _refuse(f"residual: [{m}, {n}] is wanted")
-            r = (residual.data_ptr(), _ld(residual))
-    _run(load_library().kk_fp8_linear(dev.index, torch.cuda.current_stream(dev).cuda_stream, m, n, k, *x._args(),
-                                      *w._args(), None if bias is None else bias.data_ptr(), _ACTS[act], *r, y_type,
-                                      *y))
+        y = (out.data_ptr(), ldy, None, 0)
+    if out.device != dev:
+        _one_device(dev, out.device)
+    _run(load_library().kk_fp8_linear(dev.index, _stream(dev.index), m, n, k, *x._args, *w._args, b, _ACTS[act], res, ldr,
+                                      _TYPES[out_dtype], *y))
     return out
 
 
@@ -201,4 +231,4 @@ def check(device=None) -> None:
     device gave up since the last check (its results are then not valid)."""
     dev = torch.device("cuda") if device is None else torch.device(device)
     idx = torch.cuda.current_device() if dev.index is None else dev.index
-    _run(load_library().kk_fp8_check(idx, torch.cuda.current_stream(idx).cuda_stream))
+    _run(load_library().kk_fp8_check(idx, _stream(idx)))
