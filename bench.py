@@ -311,7 +311,7 @@ def main():
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--impl", default="ours", choices=["ours", "reference"])
     ap.add_argument("--workload", default="config4", choices=["config4", "config3", "config2", "config5", "conv"])
-    ap.add_argument("--precision", default=os.environ.get("KK_PRECISION", "bf16"), choices=["bf16", "fp32"])
+    ap.add_argument("--precision", default=os.environ.get("KK_PRECISION", "bf16"), choices=["bf16", "fp32", "fp8"])
     ap.add_argument("--cpu-lines", type=int, default=3, help="lines in the CPU-baseline sample")
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--launch-log", default=None, help="write every profiled launch (class, ms, FLOPs, bytes) of the PROF_STEPS profiled steps as CSV")
@@ -579,7 +579,7 @@ def main():
                                                   "config2": " (vocoder-only decoder+generator)"}[args.workload],
             "value": value, "unit": "audio-s/s", "n_gpus": world, "steps": args.steps, "warmup": args.warmup,
             "ms_per_step": max_ms / args.steps, "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
-            "dtype": "bf16" if "tcgen05" in eng.identity else "f32", "data": "synthetic",
+            "dtype": args.precision if "tcgen05" in eng.identity else "f32", "data": "synthetic",
             "config": {"workload": workload_desc, "precision": args.precision, "engine": eng.identity,
                        "audio_s_per_step": total_audio / args.steps / world,
                        "l2": "inputs larger than L2: each step moves tens of GB of activations (L2 126 MB)",

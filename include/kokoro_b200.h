@@ -43,8 +43,12 @@ typedef enum {
 
 typedef enum {
   KK_PRECISION_FP32 = 0, /* fp32 everywhere (SIMT FFMA); the parity path */
-  KK_PRECISION_BF16 = 1  /* bf16 tensor-core (tcgen05) convs and GEMMs, fp32 accumulation; the LSTM
+  KK_PRECISION_BF16 = 1, /* bf16 tensor-core (tcgen05) convs and GEMMs, fp32 accumulation; the LSTM
                             recurrence on tensor cores at fp32-level accuracy */
+  KK_PRECISION_FP8 = 2   /* the BF16 mode with ALBERT's layers (QKV, output projection, FFN) in 8 bits: e4m3
+                            rows and weights with a scale for each block of 128 (see kk_fp8_linear), fp32
+                            accumulation and residual rows; some predicted durations differ from the
+                            BF16 mode's, by a frame */
 } kk_precision;
 
 typedef struct kk_engine kk_engine;
@@ -364,7 +368,7 @@ KK_API const char* kk_conv_selftest_error(void);
 /*
  * 8-bit operators on device buffers: rows held as e4m3 values with a power-of-two scale for each block
  * of 128, and the linear layer over them. No counterpart in the reference (its linear layers are f32 and
- * BF16x, docs/VALIDATION.md:38-45).
+ * BF16x, docs/VALIDATION.md:38-45); the engine's KK_PRECISION_FP8 runs ALBERT's linear layers on them.
  *
  * A store is values (e4m3 bytes, rows ldv bytes apart) and exps (E8M0 bytes E, rows lde bytes apart, one
  * byte per 128 columns): a block stands for value * 2^(E - 127). block_rows is 1 for activations (one

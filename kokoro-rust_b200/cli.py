@@ -470,7 +470,7 @@ def build_parser() -> argparse.ArgumentParser:
     s.add_argument("--cuda-devices", default=None,
                    help="comma-separated CUDA ordinals: one engine process per GPU, each batch window "
                         "spread over them (longest first to the least-loaded GPU), results in line order")
-    s.add_argument("--precision", choices=["bf16", "fp32"], default="bf16")
+    s.add_argument("--precision", choices=["bf16", "fp32", "fp8"], default="bf16")
     s.add_argument("--batch-phonemes", type=int, default=8000)
     s.add_argument("--batch-items", type=int, default=64)
     s.add_argument("--batch-window", type=int, default=256)

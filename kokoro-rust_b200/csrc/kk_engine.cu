@@ -248,6 +248,12 @@ struct Conv {
   float* b = nullptr;
   TcWeights tc;        // bf16 tcgen05 operand layout (BF16 precision only)
 };
+// A linear layer's weights held in 8 bits (FP8 mode): [cout][cin] in blocks of 128 x 128.
+struct Lin8 {
+  int cin = 0, cout = 0;
+  Fp8Store w{};
+  const float* b = nullptr;
+};
 struct AdaIN {
   float* nw = nullptr;
   float* nb = nullptr;
@@ -281,6 +287,7 @@ struct Model {
   Conv map_in, qkv, dense, ffn, ffn_out;
   float *attn_g, *attn_b, *full_g, *full_b;
   Conv bert_enc;
+  Lin8 qkv8, dense8, ffn8, ffn_out8;  // FP8 mode
   Lstm dur_lstm[3];
   int adaln_off[3];
   Lstm pred_lstm, shared, te_lstm;
@@ -330,6 +337,7 @@ static const int MIN_LAYOUT_ROWS = 64;
 struct Engine {
   int dev = 0;
   int precision = KK_PRECISION_FP32;
+  bool text_fp8 = false;  // FP8 mode: the BF16 mode with ALBERT's linear layers in 8 bits
   cudaStream_t st = nullptr;
   Model m{};
   std::vector<void*> wallocs;
@@ -389,6 +397,7 @@ struct Engine {
   Conv load_conv(const Checkpoint& ck, const std::string& p, int cin, int cout, int K, int dil, int pad, int stride,
                  bool bias);
   Conv load_linear(const Checkpoint& ck, const std::string& p, int din, int dout, bool bias = true);
+  Lin8 hold_fp8(const std::vector<float>& w, const Conv& c);
   AdaIN load_adain(const Checkpoint& ck, const std::string& p, int c, std::vector<float>& fcw, std::vector<float>& fcb);
   ResBlk load_resblk(const Checkpoint& ck, const std::string& p, int din, int dout, bool up, std::vector<float>& fcw,
                      std::vector<float>& fcb);
@@ -412,6 +421,9 @@ struct Engine {
   void stage_sync(const char* what);
   ConvArgs ca(const Conv& c);
   void run_conv(const Conv& c, ConvArgs& a);
+  Fp8Store fp8_rows(long rows, int k);
+  void linear8(const Lin8& c, const Fp8Store& x, long rows, bool gelu, const float* res, int y_type, void* y, long ldy,
+               const Fp8Store& q);
   bool tc_route(const Conv& c, const ConvArgs& a) const;
   bool tc_pre(const Conv& c, const ConvArgs& a) const;
   void run_conv_stats(const Conv& c, ConvArgs& a, const Dom& dout, const ItemTab* items, int B, int max_len,
@@ -586,6 +598,26 @@ Conv Engine::load_linear(const Checkpoint& ck, const std::string& p, int din, in
   return conv_from(w, bias ? b.data() : nullptr, din, dout, 1, 1, 0, 1);
 }
 
+// The weights of a loaded linear layer ([cout][cin]) in 8 bits, quantised on the device.
+Lin8 Engine::hold_fp8(const std::vector<float>& w, const Conv& c) {
+  Lin8 l;
+  l.cin = c.cin, l.cout = c.cout, l.b = c.b;
+  l.w.ldv = (c.cin + 15) / 16 * 16, l.w.lde = (c.cin + 511) / 512 * 4;
+  const size_t nv = (size_t)c.cout * l.w.ldv, ne = (size_t)(c.cout + 127) / 128 * l.w.lde;
+  KK_CUDA(cudaMalloc(&l.w.v, nv + ne));
+  wallocs.push_back(l.w.v);
+  wbytes += nv + ne;
+  l.w.e = l.w.v + nv;
+  float* f = nullptr;
+  KK_CUDA(cudaMalloc(&f, w.size() * sizeof(float)));
+  cudaError_t e = cudaMemcpyAsync(f, w.data(), w.size() * sizeof(float), cudaMemcpyHostToDevice, st);
+  if (e == cudaSuccess) e = launch_fp8_quantize(f, FP8_F32, c.cout, c.cin, c.cin, 128, l.w, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  cudaFree(f);
+  KK_CUDA(e);
+  return l;
+}
+
 // AdaIN1d (src/nn.rs:87-100): affine defaults, and fc rows appended to the fused projection.
 AdaIN Engine::load_adain(const Checkpoint& ck, const std::string& p, int c, std::vector<float>& fcw,
                          std::vector<float>& fcb) {
@@ -704,6 +736,7 @@ void Engine::load(const Checkpoint& ck) {
       b.insert(b.end(), c.begin(), c.end());
     }
     m.qkv = conv_from(w, b.data(), 768, 2304, 1, 1, 0, 1);
+    if (text_fp8) m.qkv8 = hold_fp8(w, m.qkv);
   }
   m.dense = load_linear(ck, L + ".attention.dense", 768, 768);
   m.attn_g = up(ck.get(L + ".attention.LayerNorm.weight", {768}));
@@ -713,6 +746,11 @@ void Engine::load(const Checkpoint& ck) {
   m.full_g = up(ck.get(L + ".full_layer_layer_norm.weight", {768}));
   m.full_b = up(ck.get(L + ".full_layer_layer_norm.bias", {768}));
   m.bert_enc = load_linear(ck, "bert_encoder", 768, 512);
+  if (text_fp8) {
+    m.dense8 = hold_fp8(ck.get(L + ".attention.dense.weight", {768, 768}), m.dense);
+    m.ffn8 = hold_fp8(ck.get(L + ".ffn.weight", {2048, 768}), m.ffn);
+    m.ffn_out8 = hold_fp8(ck.get(L + ".ffn_output.weight", {768, 2048}), m.ffn_out);
+  }
   // ---- predictor (src/model.rs:60-86)
   for (int i = 0; i < 3; i++) {
     m.dur_lstm[i] = load_lstm(ck, "predictor.text_encoder.lstms." + std::to_string(2 * i), 640);
@@ -1002,6 +1040,29 @@ void Engine::linear(const Conv& c, const float* x, int ldx, int rows, float* y, 
   a.x = x, a.ldx = ldx, a.L_in = rows, a.y = y, a.ldy = ldy, a.L_out = rows, a.out_mode = out_mode, a.sc = sc,
   a.ldsc = ldsc;
   run_conv(c, a);
+}
+
+// A store of token rows from the arena (block_rows 1, k a multiple of 16).
+Fp8Store Engine::fp8_rows(long rows, int k) {
+  Fp8Store q;
+  q.ldv = k, q.lde = (k + 511) / 512 * 4;
+  q.v = ar.get<uint8_t>((size_t)rows * q.ldv);
+  q.e = ar.get<uint8_t>((size_t)rows * q.lde);
+  return q;
+}
+
+// y (or the store q) = act(x W^T + b) + res over token rows held in 8 bits; res has y's type and stride
+void Engine::linear8(const Lin8& c, const Fp8Store& x, long rows, bool gelu, const float* res, int y_type, void* y,
+                     long ldy, const Fp8Store& q) {
+  cudaEvent_t e0;
+  prof_begin(&e0);
+  Fp8Linear a{};
+  a.m = rows, a.n = c.cout, a.k = c.cin, a.x = x, a.w = c.w, a.bias = c.b, a.gelu = gelu;
+  a.res = res, a.ldr = ldy, a.y_type = y_type, a.y = y, a.ldy = ldy, a.q = q;
+  check(launch_fp8_linear(a, err_flag, st), "linear(8 bit)");
+  const double out_b = y_type == FP8_F32 ? (res ? 8.0 : 4.0) : (y_type == FP8_BF16 ? 2.0 : 1.0);
+  prof_end(e0, "linear_fp8", 2.0 * rows * c.cin * c.cout,
+           (double)rows * c.cin + (double)c.cin * c.cout + out_b * rows * c.cout);
 }
 
 void Engine::stats(const float* x, int ldx, int C, const Dom& d, const ItemTab* items, int B, int max_len, float** mean,
@@ -1548,7 +1609,14 @@ void Engine::forward(int B, const int64_t* ids, const int32_t* ids_len, const fl
       planes = attn_tc && tc_route(m.qkv, t0) && tc_route(m.qkv, t00) && tc_pre(m.qkv, t00) &&
                tc_route(m.dense, t1) && tc_route(m.ffn, t2) && tc_route(m.ffn_out, t3);
     }
-    if (!planes) f = ar.get<float>((size_t)LT * 2048);
+    // FP8 mode: the same chain with its rows held in 8 bits between the layers, written by the LayerNorms and the
+    // GELU layer as they finish them (the attention's rows by the quantiser); the residual rows stay in 32 bits
+    Fp8Store hq{}, cq{}, aq{}, fq{};
+    if (text_fp8) {
+      planes = false;
+      hq = fp8_rows(LT, 768), cq = fp8_rows(LT, 768), aq = fp8_rows(LT, 768), fq = fp8_rows(LT, 2048);
+    }
+    if (!planes && !text_fp8) f = ar.get<float>((size_t)LT * 2048);
     linear(m.map_in, emb, 128, LT, h, 768);
     int max_t = 0;
     for (int b = 0; b < B; b++) max_t = std::max(max_t, ids_len[b]);
@@ -1569,8 +1637,11 @@ void Engine::forward(int B, const int64_t* ids, const int32_t* ids_len, const fl
       }
       work_d = upload(all.data(), all.size());
     }
+    if (text_fp8) check(launch_fp8_quantize(h, FP8_F32, LT, 768, 768, 1, hq, st), "quantize");
     for (int layer = 0; layer < 12; layer++) {
-      if (planes && layer > 0) {
+      if (text_fp8) {
+        linear8(m.qkv8, hq, LT, false, nullptr, attn_tc ? FP8_BF16 : FP8_F32, qkv, 2304, {});
+      } else if (planes && layer > 0) {
         ConvArgs t = pre_args(m.qkv, hpre, qkv, 2304, OUT_STORE_BF, nullptr, nullptr);
         run_conv(m.qkv, t);
       } else if (planes) {
@@ -1583,7 +1654,7 @@ void Engine::forward(int B, const int64_t* ids, const int32_t* ids_len, const fl
       cudaEvent_t e0;
       prof_begin(&e0);
       if (attn_tc) {
-        check(launch_attention_tc(qkv, 2304, planes, items_d, work_d, n_work, ctx, 768, err_flag, st,
+        check(launch_attention_tc(qkv, 2304, planes || text_fp8, items_d, work_d, n_work, ctx, 768, err_flag, st,
                                   planes ? ctxpre : nullptr, pre_rows),
               "attention(tcgen05)");
         launches += (n_work[0] > 0) + (n_work[1] > 0) + (n_work[2] > 0) - 1;  // one kernel per non-empty bucket
@@ -1592,16 +1663,22 @@ void Engine::forward(int B, const int64_t* ids, const int32_t* ids_len, const fl
       double af = 0;
       for (int b = 0; b < B; b++) af += 4.0 * 12 * 64 * (double)ids_len[b] * ids_len[b];
       prof_end(e0, "attention", af);
-      if (planes) {
+      if (text_fp8) {
+        check(launch_fp8_quantize(ctx, FP8_F32, LT, 768, 768, 1, cq, st), "quantize");
+        linear8(m.dense8, cq, LT, false, h, FP8_F32, a, 768, {});
+      } else if (planes) {
         ConvArgs t1 = pre_args(m.dense, ctxpre, a, 768, OUT_PLUS, h, nullptr);
         run_conv(m.dense, t1);
       } else {
         linear(m.dense, ctx, 768, LT, a, 768, OUT_PLUS, h, 768);
       }
       check(launch_ln_rows(a, 768, LT, 768, m.attn_g, m.attn_b, 1e-12f, 0, 0.0f, nullptr, nullptr, 0, nullptr, 0, a,
-                           768, st, planes ? apre : nullptr, pre_rows),
+                           768, st, planes ? apre : nullptr, pre_rows, aq),
             "ln");
-      if (planes) {
+      if (text_fp8) {
+        linear8(m.ffn8, aq, LT, true, nullptr, FP8_E4M3, nullptr, 0, fq);
+        linear8(m.ffn_out8, fq, LT, false, a, FP8_F32, h, 768, {});
+      } else if (planes) {
         ConvArgs t2 = pre_args(m.ffn, apre, nullptr, 0, OUT_GELU_PRE, nullptr, fpre);
         run_conv(m.ffn, t2);
         ConvArgs t3 = pre_args(m.ffn_out, fpre, h, 768, OUT_PLUS, a, nullptr);
@@ -1611,7 +1688,7 @@ void Engine::forward(int B, const int64_t* ids, const int32_t* ids_len, const fl
         linear(m.ffn_out, f, 2048, LT, h, 768, OUT_PLUS, a, 768);
       }
       check(launch_ln_rows(h, 768, LT, 768, m.full_g, m.full_b, 1e-12f, 0, 0.0f, nullptr, nullptr, 0, nullptr, 0, h,
-                           768, st, planes && layer < 11 ? hpre : nullptr, pre_rows),
+                           768, st, planes && layer < 11 ? hpre : nullptr, pre_rows, layer < 11 ? hq : Fp8Store{}),
             "ln");
     }
     // bert_encoder -> d_en, then [d_en | s_pro] (src/gpu_batch.rs:223-231)
@@ -2023,7 +2100,7 @@ kk_status kk_create(const char* path, int cuda_ordinal, int precision, kk_engine
     return KK_ERR_INVALID_ARG;
   }
   *out = nullptr;
-  if (precision != KK_PRECISION_FP32 && precision != KK_PRECISION_BF16) {
+  if (precision != KK_PRECISION_FP32 && precision != KK_PRECISION_BF16 && precision != KK_PRECISION_FP8) {
     g_create_error = "unknown precision";
     return KK_ERR_INVALID_ARG;
   }
@@ -2038,16 +2115,17 @@ kk_status kk_create(const char* path, int cuda_ordinal, int precision, kk_engine
     if (prop.major != 10)
       throw kk::KKError(KK_ERR_CUDA, std::string("device ") + prop.name + " is not compute capability 10.x (sm_100a)");
     e.dev = cuda_ordinal;
-    e.precision = precision;
+    e.text_fp8 = precision == KK_PRECISION_FP8;
+    e.precision = precision == KK_PRECISION_FP8 ? (int)KK_PRECISION_BF16 : precision;
     KK_CUDA(cudaSetDevice(cuda_ordinal));
     KK_CUDA(cudaStreamCreateWithFlags(&e.st, cudaStreamNonBlocking));
     KK_CUDA(cudaMalloc(&e.err_flag, sizeof(int)));
     e.wallocs.push_back(e.err_flag);
     KK_CUDA(cudaMemset(e.err_flag, 0, sizeof(int)));
-    e.tc_ok = precision == KK_PRECISION_BF16 && kk::tc_available();
+    e.tc_ok = e.precision == KK_PRECISION_BF16 && kk::tc_available();
     kk::Checkpoint ck(path);
     e.load(ck);
-    e.ident = std::string("cuda-b200 ") + (precision == KK_PRECISION_BF16 ? "bf16" : "fp32") +
+    e.ident = std::string("cuda-b200 ") + (e.text_fp8 ? "fp8" : (precision == KK_PRECISION_BF16 ? "bf16" : "fp32")) +
               (e.tc_ok ? " tcgen05" : " simt");
   });
   if (s != KK_OK) return s;

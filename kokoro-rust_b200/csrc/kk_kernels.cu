@@ -11,6 +11,7 @@
 #include <math.h>
 #include <string.h>
 #include "kk_common.cuh"
+#include "kk_fp8_math.cuh"
 #include "kk_launch.h"
 
 namespace kk {
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(256) ln_rows_warp_kernel(const float* x, int l
                                                            const float* bb, float eps, int mode, float slope,
                                                            const int* row_item, const float* gb, int ldgb,
                                                            const float* style, int sdim, float* y, int ldy,
-                                                           uint8_t* ypre, long ypre_rows) {
+                                                           uint8_t* ypre, long ypre_rows, Fp8Store q) {
   constexpr int d = 128 * NV;
   const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (r >= rows) return;
@@ -241,14 +242,14 @@ __global__ void __launch_bounds__(256) ln_rows_warp_kernel(const float* x, int l
 #pragma unroll
   for (int k = 0; k < NV; k++) s += ((double)v[k].x + (double)v[k].y) + ((double)v[k].z + (double)v[k].w);
   const float mean = (float)(warp_sum_d(s) / (double)d);
-  double q = 0.0;
+  double var = 0.0;
 #pragma unroll
   for (int k = 0; k < NV; k++) {
     const double c0 = (double)(v[k].x - mean), c1 = (double)(v[k].y - mean);
     const double c2 = (double)(v[k].z - mean), c3 = (double)(v[k].w - mean);
-    q += (c0 * c0 + c1 * c1) + (c2 * c2 + c3 * c3);
+    var += (c0 * c0 + c1 * c1) + (c2 * c2 + c3 * c3);
   }
-  const float inv = 1.0f / sqrtf((float)(warp_sum_d(q) / (double)d) + eps);
+  const float inv = 1.0f / sqrtf((float)(warp_sum_d(var) / (double)d) + eps);
   float4* yo = reinterpret_cast<float4*>(yr);
 #pragma unroll
   for (int k = 0; k < NV; k++) {
@@ -275,6 +276,13 @@ __global__ void __launch_bounds__(256) ln_rows_warp_kernel(const float* x, int l
       const int plane = (j >> 6) * 8 + ((j & 31) >> 2);
       *reinterpret_cast<uint2*>(ypre + ((size_t)plane * ypre_rows + PRE_PAD_FRONT + r) * 16 + ((j >> 5) & 1) * 8) = u;
     }
+    if (q.v) {  // the warp holds the 128 columns of block k
+      const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, max(max(finite_bits(o[0]), finite_bits(o[1])),
+                                                            max(finite_bits(o[2]), finite_bits(o[3]))));
+      const int e = fp8_exp(m);
+      *reinterpret_cast<uint32_t*>(q.v + r * q.ldv + j) = e4m3x4(o[0], o[1], o[2], o[3], fp8_inv_scale(e));
+      if (lane == 0) q.e[r * q.lde + k] = (uint8_t)e;
+    }
   }
   if (mode == 2)
     for (int j = lane; j < sdim; j += 32) yr[d + j] = style[(long)item * sdim + j];
@@ -283,19 +291,20 @@ __global__ void __launch_bounds__(256) ln_rows_warp_kernel(const float* x, int l
 cudaError_t launch_ln_rows(const float* x, int ldx, int rows, int d, const float* g, const float* b, float eps,
                            int mode, float slope, const int* row_item, const float* gb, int ldgb,
                            const float* style, int sdim, float* y, int ldy, cudaStream_t st, void* ypre,
-                           long ypre_rows) {
+                           long ypre_rows, Fp8Store q) {
   if (rows == 0) return cudaSuccess;
   const bool vec = ldx % 4 == 0 && ldy % 4 == 0 && (((uintptr_t)x | (uintptr_t)y) & 15) == 0;
   if (ypre && (!vec || mode == 2 || (d != 512 && d != 768) || (((uintptr_t)ypre) & 15) != 0))
     return cudaErrorInvalidValue;
+  if (q.v && (!vec || mode == 2 || (d != 512 && d != 768))) return cudaErrorInvalidValue;
   if (vec && (d == 512 || d == 768)) {
     const int grid = (rows + 7) / 8;
     if (d == 512)
       ln_rows_warp_kernel<4><<<grid, 256, 0, st>>>(x, ldx, rows, g, b, eps, mode, slope, row_item, gb, ldgb, style,
-                                                   sdim, y, ldy, (uint8_t*)ypre, ypre_rows);
+                                                   sdim, y, ldy, (uint8_t*)ypre, ypre_rows, q);
     else
       ln_rows_warp_kernel<6><<<grid, 256, 0, st>>>(x, ldx, rows, g, b, eps, mode, slope, row_item, gb, ldgb, style,
-                                                   sdim, y, ldy, (uint8_t*)ypre, ypre_rows);
+                                                   sdim, y, ldy, (uint8_t*)ypre, ypre_rows, q);
     return cudaGetLastError();
   }
   ln_rows_kernel<<<rows, 256, 0, st>>>(x, ldx, d, g, b, eps, mode, slope, row_item, gb, ldgb, style, sdim, y, ldy);

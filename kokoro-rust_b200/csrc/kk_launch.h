@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include "kk_common.cuh"
+#include "kk_fp8.h"
 
 namespace kk {
 
@@ -39,10 +40,12 @@ cudaError_t launch_embed_rows(const int* ids, const int* row_item, int rows, con
 //          :375-383); gap rows of y -> 0.
 // ypre (optional, d = 512 / 768, modes 0 / 1): the output rows also as bf16 window planes (the
 // IN_PRE operand layout of kk_common.cuh, ypre_rows rows per plane) for a following tensor-core layer.
+// q (optional, d = 512 / 768, modes 0 / 1): the output rows also quantised into a store (kk_fp8.h, block_rows
+// 1) for a following 8-bit layer.
 cudaError_t launch_ln_rows(const float* x, int ldx, int rows, int d, const float* g, const float* b,
                            float eps, int mode, float slope, const int* row_item, const float* gb,
                            int ldgb, const float* style, int sdim, float* y, int ldy, cudaStream_t st,
-                           void* ypre = nullptr, long ypre_rows = 0);
+                           void* ypre = nullptr, long ypre_rows = 0, Fp8Store q = {});
 // cat_style_rows_seg: y[:, d:d+sdim] = style[item]; gap rows of y[:, 0:d+sdim] -> 0
 cudaError_t launch_cat_style(const int* row_item, int rows, int d, const float* style, int sdim, float* y,
                              int ldy, cudaStream_t st);

@@ -26,7 +26,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libkokoro_b200.so")
 
 KK_OK, KK_ERR_INVALID_ARG, KK_ERR_OOM, KK_ERR_CUDA, KK_ERR_TIMEOUT, KK_ERR_IO = range(6)
-KK_PRECISION_FP32, KK_PRECISION_BF16 = 0, 1
+KK_PRECISION_FP32, KK_PRECISION_BF16, KK_PRECISION_FP8 = 0, 1, 2
 KK_OPT_KEEP_AUDIO_ON_DEVICE, KK_OPT_SYNC_EACH_STAGE, KK_OPT_PROFILE, KK_OPT_OUTPUT_PCM16 = 1, 2, 3, 4
 KK_OPT_GAP_CANARY, KK_OPT_NEGCTL_NOMASK, KK_OPT_ATTENTION_F32 = 5, 6, 7
 STATUS_NAMES = {0: "OK", 1: "INVALID_ARG", 2: "OOM", 3: "CUDA", 4: "TIMEOUT", 5: "IO"}
@@ -235,7 +235,7 @@ class GpuKokoro:
 
     def __init__(self, weights_path: str, cuda_ordinal: int = 0, precision: str = "fp32"):
         self.lib = load_library()
-        prec = {"fp32": KK_PRECISION_FP32, "bf16": KK_PRECISION_BF16}[precision]
+        prec = {"fp32": KK_PRECISION_FP32, "bf16": KK_PRECISION_BF16, "fp8": KK_PRECISION_FP8}[precision]
         h = ctypes.c_void_p()
         st = self.lib.kk_create(weights_path.encode(), cuda_ordinal, prec, ctypes.byref(h))
         if st != KK_OK:
