@@ -88,6 +88,11 @@ __device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// The same where no memory is handed over, only TMEM columns, whose reads are complete (tcgen05.wait::ld and the
+// fence before): a release would wait for every load the warp has on its way, 1000 to 3000 cycles here.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 // a load into this CTA's shared memory whose bytes complete on a barrier of either CTA of the pair
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
@@ -99,8 +104,20 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// mbar_wait on a barrier that the other CTA of the cluster arrives on
+// whether a phase of a barrier that the other CTA of the cluster arrives on is complete
 __device__ __forceinline__ bool mbar_try_cluster(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(b)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// the same, asleep until it is or about 0.5 ms have passed
+__device__ __forceinline__ bool mbar_sleep_cluster(uint64_t* b, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -111,11 +128,12 @@ __device__ __forceinline__ bool mbar_try_cluster(uint64_t* b, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// mbar_wait on such a barrier
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* b, uint32_t parity, volatile int* abort_flag, int* err) {
-  if (mbar_try_cluster(b, parity)) return true;
+  if (mbar_sleep_cluster(b, parity)) return true;
   const unsigned long long t0 = tc_now();
   while (true) {
-    if (mbar_try_cluster(b, parity)) return true;
+    if (mbar_sleep_cluster(b, parity)) return true;
     if (*abort_flag) return false;
     if (tc_now() - t0 > KK_WAIT_TIMEOUT_NS) {
       *abort_flag = 1;
@@ -130,12 +148,153 @@ __device__ __forceinline__ void mbar_drain(uint64_t* b, uint32_t parity) {
   while (!mbar_try_sleep(b, parity) && tc_now() - t0 < KK_WAIT_TIMEOUT_NS) {
   }
 }
+// Waits of a whole warp. The lanes meet after each: one that fell behind the lane that issues by a whole ring of
+// stages would wait for a phase whose parity has come round, and what a wait says has to be the same for all.
+__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, int* err) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, err));
+}
+__device__ __forceinline__ bool warp_wait_cluster(uint64_t* b, uint32_t parity, volatile int* abort_flag, int* err) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait_cluster(b, parity, abort_flag, err));
+}
+
+constexpr int SF_RING = 4;  // scale groups (4 blocks of K each) of a pair, in shared memory and TMEM
+
+// ---- scales
+// One warp brings the scales of a CTA's tiles, a group (four blocks of K: a word for each row of x and of W) at a
+// time, into a ring of shared-memory slots in the layout of the TMEM copy. A word waits behind the TMA's boxes on its
+// way from L2 (about 2000 cycles, as long as the MMAs of two or three groups), so the words of the next AHEAD groups
+// are always on their way, in registers; waiting for each group in turn held the MMAs up by half.
+// TILES: the slots of a tile (at most RING / 2 groups) are handed on together, and are free again when the tile before
+// the last is done: two barriers take the place of the ring's (full: [2]; empty: the tiles' accumulators, [2]).
+template <int RING, int ROWS_W, bool TILES = false>
+struct ScaleFeed {
+  static constexpr int NB = (ROWS_W + 127) / 128, BYTES = 512 * (1 + NB), AHEAD = 4;
+  const Fp8Linear& a;
+  uint32_t ring;  // shared-memory address of the slots
+  uint64_t *full, *empty;
+  volatile int* abort_flag;
+  int* err;
+  int lane;
+
+  // start(t, &m0, &n0): rows and columns of a CTA's tile t; its groups are the blocks b_lo, b_lo + 4, .. below b_hi
+  // (b_lo a multiple of 4). Tiles first, first + step, .. below tiles.
+  template <class F>
+  __device__ __forceinline__ void run(int first, int step, int tiles, int b_lo, int b_hi, F&& start) {
+    uint32_t w[AHEAD][4 + 4 * NB];
+    const uint8_t *px[4], *pw[4 * NB];
+    int t = first, b = b_lo;  // of the next group to load
+    auto open = [&] {
+      if (t >= tiles) return;
+      long m0, n0;
+      start(t, &m0, &n0);
+      // (rows past the last take the last one's scales: what they scale is zero, and is not stored)
+#pragma unroll
+      for (int i = 0; i < 4; i++) px[i] = a.x.e + min(m0 + 32 * i + lane, a.m - 1) * a.x.lde;
+#pragma unroll
+      for (int i = 0; i < 4 * NB; i++)  // (a tile may begin inside a block of W's rows)
+        pw[i] = a.w.e + (min(n0 + 32 * i, a.n - 1) >> 7) * a.w.lde;
+    };
+    auto load = [&](uint32_t(&d)[4 + 4 * NB]) {
+      if (t >= tiles) return;
+#pragma unroll
+      for (int i = 0; i < 4; i++) d[i] = __ldg(reinterpret_cast<const uint32_t*>(px[i] + b));
+#pragma unroll
+      for (int i = 0; i < 4 * NB; i++) d[4 + i] = __ldg(reinterpret_cast<const uint32_t*>(pw[i] + b));
+      b += 4;
+      if (b >= b_hi) b = b_lo, t += step, open();
+    };
+    open();
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) load(w[i]);
+    const int groups = (b_hi - b_lo + 3) / 4;  // of a tile
+    long left = first < tiles ? (long)((tiles - first + step - 1) / step) * groups : 0;
+    uint32_t slot = 0, ph = 1;
+    bool used = false;  // the ring has gone round once
+    int in_tile = 0, tile_n = 0;
+    while (true) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; i++) {
+        if (left-- == 0) return;
+        if (TILES) {
+          if (in_tile == 0 && tile_n > 1 && !warp_wait(empty + (tile_n & 1), ((tile_n >> 1) + 1) & 1, abort_flag, err)) return;
+        } else if (used && !warp_wait(empty + slot, ph, abort_flag, err)) {
+          return;
+        }
+        const uint32_t dst = ring + (TILES ? (tile_n & 1) * (RING / 2) + in_tile : slot) * BYTES + lane * 16;
+#pragma unroll
+        for (int j = 0; j < 1 + NB; j++)
+          sts_u4(dst + 512 * j, make_uint4(w[i][4 * j], w[i][4 * j + 1], w[i][4 * j + 2], w[i][4 * j + 3]));
+        if (TILES) {
+          if (++in_tile == groups) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + (tile_n & 1));
+            in_tile = 0, tile_n++;
+          }
+        } else {
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full + slot);
+          if (++slot == RING) slot = 0, ph ^= 1, used = true;
+        }
+        load(w[i]);
+      }
+    }
+  }
+};
+
+// What the MMA warp waits for: stages and scale groups. Asking a barrier takes about 130 cycles, so the next one is asked
+// while the MMAs before it are issued.
+struct MmaFeed {
+  uint64_t *full, *sf_full;
+  int stages;
+  volatile int* abort_flag;
+  int* err;
+  uint32_t s = 0, ph = 0, slot = 0, sph = 0;
+  uint32_t last = 0, last_ph = 0;  // the stage of the last MMAs issued
+  bool any = false, stage_in = false, scales_in = false;
+
+  __device__ __forceinline__ bool stage() {
+    if (!__all_sync(0xFFFFFFFFu, stage_in) && !warp_wait_cluster(full + s, ph, abort_flag, err)) return false;
+    tc_fence_after();
+    last = s, last_ph = ph, any = true;
+    const bool wrap = (int)s + 1 == stages;
+    stage_in = mbar_try_cluster(full + (wrap ? 0 : s + 1), wrap ? ph ^ 1 : ph);
+    return true;
+  }
+  __device__ __forceinline__ void next_stage() {
+    if ((int)++s == stages) s = 0, ph ^= 1;
+  }
+  __device__ __forceinline__ bool scales() {
+    if (!__all_sync(0xFFFFFFFFu, scales_in) && !warp_wait_cluster(sf_full + slot, sph, abort_flag, err)) return false;
+    const bool wrap = slot + 1 == SF_RING;
+    scales_in = mbar_try_cluster(sf_full + (wrap ? 0 : slot + 1), wrap ? sph ^ 1 : sph);
+    return true;
+  }
+  __device__ __forceinline__ void next_scales() {
+    if (++slot == SF_RING) slot = 0, sph ^= 1;
+  }
+};
+
+// In the pair's second CTA: hands each of its groups on to the first CTA, whose MMA warp takes both. (The loading warp
+// could arrive there itself, but a release to the cluster waits for the loads that it has on its way.)
+template <int RING>
+__device__ __forceinline__ void forward_scales(long groups, uint64_t* full, int lane, volatile int* abort_flag, int* err) {
+  uint32_t slot = 0, ph = 0;
+  for (long g = 0; g < groups; g++) {
+    if (!warp_wait(full + slot, ph, abort_flag, err)) return;
+    if (lane == 0) mbar_arrive_cluster(map_rank(full + slot, 0));
+    if (++slot == RING) slot = 0, ph ^= 1;
+  }
+}
+
 struct TcFp8Args {
   Fp8Linear a;
   int* err;
   int kb;              // blocks of 128 columns of K
   int m_tiles, n_tiles;
   int tma_y;           // y (and the residual) can be stored (loaded) by TMA: 16-byte aligned rows
+  int stages;          // (tile kernel)
   int tma_edge;        // so can their last columns: TMA writes whole 16-byte units, so n has to end on one
 };
 
@@ -145,21 +304,19 @@ struct TcFp8Args {
 // L2 per SM and clock at the full MMA rate, more than L2 gives; a pair shares the 256 rows of W (each CTA loads
 // and holds half of them), which takes 64.
 constexpr int TM = 128, TN = 256;  // a CTA's rows, the pair's columns
-constexpr int SF_RING = 4;         // scale groups (4 blocks of K each) in shared memory and TMEM
 constexpr int EPI_WARPS = 8;       // two per TMEM lane quarter, 128 columns each
 constexpr int PAIR_THREADS = 32 * (4 + EPI_WARPS);
 constexpr int BOX = 4096;          // 32 rows of 128 bytes: what an epilogue warp stores (or loads) at once
 
-template <int OUT, bool RES>
+template <int OUT>
 struct PairShape {
-  static constexpr int STAGES = RES ? 4 : 5;
-  static constexpr int NBUF = RES ? 2 : 1;  // boxes of an epilogue warp; two, so that a residual is loaded ahead
+  static constexpr int STAGES = 5;
   static constexpr int A_BYTES = TM * 128, B_BYTES = TN / 2 * 128;
   static constexpr int SF_BYTES = 512 * 3;
   // TMEM columns: the two accumulators share columns 192..255 (see the epilogue); scales behind them
   static constexpr int D1 = 192, SF_COL = D1 + TN, SF_COLS = 12;
   static constexpr int OFF_B = STAGES * A_BYTES, OFF_BOX = OFF_B + STAGES * B_BYTES;
-  static constexpr int OFF_SF = OFF_BOX + EPI_WARPS * NBUF * BOX, OFF_BIAS = OFF_SF + SF_RING * SF_BYTES;
+  static constexpr int OFF_SF = OFF_BOX + EPI_WARPS * BOX, OFF_BIAS = OFF_SF + SF_RING * SF_BYTES;
   static constexpr int OFF_BAR = OFF_BIAS + EPI_WARPS * 128 * 4;
   static constexpr int SMEM = OFF_BAR + 512 + 1024;  // 1024: alignment of the first stage
   static_assert(SF_COL + SF_RING * SF_COLS <= 512, "TMEM columns");
@@ -237,7 +394,8 @@ __device__ __forceinline__ void add_bias32(float* v, const float* bias_s) {
 #pragma unroll
   for (int j = 0; j < 32; j += 4) {
     const float4 b = *reinterpret_cast<const float4*>(bias_s + j);
-    v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
+    add2(v[j], v[j + 1], b.x, b.y);
+    add2(v[j + 2], v[j + 3], b.z, b.w);
   }
 }
 
@@ -255,19 +413,17 @@ __device__ __forceinline__ void tile_at(const TcFp8Args& p, int t, int* mt, int*
 // ring of stages, warp 2 brings the scales, four blocks of K at a time, into shared memory in the layout of the
 // TMEM copy, warps 4..11 are the epilogue (a thread holds 128 columns of one row); warp 1 of the first CTA issues
 // the pair's MMAs. Barriers that the MMA warp waits on live in the first CTA; those it commits to, in both.
-template <int OUT, bool RES>
+template <int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
-                           const __grid_constant__ CUtensorMap ymap, const __grid_constant__ CUtensorMap rmap,
-                           const __grid_constant__ TcFp8Args p) {
-  using S = PairShape<OUT, RES>;
+                           const __grid_constant__ CUtensorMap ymap, const __grid_constant__ TcFp8Args p) {
+  using S = PairShape<OUT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint64_t* full = (uint64_t*)(smem + S::OFF_BAR);
   uint64_t *empty = full + S::STAGES, *sf_full = empty + S::STAGES, *sf_empty = sf_full + SF_RING;
   uint64_t *acc_full = sf_empty + SF_RING, *acc_free = acc_full + 1;
-  uint64_t* res_full = acc_free + 1;  // [EPI_WARPS][NBUF]
-  uint32_t* tmem_slot = (uint32_t*)(res_full + EPI_WARPS * 2);
+  uint32_t* tmem_slot = (uint32_t*)(acc_free + 1);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cta_rank();
@@ -275,10 +431,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
   int* err = p.err ? p.err : &g_fp8_wait_error;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::STAGES; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
-    for (int i = 0; i < SF_RING; i++) mbar_init(sf_full + i, 2), mbar_init(sf_empty + i, 1);
+    for (int i = 0; i < SF_RING; i++) mbar_init(sf_full + i, rank == 0 ? 2 : 1), mbar_init(sf_empty + i, 1);
     mbar_init(acc_full, 1);
     mbar_init(acc_free, 2 * EPI_WARPS);
-    for (int i = 0; i < EPI_WARPS * 2; i++) mbar_init(res_full + i, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -295,7 +450,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
   if (warp == 0) {
-    if (lane == 0) {
+    {
+      const bool lead = elect_one();
       uint32_t it = 0, s = 0, ph = 1;  // ph: of the wait for the stage's last use
       bool ok = true;
       for (int t = first; ok && t < tiles; t += step) {
@@ -303,14 +459,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         tile_at(p, t, &mt, &nt);
         const int m0 = mt * 2 * TM + (int)rank * TM, n0 = nt * TN + (int)rank * (TN / 2);
         for (int b = 0; b < kb; b++, it++) {
-          if (it >= S::STAGES && !mbar_wait(empty + s, ph, abort_flag, err)) {
+          if (it >= S::STAGES && !warp_wait(empty + s, ph, abort_flag, err)) {
             ok = false;
             break;
           }
-          if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * (S::A_BYTES + S::B_BYTES));
-          const uint32_t bar = map_rank(full + s, 0);
-          tma_load_2d_pair(smem + s * S::A_BYTES, &xmap, b * 128, m0, bar);
-          tma_load_2d_pair(smem + S::OFF_B + s * S::B_BYTES, &wmap, b * 128, n0, bar);
+          if (lead) {
+            if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * (S::A_BYTES + S::B_BYTES));
+            const uint32_t bar = map_rank(full + s, 0);
+            tma_load_2d_pair(smem + s * S::A_BYTES, &xmap, b * 128, m0, bar);
+            tma_load_2d_pair(smem + S::OFF_B + s * S::B_BYTES, &wmap, b * 128, n0, bar);
+          }
           if (++s == S::STAGES) s = 0, ph ^= 1;
         }
       }
@@ -334,18 +492,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
       const bool lead = elect_one();
       const uint64_t da0 = sdesc_sw128(smem_u32(smem)), db0 = sdesc_sw128(smem_u32(smem + S::OFF_B));
       const uint64_t dsf0 = sdesc(smem_u32(smem + S::OFF_SF), 128, 128);
-      uint32_t s = 0, ph = 0, slot = 0, sph = 0, tile_n = 0, last = 0, last_ph = 0;
-      bool ok = true, issued = false;
+      MmaFeed f{full, sf_full, S::STAGES, abort_flag, err};
+      uint32_t tile_n = 0;
+      bool ok = true;
       for (int t = first; ok && t < tiles; t += step, tile_n++) {
-        if (tile_n > 0 && !mbar_wait_cluster(acc_free, (tile_n - 1) & 1, abort_flag, err)) break;
+        if (tile_n > 0 && !warp_wait_cluster(acc_free, (tile_n - 1) & 1, abort_flag, err)) break;
         tc_fence_after();
         const uint32_t d = tmem + (tile_n & 1) * S::D1;
         for (int b0 = 0; ok && b0 < kb; b0 += 4) {
-          const uint32_t sfa = tmem + S::SF_COL + slot * S::SF_COLS;
-          ok = mbar_wait_cluster(sf_full + slot, sph, abort_flag, err);
+          ok = f.scales();
           if (!ok) break;
+          const uint32_t sfa = tmem + S::SF_COL + f.slot * S::SF_COLS;
           if (lead) {
-            const uint64_t dsf = dsf0 + slot * (S::SF_BYTES >> 4);
+            const uint64_t dsf = dsf0 + f.slot * (S::SF_BYTES >> 4);
             tmem_cp_scales_pair(sfa, dsf);
             tmem_cp_scales_pair(sfa + 4, dsf + (512 >> 4));
             tmem_cp_scales_pair(sfa + 8, dsf + (1024 >> 4));
@@ -353,68 +512,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             if (b0 + j >= kb) break;
-            ok = mbar_wait_cluster(full + s, ph, abort_flag, err);
+            ok = f.stage();
             if (!ok) break;
-            tc_fence_after();
             if (lead) {
-              const uint64_t da = da0 + s * (S::A_BYTES >> 4), db = db0 + s * (S::B_BYTES >> 4);
+              const uint64_t da = da0 + f.s * (S::A_BYTES >> 4), db = db0 + f.s * (S::B_BYTES >> 4);
 #pragma unroll
               for (int k = 0; k < 4; k++)
                 mma_mxf8_pair(d, da + 2 * k, db + 2 * k, idesc_mxf8(2 * TM, TN, j), sfa, sfa + 4, j > 0 || k > 0 || b0 > 0);
-              mma_commit_pair(empty + s);
+              mma_commit_pair(empty + f.s);
             }
-            issued = true, last = s, last_ph = ph;
-            if (++s == S::STAGES) s = 0, ph ^= 1;
+            f.next_stage();
           }
-          if (ok && lead) mma_commit_pair(sf_empty + slot);
-          if (++slot == SF_RING) slot = 0, sph ^= 1;
+          if (ok && lead) mma_commit_pair(sf_empty + f.slot);
+          f.next_scales();
         }
         if (ok && lead) mma_commit_pair(acc_full);
       }
-      if (*abort_flag && issued) mbar_drain(empty + last, last_ph);  // MMAs in flight end before their operands and TMEM go
+      if (*abort_flag && f.any) mbar_drain(empty + f.last, f.last_ph);  // MMAs in flight end before their operands and TMEM go
+    } else if (first < tiles) {
+      forward_scales<SF_RING>((long)((tiles - first + step - 1) / step) * ((kb + 3) / 4), sf_full, lane, abort_flag, err);
     }
   } else if (warp == 2) {
-    uint32_t g = 0;
-    bool ok = true;
-    for (int t = first; ok && t < tiles; t += step) {
+    ScaleFeed<SF_RING, TN> feed{a, smem_u32(smem + S::OFF_SF), sf_full, sf_empty, abort_flag, err, lane};
+    feed.run(first, step, tiles, 0, kb, [&](int t, long* m0, long* n0) {
       int mt, nt;
       tile_at(p, t, &mt, &nt);
-      const long m0 = (long)mt * 2 * TM + rank * TM, n0 = (long)nt * TN;
-      for (int b = 0; b < kb; b += 4, g++) {
-        uint32_t wx[4], ww[2];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const long r = m0 + 32 * i + lane;
-          wx[i] = r < a.m ? *reinterpret_cast<const uint32_t*>(a.x.e + r * a.x.lde + b) : 0u;
-        }
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const long c = n0 + 128 * j;
-          ww[j] = c < a.n ? *reinterpret_cast<const uint32_t*>(a.w.e + (c >> 7) * a.w.lde + b) : 0u;
-        }
-        const uint32_t slot = g % SF_RING;
-        if (g >= SF_RING) {
-          ok = __all_sync(0xFFFFFFFFu, mbar_wait(sf_empty + slot, (g / SF_RING + 1) & 1, abort_flag, err));
-          if (!ok) break;
-        }
-        const uint32_t sf = smem_u32(smem + S::OFF_SF + slot * S::SF_BYTES) + lane * 16;
-        sts_u4(sf, make_uint4(wx[0], wx[1], wx[2], wx[3]));
-        sts_u4(sf + 512, make_uint4(ww[0], ww[0], ww[0], ww[0]));
-        sts_u4(sf + 1024, make_uint4(ww[1], ww[1], ww[1], ww[1]));
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_rank(sf_full + slot, 0));
-      }
-    }
+      *m0 = (long)mt * 2 * TM + rank * TM, *n0 = (long)nt * TN;
+    });
   } else if (warp >= 4) {
     const int ew = warp - 4, half = ew >> 2;
     float* bias_s = (float*)(smem + S::OFF_BIAS) + ew * 128;
-    uint8_t* box = smem + S::OFF_BOX + ew * S::NBUF * BOX;
+    uint8_t* box = smem + S::OFF_BOX + ew * BOX;
     const uint32_t row_s = smem_u32(box) + lane * 128;  // this thread's row of the box; 16-byte units swizzled by row
     const uint32_t acc_free0 = map_rank(acc_free, 0);
     constexpr int BC = OUT == FP8_F32 ? 32 : (OUT == FP8_BF16 ? 64 : 128);  // columns of a box
     constexpr int NCH = 128 / BC;
-    uint32_t tile_n = 0, nres = 0;
+    uint32_t tile_n = 0;
     bool ok = true;
     float4 bias_r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (first < tiles) {
@@ -437,21 +570,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
       const int live = r0 < a.m && c0 < a.n ? (int)min((long)NCH, (a.n - c0 + BC - 1) / BC) : 0;
       const int boxes = !p.tma_y || live == 0 ? 0 : (p.tma_edge ? live : (int)min((long)live, (a.n - c0) / BC));
       // (boxes are used in the order ch0, ch0 + 1, .. round to ch0 - 1)
-      if constexpr (RES) {
-        // the first boxes' residuals, while the tile's MMAs run; a box is free once its last store has read it
-        if (boxes > 0 && lane == 0) {
-          bulk_wait_all_read();
-          int q = 0;
-          for (int i = 0; i < NCH && q < 2; i++) {
-            const int ch = (i + ch0) % NCH;
-            if (ch >= boxes) continue;
-            const uint32_t n = nres + q, bf = n & 1;
-            mbar_arrive_expect_tx(res_full + ew * 2 + bf, BOX);
-            tma_load_2d(box + bf * BOX, &rmap, (int)c0 + ch * BC, (int)r0, res_full + ew * 2 + bf);
-            q++;
-          }
-        }
-      }
       __syncwarp();
       *reinterpret_cast<float4*>(bias_s + 4 * lane) = bias_r;
       __syncwarp();
@@ -460,11 +578,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         tile_at(p, t + step, &mt1, &nt1);
         bias_r = load_bias(a, (long)nt1 * TN + half * 128 + 4 * lane);
       }
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait(acc_full, tile_n & 1, abort_flag, err));
+      ok = warp_wait(acc_full, tile_n & 1, abort_flag, err);
       if (!ok) break;
       tc_fence_after();
       const uint32_t d = tmem + ((uint32_t)(ew & 3) << 21) + (tile_n & 1) * S::D1 + half * 128;
-      if (!shares && lane == 0) mbar_arrive_cluster(acc_free0);
+      if (!shares && lane == 0) mbar_arrive_cluster_relaxed(acc_free0);
       if constexpr (OUT == FP8_E4M3) {
         float v[128];
         tmem_ld64(d, v);
@@ -472,13 +590,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         if (shares) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(acc_free0);
+          if (lane == 0) mbar_arrive_cluster_relaxed(acc_free0);
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) add_bias32(v + 32 * i, bias_s + 32 * i);
         if (a.gelu) {
 #pragma unroll
-          for (int i = 0; i < 128; i++) v[i] = gelu_fast(v[i]);
+          for (int i = 0; i < 128; i += 2) gelu_fast2(v[i], v[i + 1]);
         }
         if (live) {
           uint32_t u[32];
@@ -504,21 +622,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
           }
         }
       } else {
-        int used = 0;
 #pragma unroll 1
         for (int i = 0; i < NCH; i++) {
           const int ch = (i + ch0) % NCH;
-          const uint32_t bf = RES ? (nres & 1) : 0;
-          const uint32_t row_b = row_s + bf * BOX;
           const bool on = ch < live, tma = ch < boxes;
           if (tma) {
-            if constexpr (RES) {
-              ok = __all_sync(0xFFFFFFFFu, mbar_wait(res_full + ew * 2 + bf, (nres >> 1) & 1, abort_flag, err));
-              if (!ok) break;
-            } else {
-              if (lane == 0) bulk_wait_all_read();
-              __syncwarp();
-            }
+            if (lane == 0) bulk_wait_all_read();
+            __syncwarp();
           }
 #pragma unroll
           for (int h = 0; h < BC / 32; h++) {
@@ -528,13 +638,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             if (shares && (BC == 32 ? i == 1 : i == 0 && h == 1)) {
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive_cluster(acc_free0);
+              if (lane == 0) mbar_arrive_cluster_relaxed(acc_free0);
             }
             if (!on) continue;
             add_bias32(v, bias_s + c);
             if (a.gelu) {
 #pragma unroll
-              for (int j = 0; j < 32; j++) v[j] = gelu_fast(v[j]);
+              for (int j = 0; j < 32; j += 2) gelu_fast2(v[j], v[j + 1]);
             }
             if (!tma) {
               if (c0 + c < a.n) {
@@ -548,28 +658,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             if constexpr (OUT == FP8_F32) {
 #pragma unroll
               for (int q = 0; q < 8; q++) {
-                const uint32_t at = row_b + ((q ^ (lane & 7)) << 4);
-                float4 o = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-                if constexpr (RES) {
-                  const float4 r = lds_f4(at);
-                  o.x += r.x, o.y += r.y, o.z += r.z, o.w += r.w;
-                }
-                sts_u4(at, make_uint4(__float_as_uint(o.x), __float_as_uint(o.y), __float_as_uint(o.z), __float_as_uint(o.w)));
+                sts_u4(row_s + ((q ^ (lane & 7)) << 4),
+                       make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]),
+                                  __float_as_uint(v[4 * q + 3])));
               }
             } else {
 #pragma unroll
               for (int q = 0; q < 4; q++) {
-                const uint32_t at = row_b + (((4 * h + q) ^ (lane & 7)) << 4);
-                if constexpr (RES) {
-                  const float4 r = lds_f4(at);
-                  const uint32_t u[4] = {__float_as_uint(r.x), __float_as_uint(r.y), __float_as_uint(r.z), __float_as_uint(r.w)};
-#pragma unroll
-                  for (int k = 0; k < 4; k++) {
-                    v[8 * q + 2 * k] += __uint_as_float(u[k] << 16);
-                    v[8 * q + 2 * k + 1] += __uint_as_float(u[k] & 0xFFFF0000u);
-                  }
-                }
-                sts_u4(at, make_uint4(bf16x2(v[8 * q], v[8 * q + 1]), bf16x2(v[8 * q + 2], v[8 * q + 3]),
+                sts_u4(row_s + (((4 * h + q) ^ (lane & 7)) << 4), make_uint4(bf16x2(v[8 * q], v[8 * q + 1]), bf16x2(v[8 * q + 2], v[8 * q + 3]),
                                       bf16x2(v[8 * q + 4], v[8 * q + 5]), bf16x2(v[8 * q + 6], v[8 * q + 7])));
               }
             }
@@ -578,34 +674,402 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&ymap, (int)c0 + ch * BC, (int)r0, box + bf * BOX);
+            tma_store_2d(&ymap, (int)c0 + ch * BC, (int)r0, box);
             bulk_commit();
-          }
-          nres++;
-          used++;
-          if constexpr (RES) {
-            // the box of this store takes the residual after next, if the tile has one (boxes in use order)
-            if (used + 1 < boxes && lane == 0) {
-              int seen = 0, nx = 0;
-              for (int k = 0; k < NCH; k++) {
-                const int cc = (k + ch0) % NCH;
-                if (cc >= boxes) continue;
-                if (seen == used + 1) nx = cc;
-                seen++;
-              }
-              bulk_wait_all_read();
-              mbar_arrive_expect_tx(res_full + ew * 2 + bf, BOX);
-              tma_load_2d(box + bf * BOX, &rmap, (int)c0 + nx * BC, (int)r0, res_full + ew * 2 + bf);
-            }
           }
         }
       }
       tc_fence_before();  // this tile's TMEM reads before the arrivals of the next
     }
+    if (lane == 0) bulk_wait_all();
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// ---- large layers with few blocks of K, or with a residual: two whole accumulators
+//
+// With K = 768 a tile's MMAs take 1.6 us, and the kernel above stands still for another between two tiles, while
+// their shared columns are handed over; with a residual its two boxes a warp are too few to load it ahead. Here the
+// pair's tile is 192 columns (128 when the result is quantised: a block is 128), so that both accumulators fit TMEM
+// side by side, and a warp has a box for each of its columns of a tile. Where the pair's columns of W fit shared
+// memory (STAT) they are loaded once and the pair takes one column of tiles; then only x is read again for each.
+// f32 / bf16: 12 epilogue warps, three for each lane quarter, 64 columns each. e4m3: 8, in two groups that take
+// turns (a thread holds a row's 128 columns), each with an accumulator of its own.
+template <int OUT, bool RES, bool STAT>
+struct TileShape {
+  static constexpr int N = OUT == FP8_E4M3 ? 128 : 192;
+  static constexpr int EPI = OUT == FP8_E4M3 ? 8 : 12;
+  static constexpr int THREADS = 32 * (4 + EPI);
+  static constexpr int COLS = OUT == FP8_E4M3 ? 128 : 64;                          // of an epilogue thread
+  static constexpr int BC = OUT == FP8_F32 ? 32 : (OUT == FP8_BF16 ? 64 : 128);    // columns of a box
+  static constexpr int NBOX = COLS / BC;
+  static constexpr int KB_MAX = OUT == FP8_F32 ? 6 : 8;          // blocks of K that STAT holds
+  static constexpr int BPS = STAT && OUT != FP8_F32 ? 2 : 1;     // blocks of a stage
+  static constexpr int MAX_STAGES = 10;
+  static constexpr int A_BYTES = TM * 128, B_BYTES = N / 2 * 128;
+  static constexpr int NB = (N + 127) / 128;
+  static constexpr int SF_BYTES = 512 * (1 + NB), SF_COLS = 4 * (1 + NB), SF_COL = 2 * N;
+  static constexpr int OFF_SF = EPI * NBOX * BOX, OFF_BIAS = OFF_SF + SF_RING * SF_BYTES;
+  static constexpr int OFF_BAR = OFF_BIAS + EPI * COLS * 4;
+  static constexpr int OFF_BOX = 0, OFF_A = (OFF_BAR + 512 + 1023) / 1024 * 1024;  // then the operands, in what is left
+  static constexpr int ROOM = 227 * 1024 - 1024 - OFF_A;
+  static int stages(int kb) {
+    const int n = STAT ? (ROOM - kb * B_BYTES) / (BPS * A_BYTES) : ROOM / (A_BYTES + B_BYTES);
+    return n < MAX_STAGES ? n : MAX_STAGES;
+  }
+  static_assert(SF_COL + SF_RING * SF_COLS <= 512, "TMEM columns");
+  static_assert(ROOM >= (STAT ? KB_MAX * B_BYTES + 2 * BPS * A_BYTES : 4 * (A_BYTES + B_BYTES)), "shared memory");
+  static_assert(!STAT || KB_MAX <= 4 * (SF_RING / 2), "a tile's scale groups fit half the ring");
+};
+
+template <int OUT, bool RES, bool STAT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TileShape<OUT, RES, STAT>::THREADS, 1)
+    fp8_linear_tile_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
+                           const __grid_constant__ CUtensorMap ymap, const __grid_constant__ CUtensorMap rmap,
+                           const __grid_constant__ TcFp8Args p) {
+  using S = TileShape<OUT, RES, STAT>;
+  constexpr bool Q = OUT == FP8_E4M3;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint64_t* full = (uint64_t*)(smem + S::OFF_BAR);
+  uint64_t *empty = full + S::MAX_STAGES, *sf_full = empty + S::MAX_STAGES, *sf_empty = sf_full + SF_RING;
+  uint64_t *acc_full = sf_empty + SF_RING, *acc_free = acc_full + 2;
+  uint64_t* res_full = acc_free + 2;  // [EPI][NBOX]
+  uint32_t* tmem_slot = (uint32_t*)(res_full + S::EPI * S::NBOX);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t off_a = S::OFF_A, off_b = S::OFF_A + p.stages * S::BPS * S::A_BYTES;  // the operands: x, then W
+  const uint32_t rank = cta_rank();
+  const Fp8Linear& a = p.a;
+  int* err = p.err ? p.err : &g_fp8_wait_error;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::MAX_STAGES; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
+    for (int i = 0; i < SF_RING; i++) mbar_init(sf_full + i, rank == 0 ? 2 : 1), mbar_init(sf_empty + i, 1);
+    for (int i = 0; i < 2; i++) mbar_init(acc_full + i, 1), mbar_init(acc_free + i, Q ? S::EPI : 2 * S::EPI);
+    for (int i = 0; i < S::EPI * S::NBOX; i++) mbar_init(res_full + i, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int kb = p.kb, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  // STAT: a pair keeps column pair % n_tiles of the tiles and takes every (pairs / n_tiles)-th row of it, so that
+  // all columns of a row of tiles are worked on at about the same time and x comes from HBM once
+  const int first = STAT ? pair / p.n_tiles : pair, step = STAT ? pairs / p.n_tiles : pairs;
+  const int tiles = STAT ? p.m_tiles : p.m_tiles * p.n_tiles;
+  auto tile = [&](int t, int* mt, int* nt) {
+    if (STAT)
+      *mt = t, *nt = pair % p.n_tiles;
+    else
+      tile_at(p, t, mt, nt);
+  };
+
+  if (warp == 0) {
+    {
+      const bool lead = elect_one();
+      uint32_t it = 0, s = 0, ph = 1;
+      const uint32_t stages = p.stages;
+      bool ok = true;
+      for (int t = first; ok && t < tiles; t += step) {
+        int mt, nt;
+        tile(t, &mt, &nt);
+        const int m0 = mt * 2 * TM + (int)rank * TM, n0 = nt * S::N + (int)rank * (S::N / 2);
+        const bool load_w = !STAT || t == first;
+        for (int b = 0; b < kb; b += S::BPS, it++) {
+          if (it >= stages && !warp_wait(empty + s, ph, abort_flag, err)) {
+            ok = false;
+            break;
+          }
+          if (lead) {
+            const int blocks = min(S::BPS, kb - b);
+            if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * blocks * (S::A_BYTES + (load_w ? S::B_BYTES : 0)));
+            const uint32_t bar = map_rank(full + s, 0);
+#pragma unroll
+            for (int i = 0; i < S::BPS; i++) {
+              if (i >= blocks) break;
+              tma_load_2d_pair(smem + off_a + (s * S::BPS + i) * S::A_BYTES, &xmap, (b + i) * 128, m0, bar);
+              if (load_w) tma_load_2d_pair(smem + off_b + (STAT ? b + i : s) * S::B_BYTES, &wmap, (b + i) * 128, n0, bar);
+            }
+          }
+          if (++s == stages) s = 0, ph ^= 1;
+        }
+      }
+      // After an expired wait, loads still in flight land before the shared memory goes: the first CTA sees them
+      // complete, the second, whose loads complete there, waits far longer than a load takes.
+      if (!ok) {
+        if (rank == 0) {
+          for (uint32_t i = it > stages ? it - stages : 0; i < it; i++) mbar_drain(full + i % stages, (i / stages) & 1);
+        } else {
+          const unsigned long long t0 = tc_now();
+          while (tc_now() - t0 < 1000000ull) __nanosleep(1000);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const bool lead = elect_one();
+      const uint64_t da0 = sdesc_sw128(smem_u32(smem + off_a)), db0 = sdesc_sw128(smem_u32(smem + off_b));
+      const uint64_t dsf0 = sdesc(smem_u32(smem + S::OFF_SF), 128, 128);
+      MmaFeed f{full, sf_full, p.stages, abort_flag, err};
+      uint32_t tile_n = 0;
+      bool ok = true;
+      for (int t = first; ok && t < tiles; t += step, tile_n++) {
+        const uint32_t buf = tile_n & 1;
+        if (tile_n > 1 && !warp_wait_cluster(acc_free + buf, ((tile_n >> 1) + 1) & 1, abort_flag, err)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + buf * S::N;
+        if constexpr (STAT) {
+          // all of the tile's scales, then its stages: few waits and commits a tile, because they, not the MMAs, are
+          // what takes this warp's time
+          ok = warp_wait_cluster(sf_full + buf, (tile_n >> 1) & 1, abort_flag, err);
+          if (!ok) break;
+          const uint32_t sf0 = tmem + S::SF_COL + buf * (SF_RING / 2) * S::SF_COLS;
+          if (lead) {
+            for (int g = 0; 4 * g < kb; g++) {
+              const uint64_t dsf = dsf0 + (buf * (SF_RING / 2) + g) * (S::SF_BYTES >> 4);
+#pragma unroll
+              for (int i = 0; i < 1 + S::NB; i++) tmem_cp_scales_pair(sf0 + g * S::SF_COLS + 4 * i, dsf + (512 >> 4) * i);
+            }
+          }
+#pragma unroll 4
+          for (int b = 0; b < kb; b += S::BPS) {
+            ok = f.stage();
+            if (!ok) break;
+            if (lead) {
+#pragma unroll
+              for (int i = 0; i < S::BPS; i++) {
+                if (b + i >= kb) break;
+                const uint64_t da = da0 + (f.s * S::BPS + i) * (S::A_BYTES >> 4), db = db0 + (b + i) * (S::B_BYTES >> 4);
+                const uint32_t sfa = sf0 + ((b + i) >> 2) * S::SF_COLS, sel = (b + i) & 3;
+                const uint32_t id = idesc_mxf8(2 * TM, S::N, 0) | (sel << 4) | (sel << 29);
+#pragma unroll
+                for (int j = 0; j < 4; j++) mma_mxf8_pair(d, da + 2 * j, db + 2 * j, id, sfa, sfa + 4, j > 0 || b + i > 0);
+              }
+              mma_commit_pair(empty + f.s);
+            }
+            f.next_stage();
+          }
+        } else {
+          for (int b0 = 0; ok && b0 < kb; b0 += 4) {
+            ok = f.scales();
+            if (!ok) break;
+            const uint32_t sfa = tmem + S::SF_COL + f.slot * S::SF_COLS;
+            if (lead) {
+              const uint64_t dsf = dsf0 + f.slot * (S::SF_BYTES >> 4);
+  #pragma unroll
+              for (int i = 0; i < 1 + S::NB; i++) tmem_cp_scales_pair(sfa + 4 * i, dsf + (512 >> 4) * i);
+            }
+  #pragma unroll
+            for (int j = 0; j < 4; j++) {
+              if (b0 + j >= kb) break;
+              ok = f.stage();
+              if (!ok) break;
+              if (lead) {
+                const uint64_t da = da0 + f.s * (S::A_BYTES >> 4), db = db0 + (STAT ? b0 + j : f.s) * (S::B_BYTES >> 4);
+  #pragma unroll
+                for (int k = 0; k < 4; k++)
+                  mma_mxf8_pair(d, da + 2 * k, db + 2 * k, idesc_mxf8(2 * TM, S::N, j), sfa, sfa + 4, j > 0 || k > 0 || b0 > 0);
+                mma_commit_pair(empty + f.s);
+              }
+              f.next_stage();
+            }
+            if (ok && lead) mma_commit_pair(sf_empty + f.slot);
+            f.next_scales();
+          }
+        }
+        if (ok && lead) mma_commit_pair(acc_full + buf);
+      }
+      if (*abort_flag && f.any) mbar_drain(empty + f.last, f.last_ph);  // MMAs in flight end before their operands and TMEM go
+    } else if (first < tiles) {
+      const long n = (tiles - first + step - 1) / step;
+      if (STAT)
+        forward_scales<2>(n, sf_full, lane, abort_flag, err);
+      else
+        forward_scales<SF_RING>(n * ((kb + 3) / 4), sf_full, lane, abort_flag, err);
+    }
+  } else if (warp == 2) {
+    ScaleFeed<SF_RING, S::N, STAT> feed{a, smem_u32(smem + S::OFF_SF), sf_full, STAT ? acc_full : sf_empty, abort_flag, err, lane};
+    feed.run(first, step, tiles, 0, kb, [&](int t, long* m0, long* n0) {
+      int mt, nt;
+      tile(t, &mt, &nt);
+      *m0 = (long)mt * 2 * TM + rank * TM, *n0 = (long)nt * S::N;
+    });
+  } else if (warp >= 4) {
+    const int ew = warp - 4, group = ew >> 2, q = ew & 3;
+    constexpr int PB = S::COLS / 32;  // bias values of a lane
+    float* bias_s = (float*)(smem + S::OFF_BIAS) + ew * S::COLS;
+    uint8_t* box = smem + S::OFF_BOX + ew * S::NBOX * BOX;
+    const uint32_t row_s = smem_u32(box) + lane * 128;  // this thread's row of a box; 16-byte units swizzled by row
+    const int col = Q ? 0 : group * S::COLS;            // of the tile
+    uint32_t tile_n = 0, nres = 0;
+    bool ok = true;
+    float bias_r[PB];
+    auto load_bias_r = [&](int t) {
+      int mt, nt;
+      tile(t, &mt, &nt);
+      const long c = (long)nt * S::N + col + PB * lane;
+#pragma unroll
+      for (int i = 0; i < PB; i++) bias_r[i] = a.bias && c + i < a.n ? a.bias[c + i] : 0.0f;
+    };
+    // e4m3: this group takes every second tile of the pair's
+    const int t0 = Q ? first + group * step : first, tstep = Q ? 2 * step : step;
+    if (t0 < tiles) load_bias_r(t0);
+    tile_n = Q ? group : 0;
+    for (int t = t0; ok && t < tiles; t += tstep, tile_n += Q ? 2 : 1) {
+      int mt, nt;
+      tile(t, &mt, &nt);
+      const long r0 = (long)mt * 2 * TM + rank * TM + q * 32;
+      const long c0 = (long)nt * S::N + col;
+      const uint32_t buf = tile_n & 1;
+      // boxes with columns, and how many of them go by TMA
+      const int live = r0 < a.m && c0 < a.n ? (int)min((long)S::NBOX, (a.n - c0 + S::BC - 1) / S::BC) : 0;
+      const int boxes = !p.tma_y || live == 0 ? 0 : (p.tma_edge ? live : (int)min((long)live, (a.n - c0) / S::BC));
+      if (lane == 0) bulk_wait_all_read();  // the boxes are free once the last tile's stores have read them
+      if constexpr (RES) {                  // the residual comes while the tile's MMAs run
+        if (lane == 0) {
+          for (int i = 0; i < boxes; i++) {
+            mbar_arrive_expect_tx(res_full + ew * S::NBOX + i, BOX);
+            tma_load_2d(box + i * BOX, &rmap, (int)c0 + i * S::BC, (int)r0, res_full + ew * S::NBOX + i);
+          }
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < PB; i++) bias_s[PB * lane + i] = bias_r[i];
+      __syncwarp();
+      if (!STAT && t + tstep < tiles) load_bias_r(t + tstep);  // the next tile's arrives during this one
+      ok = warp_wait(acc_full + buf, (tile_n >> 1) & 1, abort_flag, err);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t d = tmem + ((uint32_t)q << 21) + buf * S::N + col;
+      const uint32_t free0 = map_rank(acc_free + buf, 0);
+      if constexpr (Q) {
+        float v[128];
+        tmem_ld64(d, v);
+        tmem_ld64(d + 64, v + 64);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(free0);
+#pragma unroll
+        for (int i = 0; i < 4; i++) add_bias32(v + 32 * i, bias_s + 32 * i);
+        if (a.gelu) {
+#pragma unroll
+          for (int i = 0; i < 128; i += 2) gelu_fast2(v[i], v[i + 1]);
+        }
+        if (live) {
+          uint32_t u[32];
+          const int e = quantize_block(v, u);
+          if (r0 + lane < a.m) a.q.e[(r0 + lane) * a.q.lde + (c0 >> 7)] = (uint8_t)e;
+          if (boxes) {
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+              sts_u4(row_s + ((k ^ (lane & 7)) << 4), make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]));
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&ymap, (int)c0, (int)r0, box);
+              bulk_commit();
+            }
+          } else if (r0 + lane < a.m) {  // the last columns
+            uint8_t* row = a.q.v + (r0 + lane) * a.q.ldv + c0;
+#pragma unroll
+            for (int i = 0; i < 128; i++)
+              if (c0 + i < a.n) row[i] = (uint8_t)(u[i >> 2] >> (8 * (i & 3)));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {  // 32 columns at a time
+          const int c = 32 * h, bx = c / S::BC;
+          const bool on = bx < live, tma = bx < boxes;
+          float v[32];
+          tmem_ld32(d + c, v);
+          if (h == 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(free0);
+          }
+          if (!on) continue;
+          add_bias32(v, bias_s + c);
+          if (a.gelu) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) gelu_fast2(v[j], v[j + 1]);
+          }
+          if (!tma) {
+            if (c0 + c < a.n) {
+              if constexpr (OUT == FP8_F32)
+                store_any<float>(a, v, r0, c0 + c, lane);
+              else
+                store_any<__nv_bfloat16>(a, v, r0, c0 + c, lane);
+            }
+            continue;
+          }
+          if constexpr (RES) {
+            if (c % S::BC == 0) {
+              ok = warp_wait(res_full + ew * S::NBOX + bx, (nres >> bx) & 1, abort_flag, err);
+              if (!ok) break;
+              nres ^= 1u << bx;
+            }
+          }
+          const uint32_t row_b = row_s + bx * BOX;
+          if constexpr (OUT == FP8_F32) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+              const uint32_t at = row_b + ((k ^ (lane & 7)) << 4);
+              float4 o = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+              if constexpr (RES) {
+                const float4 r = lds_f4(at);
+                o.x += r.x, o.y += r.y, o.z += r.z, o.w += r.w;
+              }
+              sts_u4(at, make_uint4(__float_as_uint(o.x), __float_as_uint(o.y), __float_as_uint(o.z), __float_as_uint(o.w)));
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const uint32_t at = row_b + (((4 * h + k) ^ (lane & 7)) << 4);
+              if constexpr (RES) {
+                const float4 r = lds_f4(at);
+                const uint32_t u[4] = {__float_as_uint(r.x), __float_as_uint(r.y), __float_as_uint(r.z), __float_as_uint(r.w)};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                  v[8 * k + 2 * i] += __uint_as_float(u[i] << 16);
+                  v[8 * k + 2 * i + 1] += __uint_as_float(u[i] & 0xFFFF0000u);
+                }
+              }
+              sts_u4(at, make_uint4(bf16x2(v[8 * k], v[8 * k + 1]), bf16x2(v[8 * k + 2], v[8 * k + 3]),
+                                    bf16x2(v[8 * k + 4], v[8 * k + 5]), bf16x2(v[8 * k + 6], v[8 * k + 7])));
+            }
+          }
+          if ((c + 32) % S::BC == 0) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&ymap, (int)c0 + bx * S::BC, (int)r0, box + bx * BOX);
+              bulk_commit();
+            }
+          }
+        }
+      }
+      tc_fence_before();
+    }
     if (lane == 0) {
       if (!ok && RES) {  // residual boxes still in flight land before the shared memory goes
-        const unsigned long long t0 = tc_now();
-        while (tc_now() - t0 < 1000000ull) __nanosleep(1000);
+        const unsigned long long w0 = tc_now();
+        while (tc_now() - w0 < 1000000ull) __nanosleep(1000);
       }
       bulk_wait_all();
     }
@@ -737,7 +1201,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
       if ((b & 3) == 0 || b == b_lo) {
         if (slot >= 0 && lead) mma_commit(sf_empty + slot);
         if (++slot == SPLIT_RING) slot = 0, sph ^= 1;
-        ok = mbar_wait(sf_full + slot, sph, abort_flag, err);
+        ok = warp_wait(sf_full + slot, sph, abort_flag, err);
         if (!ok) break;
         sfa = tmem + NT + slot * S::SF_COLS;
         if (lead) {
@@ -746,7 +1210,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
             tmem_cp_scales(sfa + 4 * i, dsf0 + ((slot * S::SF_BYTES + 512 * i) >> 4));
         }
       }
-      ok = mbar_wait(full + s, ph, abort_flag, err);
+      ok = warp_wait(full + s, ph, abort_flag, err);
       if (!ok) break;
       tc_fence_after();
       if (lead) {
@@ -762,31 +1226,10 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     if (ok && lead) mma_commit(&acc_full);
     if (!ok && last >= 0) mbar_drain(empty + last, last_ph);  // MMAs in flight end before their operands and TMEM go
   } else if (warp == 2) {
-    int slot = 0, ph = 1, n = 0;
-    for (int b = b_lo & ~3; b < b_hi; b += 4, n++) {
-      uint32_t wx[4], ww[S::NB][4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int r = 32 * i + lane;
-        wx[i] = r < rows ? *reinterpret_cast<const uint32_t*>(a.x.e + (m0 + r) * a.x.lde + b) : 0u;
-#pragma unroll
-        for (int j = 0; j < S::NB; j++) {
-          const long cc = n0 + 128 * j + 32 * i;
-          ww[j][i] = cc < a.n ? *reinterpret_cast<const uint32_t*>(a.w.e + (cc >> 7) * a.w.lde + b) : 0u;
-        }
-      }
-      if (n >= SPLIT_RING && !__all_sync(0xFFFFFFFFu, mbar_wait(sf_empty + slot, ph, abort_flag, err))) break;
-      const uint32_t sf = smem_u32(sf_s) + slot * S::SF_BYTES + lane * 16;
-      sts_u4(sf, make_uint4(wx[0], wx[1], wx[2], wx[3]));
-#pragma unroll
-      for (int j = 0; j < S::NB; j++) sts_u4(sf + 512 * (1 + j), make_uint4(ww[j][0], ww[j][1], ww[j][2], ww[j][3]));
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(sf_full + slot);
-      if (++slot == SPLIT_RING) slot = 0, ph ^= 1;
-    }
+    ScaleFeed<SPLIT_RING, NT> feed{a, smem_u32(sf_s), sf_full, sf_empty, abort_flag, err, lane};
+    feed.run(0, 1, 1, b_lo & ~3, b_hi, [&](int, long* m, long* n) { *m = m0, *n = n0; });
   } else if (warp >= 4) {
-    const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(&acc_full, 0, abort_flag, err));
+    const bool ok = warp_wait(&acc_full, 0, abort_flag, err);
     tc_fence_after();
     const int q = warp & 3, r = 32 * q + lane;
     if (ok && 32 * q < rows) {  // the stages' memory is free now: the MMAs that read it are done
@@ -856,10 +1299,11 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
         if (i < splits) v[0] += f[i].x, v[1] += f[i].y, v[2] += f[i].z, v[3] += f[i].w;
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      v[i] += bias_r[i];
-      if (a.gelu) v[i] = gelu_fast(v[i]);
-      if (OUT != FP8_E4M3) v[i] += res_r[i];
+    for (int i = 0; i < 4; i++) v[i] += bias_r[i];
+    if (a.gelu) gelu_fast2(v[0], v[1]), gelu_fast2(v[2], v[3]);
+    if (OUT != FP8_E4M3) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] += res_r[i];
     }
     if constexpr (OUT == FP8_F32) {
       float* y = (float*)a.y + m * a.ldy + n;
@@ -963,36 +1407,71 @@ static cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>* done) 
   return e;
 }
 
-template <int OUT, bool RES>
+// Tensor maps of x, W, y and the residual for a kernel of pairs with tiles of `cols` columns.
+struct PairMaps {
+  CUtensorMap x, w, y, r;
+};
+static bool make_pair_maps(const Fp8Linear& a, int cols, TcFp8Args* p, PairMaps* m) {
+  const bool q = a.y_type == FP8_E4M3;
+  const int es = a.y_type == FP8_F32 ? 4 : (a.y_type == FP8_BF16 ? 2 : 1);
+  const void* y = q ? a.q.v : a.y;
+  const long ldy = q ? a.q.ldv : a.ldy;
+  p->a = a;
+  p->kb = (int)((a.k + 127) / 128);
+  p->m_tiles = (int)((a.m + 2 * TM - 1) / (2 * TM));
+  p->n_tiles = (int)((a.n + cols - 1) / cols);
+  p->tma_y = ((uintptr_t)y | (size_t)ldy * es) % 16 == 0 && (!a.res || ((uintptr_t)a.res | (size_t)a.ldr * es) % 16 == 0);
+  p->tma_edge = (size_t)a.n * es % 16 == 0;
+  if (!make_map(&m->x, a.x.v, 1, a.m, a.k, a.x.ldv, TM) || !make_map(&m->w, a.w.v, 1, a.n, a.k, a.w.ldv, cols / 2))
+    return false;
+  m->y = m->r = m->x;  // (not used where rows do not go by TMA)
+  if (p->tma_y && !make_map(&m->y, y, es, a.m, a.n, ldy, 32)) return false;
+  return !p->tma_y || !a.res || make_map(&m->r, a.res, es, a.m, a.n, a.ldr, 32);
+}
+
+template <int OUT>
 static cudaError_t launch_pair(const Fp8Linear& a, int* err, cudaStream_t st) {
-  using S = PairShape<OUT, RES>;
-  constexpr int es = OUT == FP8_F32 ? 4 : (OUT == FP8_BF16 ? 2 : 1);
+  using S = PairShape<OUT>;
   TcFp8Args p;
-  p.a = a;
+  PairMaps m;
   p.err = err;
-  p.kb = (int)((a.k + 127) / 128);
-  p.m_tiles = (int)((a.m + 2 * TM - 1) / (2 * TM));
-  p.n_tiles = (int)((a.n + TN - 1) / TN);
-  CUtensorMap xm, wm, ym, rm;
-  if (!make_map(&xm, a.x.v, 1, a.m, a.k, a.x.ldv, TM) || !make_map(&wm, a.w.v, 1, a.n, a.k, a.w.ldv, TN / 2))
-    return cudaErrorInvalidValue;
-  const void* y = OUT == FP8_E4M3 ? a.q.v : a.y;
-  const long ldy = OUT == FP8_E4M3 ? a.q.ldv : a.ldy;
-  p.tma_y = ((uintptr_t)y | (size_t)ldy * es) % 16 == 0 && (!RES || ((uintptr_t)a.res | (size_t)a.ldr * es) % 16 == 0);
-  p.tma_edge = (size_t)a.n * es % 16 == 0;
-  if (p.tma_y) {
-    if (!make_map(&ym, y, es, a.m, a.n, ldy, 32)) return cudaErrorInvalidValue;
-    if (RES && !make_map(&rm, a.res, es, a.m, a.n, a.ldr, 32)) return cudaErrorInvalidValue;
-  }
-  const auto kernel = fp8_linear_pair_kernel<OUT, RES>;
+  if (!make_pair_maps(a, TN, &p, &m)) return cudaErrorInvalidValue;
+  const auto kernel = fp8_linear_pair_kernel<OUT>;
   static std::atomic<uint64_t> allowed{0};
   const cudaError_t e = allow_smem(kernel, S::SMEM, &allowed);
   if (e != cudaSuccess) return e;
   const long tiles = (long)p.m_tiles * p.n_tiles;
   const int pairs = num_sms() / 2;
   if (pairs <= 0) return cudaErrorInvalidDevice;
-  kernel<<<2 * (unsigned)(tiles < pairs ? tiles : pairs), PAIR_THREADS, S::SMEM, st>>>(xm, wm, p.tma_y ? ym : xm,
-                                                                                       p.tma_y && RES ? rm : xm, p);
+  kernel<<<2 * (unsigned)(tiles < pairs ? tiles : pairs), PAIR_THREADS, S::SMEM, st>>>(m.x, m.w, m.y, p);
+  return cudaGetLastError();
+}
+
+template <int OUT, bool RES, bool STAT>
+static cudaError_t launch_tile(const Fp8Linear& a, int* err, cudaStream_t st) {
+  using S = TileShape<OUT, RES, STAT>;
+  TcFp8Args p;
+  PairMaps m;
+  p.err = err;
+  if (!make_pair_maps(a, S::N, &p, &m)) return cudaErrorInvalidValue;
+  const auto kernel = fp8_linear_tile_kernel<OUT, RES, STAT>;
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_smem(kernel, 227 * 1024, &allowed);
+  if (e != cudaSuccess) return e;
+  const int pairs = num_sms() / 2;
+  if (pairs <= 0) return cudaErrorInvalidDevice;
+  p.stages = S::stages(p.kb);
+  const int smem = 1024 + S::OFF_A + p.stages * S::BPS * S::A_BYTES + (STAT ? p.kb : p.stages) * S::B_BYTES;
+  long used;
+  if (STAT) {  // whole columns of tiles, no more pairs to a column than it has rows
+    const long per = pairs / p.n_tiles;
+    if (per == 0 || p.kb > S::KB_MAX) return cudaErrorInvalidValue;
+    used = (per < p.m_tiles ? per : p.m_tiles) * p.n_tiles;
+  } else {
+    const long tiles = (long)p.m_tiles * p.n_tiles;
+    used = tiles < pairs ? tiles : pairs;
+  }
+  kernel<<<2 * (unsigned)used, S::THREADS, smem, st>>>(m.x, m.w, m.y, m.r, p);
   return cudaGetLastError();
 }
 
@@ -1056,8 +1535,12 @@ static cudaError_t launch_out(const Fp8Linear& a, int* err, cudaStream_t st) {
       if (narrow) return launch_split<64, OUT>(a, splits, err, st);
     return launch_split<128, OUT>(a, splits, err, st);
   }
-  if constexpr (OUT == FP8_E4M3) return launch_pair<OUT, false>(a, err, st);
-  return a.res ? launch_pair<OUT, OUT != FP8_E4M3>(a, err, st) : launch_pair<OUT, false>(a, err, st);
+  using T = TileShape<OUT, false, true>;
+  const bool stat = (a.k + 127) / 128 <= T::KB_MAX && (a.n + T::N - 1) / T::N <= sms / 2;
+  if constexpr (OUT != FP8_E4M3) {
+    if (a.res) return stat ? launch_tile<OUT, true, true>(a, err, st) : launch_tile<OUT, true, false>(a, err, st);
+  }
+  return stat ? launch_tile<OUT, false, true>(a, err, st) : launch_pair<OUT>(a, err, st);
 }
 
 cudaError_t launch_fp8_linear(const Fp8Linear& a, int* err, cudaStream_t st) {

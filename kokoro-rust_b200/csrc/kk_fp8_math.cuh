@@ -7,6 +7,29 @@
 
 namespace kk {
 
+// ---- two 32-bit operations in one instruction (each rounds as the single one does)
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ void unpack2(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ void add2(float& a, float& b, float c, float d) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(a, b)), "l"(pack2(c, d)));
+  unpack2(r, a, b);
+}
+
 // E of a block whose largest finite magnitude has these bits: 448 = 1.75 * 2^8, so with
 // a = m * 2^p, 1 <= m < 2, E - 127 is p - 8, and one more where m > 1.75. At most 247.
 __device__ __forceinline__ int fp8_exp(uint32_t amax_bits) {
@@ -26,8 +49,11 @@ __device__ __forceinline__ uint32_t finite_bits(float v) {
 }
 // four finite or NaN values, scaled, to e4m3
 __device__ __forceinline__ uint32_t e4m3x4_finite(float a, float b, float c, float d, float inv) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * inv, d * inv), __NV_SATFINITE, __NV_E4M3);
+  float2 p, q;
+  unpack2(mul2(pack2(a, b), pack2(inv, inv)), p.x, p.y);
+  unpack2(mul2(pack2(c, d), pack2(inv, inv)), q.x, q.y);
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(p, __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(q, __NV_SATFINITE, __NV_E4M3);
   return lo | (hi << 16);
 }
 // the same with infinities (which the conversion would saturate) as NaN
@@ -63,13 +89,18 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
 // hardware exponential and reciprocal: about 2^-21 relative near 0 and above. (The bf16 layers use the
 // hardware tanh, 2^-11; here the result may be kept in 32 bits, or be rounded to e4m3, where an error of
 // 2^-11 moves one value in a hundred to the neighbouring code.)
-__device__ __forceinline__ float gelu_fast(float x) {
+__device__ __forceinline__ void gelu_fast2(float& a, float& b) {
   constexpr float c = -2.0f * 0.797884560802865355f * 1.44269504088896341f;  // -2 sqrt(2 / pi) log2(e)
-  const float z = c * fmaf(0.044715f * x * x, x, x);
-  float t, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(z));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + t));
-  return x * r;
+  const uint64_t x = pack2(a, b);
+  const uint64_t z = mul2(x, fma2(mul2(x, x), pack2(0.044715f * c, 0.044715f * c), pack2(c, c)));
+  float t0, t1, r0, r1;
+  unpack2(z, t0, t1);
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(t0));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(t1));
+  add2(t0, t1, 1.0f, 1.0f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(t0));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(t1));
+  unpack2(mul2(x, pack2(r0, r1)), a, b);
 }
 
 }  // namespace kk

@@ -142,7 +142,7 @@ def check_linear(got, y, S, rms, K, act, dtype):
 SIZES = [(1, 1, 1), (1, 16, 128), (1, 768, 768), (2, 130, 100), (7, 128, 129), (16, 2304, 768), (17, 50, 512), (33, 257, 300),
          (64, 512, 768), (65, 96, 640), (66, 2048, 768), (128, 768, 2048), (129, 255, 16), (200, 1090, 514), (300, 769, 1100),
          (512, 768, 2048), (700, 640, 520), (4800, 1000, 384), (9501, 513, 640), (2600, 2304, 768),
-         (3, 20000, 4700), (140, 1000, 2500)]
+         (3, 20000, 4700), (140, 1000, 2500), (4800, 1000, 1700), (5003, 1157, 2100), (4900, 1024, 1030)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, E4M3])
@@ -188,7 +188,7 @@ def test_linear_far_apart_scales(kk):
         assert (np.abs(got - y) <= (256 + 4) * 2.0 ** -23 * S).all()
 
 
-@pytest.mark.parametrize("m, n, k", [(1, 130, 200), (20, 300, 514), (150, 300, 514)])
+@pytest.mark.parametrize("m, n, k", [(1, 130, 200), (20, 300, 514), (150, 300, 514), (4900, 1010, 200), (4900, 1010, 1700)])
 @pytest.mark.parametrize("ldy_pad, off", [(1, 0), (2, 1), (4, 4), (8, 0), (0, 3), (6, 0), (4, 0)])
 def test_linear_any_strides_and_offsets(kk, m, n, k, ldy_pad, off):
     """Result and residual rows at strides and offsets of every alignment; nothing is written beside them."""
