@@ -164,9 +164,7 @@ constexpr int SF_RING = 4;  // scale groups (4 blocks of K each) of a pair, in s
 // time, into a ring of shared-memory slots in the layout of the TMEM copy. A word waits behind the TMA's boxes on its
 // way from L2 (about 2000 cycles, as long as the MMAs of two or three groups), so the words of the next AHEAD groups
 // are always on their way, in registers; waiting for each group in turn held the MMAs up by half.
-// TILES: the slots of a tile (at most RING / 2 groups) are handed on together, and are free again when the tile before
-// the last is done: two barriers take the place of the ring's (full: [2]; empty: the tiles' accumulators, [2]).
-template <int RING, int ROWS_W, bool TILES = false>
+template <int RING, int ROWS_W>
 struct ScaleFeed {
   static constexpr int NB = (ROWS_W + 127) / 128, BYTES = 512 * (1 + NB), AHEAD = 4;
   const Fp8Linear& a;
@@ -206,37 +204,22 @@ struct ScaleFeed {
     open();
 #pragma unroll
     for (int i = 0; i < AHEAD; i++) load(w[i]);
-    const int groups = (b_hi - b_lo + 3) / 4;  // of a tile
-    long left = first < tiles ? (long)((tiles - first + step - 1) / step) * groups : 0;
+    long left = first < tiles ? (long)((tiles - first + step - 1) / step) * ((b_hi - b_lo + 3) / 4) : 0;
     uint32_t slot = 0, ph = 1;
     bool used = false;  // the ring has gone round once
-    int in_tile = 0, tile_n = 0;
     while (true) {
 #pragma unroll
       for (int i = 0; i < AHEAD; i++) {
         if (left-- == 0) return;
-        if (TILES) {
-          if (in_tile == 0 && tile_n > 1 && !warp_wait(empty + (tile_n & 1), ((tile_n >> 1) + 1) & 1, abort_flag, err)) return;
-        } else if (used && !warp_wait(empty + slot, ph, abort_flag, err)) {
-          return;
-        }
-        const uint32_t dst = ring + (TILES ? (tile_n & 1) * (RING / 2) + in_tile : slot) * BYTES + lane * 16;
+        if (used && !warp_wait(empty + slot, ph, abort_flag, err)) return;
+        const uint32_t dst = ring + slot * BYTES + lane * 16;
 #pragma unroll
         for (int j = 0; j < 1 + NB; j++)
           sts_u4(dst + 512 * j, make_uint4(w[i][4 * j], w[i][4 * j + 1], w[i][4 * j + 2], w[i][4 * j + 3]));
-        if (TILES) {
-          if (++in_tile == groups) {
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full + (tile_n & 1));
-            in_tile = 0, tile_n++;
-          }
-        } else {
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full + slot);
-          if (++slot == RING) slot = 0, ph ^= 1, used = true;
-        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + slot);
+        if (++slot == RING) slot = 0, ph ^= 1, used = true;
         load(w[i]);
       }
     }
@@ -294,7 +277,6 @@ struct TcFp8Args {
   int kb;              // blocks of 128 columns of K
   int m_tiles, n_tiles;
   int tma_y;           // y (and the residual) can be stored (loaded) by TMA: 16-byte aligned rows
-  int stages;          // (tile kernel)
   int tma_edge;        // so can their last columns: TMA writes whole 16-byte units, so n has to end on one
 };
 
@@ -304,20 +286,27 @@ struct TcFp8Args {
 // L2 per SM and clock at the full MMA rate, more than L2 gives; a pair shares the 256 rows of W (each CTA loads
 // and holds half of them), which takes 64.
 constexpr int TM = 128, TN = 256;  // a CTA's rows, the pair's columns
-constexpr int EPI_WARPS = 8;       // two per TMEM lane quarter, 128 columns each
-constexpr int PAIR_THREADS = 32 * (4 + EPI_WARPS);
+constexpr int CTRL_WARPS = 3;      // loads, MMAs, scales
 constexpr int BOX = 4096;          // 32 rows of 128 bytes: what an epilogue warp stores (or loads) at once
 
 template <int OUT>
 struct PairShape {
+  static constexpr bool Q = OUT == FP8_E4M3;
+  // Epilogue warps: two for each TMEM lane quarter, 128 columns each (with four, f32 and bf16 results are 15% slower:
+  // the warps of the main loop get fewer of the issue slots); four with 64 columns each for an e4m3 result, whose
+  // thread holds all of its columns until their maximum is known (with 128, too few registers are left to work on
+  // several at once: 10% slower with GELU)
+  static constexpr int EPI = Q ? 16 : 8, COLS = Q ? 64 : 128;
+  static constexpr int THREADS = 32 * (CTRL_WARPS + EPI);
   static constexpr int STAGES = 5;
   static constexpr int A_BYTES = TM * 128, B_BYTES = TN / 2 * 128;
   static constexpr int SF_BYTES = 512 * 3;
   // TMEM columns: the two accumulators share columns 192..255 (see the epilogue); scales behind them
   static constexpr int D1 = 192, SF_COL = D1 + TN, SF_COLS = 12;
+  static constexpr int BOXES = 8;  // e4m3: two warps share one
   static constexpr int OFF_B = STAGES * A_BYTES, OFF_BOX = OFF_B + STAGES * B_BYTES;
-  static constexpr int OFF_SF = OFF_BOX + EPI_WARPS * BOX, OFF_BIAS = OFF_SF + SF_RING * SF_BYTES;
-  static constexpr int OFF_BAR = OFF_BIAS + EPI_WARPS * 128 * 4;
+  static constexpr int OFF_SF = OFF_BOX + BOXES * BOX, OFF_BIAS = OFF_SF + SF_RING * SF_BYTES;
+  static constexpr int OFF_MAX = OFF_BIAS + EPI * COLS * 4, OFF_BAR = OFF_MAX + (Q ? 2 * EPI * 32 * 4 : 0);
   static constexpr int SMEM = OFF_BAR + 512 + 1024;  // 1024: alignment of the first stage
   static_assert(SF_COL + SF_RING * SF_COLS <= 512, "TMEM columns");
   static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -357,36 +346,36 @@ __device__ __forceinline__ void store_any(const Fp8Linear& a, float* v, long r0,
   }
 }
 
-// A block of 128 columns of a thread's row: its scale's E, and the values as e4m3, four to a word.
-__device__ __forceinline__ int quantize_block(const float* v, uint32_t* u) {
+// The largest finite magnitude of a thread's 64 columns, as bits; *infinite: one of them is infinite.
+__device__ __forceinline__ uint32_t finite_max64(const float* v, bool* infinite) {
   float m = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 128; i++) m = fmaxf(m, fabsf(v[i]));  // (a NaN is passed over)
-  uint32_t mb = __float_as_uint(m);
-  if (mb < 0x7F800000u) {
-    const int e = fp8_exp(mb);
-    const float inv = fp8_inv_scale(e);
+  for (int i = 0; i < 64; i++) m = fmaxf(m, fabsf(v[i]));  // (a NaN is passed over)
+  uint32_t b = __float_as_uint(m);
+  *infinite = b == 0x7F800000u;
+  if (*infinite) {
+    b = 0;
 #pragma unroll
-    for (int i = 0; i < 32; i++) u[i] = e4m3x4_finite(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv);
-    return e;
+    for (int i = 0; i < 64; i++) b = max(b, finite_bits(v[i]));
   }
-  mb = 0;
+  return b;
+}
+__device__ __forceinline__ void quantize64(const float* v, float inv, bool infinite, uint32_t* u) {
+  if (!infinite) {
 #pragma unroll
-  for (int i = 0; i < 128; i++) mb = max(mb, finite_bits(v[i]));
-  const int e = fp8_exp(mb);
-  const float inv = fp8_inv_scale(e);
+    for (int i = 0; i < 16; i++) u[i] = e4m3x4_finite(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv);
+  } else {
 #pragma unroll
-  for (int i = 0; i < 32; i++) u[i] = e4m3x4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv);
-  return e;
+    for (int i = 0; i < 16; i++) u[i] = e4m3x4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv);
+  }
 }
 
-__device__ __forceinline__ float4 load_bias(const Fp8Linear& a, long c) {
-  float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+// bias of columns c and c + 1, zero past the last
+__device__ __forceinline__ float2 load_bias2(const Fp8Linear& a, long c) {
+  float2 b = make_float2(0.0f, 0.0f);
   if (!a.bias) return b;
   if (c < a.n) b.x = a.bias[c];
   if (c + 1 < a.n) b.y = a.bias[c + 1];
-  if (c + 2 < a.n) b.z = a.bias[c + 2];
-  if (c + 3 < a.n) b.w = a.bias[c + 3];
   return b;
 }
 
@@ -411,10 +400,11 @@ __device__ __forceinline__ void tile_at(const TcFp8Args& p, int t, int* mt, int*
 
 // Persistent pairs. In each CTA warp 0 loads its boxes of x and W (128 bytes x 128 rows, 128-byte swizzle) into a
 // ring of stages, warp 2 brings the scales, four blocks of K at a time, into shared memory in the layout of the
-// TMEM copy, warps 4..11 are the epilogue (a thread holds 128 columns of one row); warp 1 of the first CTA issues
+// TMEM copy, the last 16 are the epilogue (a thread holds 64 columns of one row; with 128 columns, which a block of an
+// e4m3 result would suggest, too few registers are left to work on several at once); warp 1 of the first CTA issues
 // the pair's MMAs. Barriers that the MMA warp waits on live in the first CTA; those it commits to, in both.
 template <int OUT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<OUT>::THREADS, 1)
     fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
                            const __grid_constant__ CUtensorMap ymap, const __grid_constant__ TcFp8Args p) {
   using S = PairShape<OUT>;
@@ -423,7 +413,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
   uint64_t* full = (uint64_t*)(smem + S::OFF_BAR);
   uint64_t *empty = full + S::STAGES, *sf_full = empty + S::STAGES, *sf_empty = sf_full + SF_RING;
   uint64_t *acc_full = sf_empty + SF_RING, *acc_free = acc_full + 1;
-  uint32_t* tmem_slot = (uint32_t*)(acc_free + 1);
+  uint64_t *max_in = acc_free + 1, *box_in = max_in + S::BOXES;  // e4m3: of the two warps of a box
+  uint32_t* tmem_slot = (uint32_t*)(box_in + S::BOXES);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cta_rank();
@@ -433,7 +424,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     for (int i = 0; i < S::STAGES; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     for (int i = 0; i < SF_RING; i++) mbar_init(sf_full + i, rank == 0 ? 2 : 1), mbar_init(sf_empty + i, 1);
     mbar_init(acc_full, 1);
-    mbar_init(acc_free, 2 * EPI_WARPS);
+    mbar_init(acc_free, 2 * S::EPI);
+    if (S::Q)
+      for (int i = 0; i < S::BOXES; i++) mbar_init(max_in + i, 2), mbar_init(box_in + i, 2);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -539,93 +532,104 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
       tile_at(p, t, &mt, &nt);
       *m0 = (long)mt * 2 * TM + rank * TM, *n0 = (long)nt * TN;
     });
-  } else if (warp >= 4) {
-    const int ew = warp - 4, half = ew >> 2;
-    float* bias_s = (float*)(smem + S::OFF_BIAS) + ew * 128;
-    uint8_t* box = smem + S::OFF_BOX + ew * BOX;
+  } else {
+    const int ew = warp - CTRL_WARPS, cg = ew >> 2, q4 = warp & 3;  // COLS columns; the TMEM lane quarter a warp reaches
+    float* bias_s = (float*)(smem + S::OFF_BIAS) + ew * S::COLS;
+    // e4m3: the warps of columns 0..63 and 64..127 of a block share a box (and a barrier for each of their meetings)
+    const int bx = S::Q ? (cg >> 1) * 4 + q4 : ew, odd = cg & 1;
+    uint8_t* box = smem + S::OFF_BOX + bx * BOX;
     const uint32_t row_s = smem_u32(box) + lane * 128;  // this thread's row of the box; 16-byte units swizzled by row
     const uint32_t acc_free0 = map_rank(acc_free, 0);
-    constexpr int BC = OUT == FP8_F32 ? 32 : (OUT == FP8_BF16 ? 64 : 128);  // columns of a box
-    constexpr int NCH = 128 / BC;
     uint32_t tile_n = 0;
     bool ok = true;
-    float4 bias_r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (first < tiles) {
+    float2 bias_r[S::COLS / 64];  // two columns, and two 64 further on
+    auto load_bias_r = [&](int t) {
       int mt, nt;
-      tile_at(p, first, &mt, &nt);
-      bias_r = load_bias(a, (long)nt * TN + half * 128 + 4 * lane);
-    }
+      tile_at(p, t, &mt, &nt);
+#pragma unroll
+      for (int i = 0; i < S::COLS / 64; i++) bias_r[i] = load_bias2(a, (long)nt * TN + cg * S::COLS + 64 * i + 2 * lane);
+    };
+    if (first < tiles) load_bias_r(first);
     for (int t = first; ok && t < tiles; t += step, tile_n++) {
       int mt, nt;
       tile_at(p, t, &mt, &nt);
-      const long r0 = (long)mt * 2 * TM + rank * TM + (ew & 3) * 32;
-      const long c0 = (long)nt * TN + half * 128;
+      const long r0 = (long)mt * 2 * TM + rank * TM + q4 * 32;
+      const long c0 = (long)nt * TN + cg * S::COLS;
       // The next tile's accumulator may be written once the columns that it shares with this one are read: the last
-      // 64 of the first accumulator are the first 64 of the second; the half that holds them reads them first. (The
-      // tile after next reuses all of this accumulator: it waits for the next tile's arrivals, which come after all
-      // of this tile's reads.)
-      const bool shares = half == (int)(1 - (tile_n & 1));
-      const int ch0 = !shares || half == 0 ? 0 : (BC == 32 ? 2 : NCH - 1);
-      // boxes with columns, and how many of them go by TMA
-      const int live = r0 < a.m && c0 < a.n ? (int)min((long)NCH, (a.n - c0 + BC - 1) / BC) : 0;
-      const int boxes = !p.tma_y || live == 0 ? 0 : (p.tma_edge ? live : (int)min((long)live, (a.n - c0) / BC));
-      // (boxes are used in the order ch0, ch0 + 1, .. round to ch0 - 1)
+      // 64 of the first accumulator are the first 64 of the second. (The tile after next reuses all of this
+      // accumulator: it waits for the next tile's arrivals, which come after all of this tile's reads.)
+      const bool shares = cg == (tile_n & 1 ? 0 : S::EPI / 4 - 1);
+      const bool live = r0 < a.m && c0 < a.n;
+      if (S::Q && !odd && lane == 0) bulk_wait_all_read();  // the box is free once the last tile's store has read it
       __syncwarp();
-      *reinterpret_cast<float4*>(bias_s + 4 * lane) = bias_r;
+#pragma unroll
+      for (int i = 0; i < S::COLS / 64; i++) *reinterpret_cast<float2*>(bias_s + 64 * i + 2 * lane) = bias_r[i];
       __syncwarp();
-      if (t + step < tiles) {  // the next tile's, which arrives during this one
-        int mt1, nt1;
-        tile_at(p, t + step, &mt1, &nt1);
-        bias_r = load_bias(a, (long)nt1 * TN + half * 128 + 4 * lane);
-      }
+      if (t + step < tiles) load_bias_r(t + step);  // the next tile's, which arrives during this one
       ok = warp_wait(acc_full, tile_n & 1, abort_flag, err);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t d = tmem + ((uint32_t)(ew & 3) << 21) + (tile_n & 1) * S::D1 + half * 128;
+      const uint32_t d = tmem + ((uint32_t)q4 << 21) + (tile_n & 1) * S::D1 + cg * S::COLS;
       if (!shares && lane == 0) mbar_arrive_cluster_relaxed(acc_free0);
-      if constexpr (OUT == FP8_E4M3) {
-        float v[128];
+      if constexpr (S::Q) {
+        float v[64];
         tmem_ld64(d, v);
-        tmem_ld64(d + 64, v + 64);
         if (shares) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster_relaxed(acc_free0);
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++) add_bias32(v + 32 * i, bias_s + 32 * i);
+        add_bias32(v, bias_s);
+        add_bias32(v + 32, bias_s + 32);
         if (a.gelu) {
 #pragma unroll
-          for (int i = 0; i < 128; i += 2) gelu_fast2(v[i], v[i + 1]);
+          for (int i = 0; i < 64; i += 16) gelu_fast<16>(v + i);
         }
-        if (live) {
-          uint32_t u[32];
-          const int e = quantize_block(v, u);
-          if (r0 + lane < a.m) a.q.e[(r0 + lane) * a.q.lde + (c0 >> 7)] = (uint8_t)e;
-          if (boxes) {
-            if (lane == 0) bulk_wait_all_read();
-            __syncwarp();
+        // the block's maximum: this half's and the other's
+        uint32_t* max_s = (uint32_t*)(smem + S::OFF_MAX) + (tile_n & 1) * S::EPI * 32;
+        bool infinite;
+        uint32_t m = finite_max64(v, &infinite);
+        max_s[ew * 32 + lane] = m;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(max_in + bx);
+        ok = warp_wait(max_in + bx, tile_n & 1, abort_flag, err);
+        if (!ok) break;
+        m = max(m, max_s[(ew ^ 4) * 32 + lane]);
+        const int e = fp8_exp(m);
+        uint32_t u[16];
+        quantize64(v, fp8_inv_scale(e), infinite, u);
+        const long cb = c0 - odd * 64;  // the block's first column
+        const bool block = r0 < a.m && cb < a.n, tma = block && p.tma_y && (p.tma_edge || cb + 128 <= a.n);
+        if (block && !odd && r0 + lane < a.m) a.q.e[(r0 + lane) * a.q.lde + (cb >> 7)] = (uint8_t)e;
+        if (tma) {
 #pragma unroll
-            for (int q = 0; q < 8; q++)
-              sts_u4(row_s + ((q ^ (lane & 7)) << 4), make_uint4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]));
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&ymap, (int)c0, (int)r0, box);
-              bulk_commit();
-            }
-          } else if (r0 + lane < a.m) {  // the last columns
-            uint8_t* row = a.q.v + (r0 + lane) * a.q.ldv + c0;
+          for (int q = 0; q < 4; q++)
+            sts_u4(row_s + (((4 * odd + q) ^ (lane & 7)) << 4), make_uint4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]));
+          fence_proxy_async();
+        } else if (live && r0 + lane < a.m) {  // the last columns
+          uint8_t* row = a.q.v + (r0 + lane) * a.q.ldv + c0;
 #pragma unroll
-            for (int i = 0; i < 128; i++)
-              if (c0 + i < a.n) row[i] = (uint8_t)(u[i >> 2] >> (8 * (i & 3)));
+          for (int i = 0; i < 64; i++)
+            if (c0 + i < a.n) row[i] = (uint8_t)(u[i >> 2] >> (8 * (i & 3)));
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(box_in + bx);
+        if (!odd) {
+          ok = warp_wait(box_in + bx, tile_n & 1, abort_flag, err);
+          if (!ok) break;
+          if (tma && lane == 0) {
+            tma_store_2d(&ymap, (int)cb, (int)r0, box);
+            bulk_commit();
           }
         }
       } else {
+        constexpr int BC = OUT == FP8_F32 ? 32 : 64, NCH = S::COLS / BC;  // columns of a box, boxes of a warp
+        const int ch0 = shares && cg != 0 ? NCH - 64 / BC : 0;  // the boxes of the shared columns come first
 #pragma unroll 1
         for (int i = 0; i < NCH; i++) {
           const int ch = (i + ch0) % NCH;
-          const bool on = ch < live, tma = ch < boxes;
+          const long cx = c0 + ch * BC;  // the box's first column
+          const bool on = live && cx < a.n, tma = on && p.tma_y && (p.tma_edge || cx + BC <= a.n);
           if (tma) {
             if (lane == 0) bulk_wait_all_read();
             __syncwarp();
@@ -644,7 +648,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             add_bias32(v, bias_s + c);
             if (a.gelu) {
 #pragma unroll
-              for (int j = 0; j < 32; j += 2) gelu_fast2(v[j], v[j + 1]);
+              for (int j = 0; j < 32; j += 16) gelu_fast<16>(v + j);
             }
             if (!tma) {
               if (c0 + c < a.n) {
@@ -657,24 +661,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             }
             if constexpr (OUT == FP8_F32) {
 #pragma unroll
-              for (int q = 0; q < 8; q++) {
+              for (int q = 0; q < 8; q++)
                 sts_u4(row_s + ((q ^ (lane & 7)) << 4),
                        make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]),
                                   __float_as_uint(v[4 * q + 3])));
-              }
             } else {
 #pragma unroll
-              for (int q = 0; q < 4; q++) {
-                sts_u4(row_s + (((4 * h + q) ^ (lane & 7)) << 4), make_uint4(bf16x2(v[8 * q], v[8 * q + 1]), bf16x2(v[8 * q + 2], v[8 * q + 3]),
-                                      bf16x2(v[8 * q + 4], v[8 * q + 5]), bf16x2(v[8 * q + 6], v[8 * q + 7])));
-              }
+              for (int q = 0; q < 4; q++)
+                sts_u4(row_s + (((4 * h + q) ^ (lane & 7)) << 4),
+                       make_uint4(bf16x2(v[8 * q], v[8 * q + 1]), bf16x2(v[8 * q + 2], v[8 * q + 3]),
+                                  bf16x2(v[8 * q + 4], v[8 * q + 5]), bf16x2(v[8 * q + 6], v[8 * q + 7])));
             }
           }
           if (!tma) continue;
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&ymap, (int)c0 + ch * BC, (int)r0, box);
+            tma_store_2d(&ymap, (int)cx, (int)r0, box);
             bulk_commit();
           }
         }
@@ -693,66 +696,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
   }
 }
 
-// ---- large layers with few blocks of K, or with a residual: two whole accumulators
+// ---- large layers with a residual: two whole accumulators and a box for every column
 //
-// With K = 768 a tile's MMAs take 1.6 us, and the kernel above stands still for another between two tiles, while
-// their shared columns are handed over; with a residual its two boxes a warp are too few to load it ahead. Here the
-// pair's tile is 192 columns (128 when the result is quantised: a block is 128), so that both accumulators fit TMEM
-// side by side, and a warp has a box for each of its columns of a tile. Where the pair's columns of W fit shared
-// memory (STAT) they are loaded once and the pair takes one column of tiles; then only x is read again for each.
-// f32 / bf16: 12 epilogue warps, three for each lane quarter, 64 columns each. e4m3: 8, in two groups that take
-// turns (a thread holds a row's 128 columns), each with an accumulator of its own.
-template <int OUT, bool RES, bool STAT>
+// Bound by HBM (a residual read and a result written for each element). Above, a warp's single box would hold one
+// residual at a time and wait for each. Here the pair's tile is 192 columns, so that both accumulators fit TMEM side by
+// side and boxes for a whole tile fit shared memory: a tile's residual is loaded while its MMAs run. 12 epilogue warps,
+// three for each lane quarter, 64 columns each.
+template <int OUT>
 struct TileShape {
-  static constexpr int N = OUT == FP8_E4M3 ? 128 : 192;
-  static constexpr int EPI = OUT == FP8_E4M3 ? 8 : 12;
-  static constexpr int THREADS = 32 * (4 + EPI);
-  static constexpr int COLS = OUT == FP8_E4M3 ? 128 : 64;                          // of an epilogue thread
-  static constexpr int BC = OUT == FP8_F32 ? 32 : (OUT == FP8_BF16 ? 64 : 128);    // columns of a box
-  static constexpr int NBOX = COLS / BC;
-  static constexpr int KB_MAX = OUT == FP8_F32 ? 6 : 8;          // blocks of K that STAT holds
-  static constexpr int BPS = STAT && OUT != FP8_F32 ? 2 : 1;     // blocks of a stage
-  static constexpr int MAX_STAGES = 10;
+  static constexpr int N = 192, EPI = 12;
+  static constexpr int THREADS = 32 * (CTRL_WARPS + EPI);
+  static constexpr int BC = OUT == FP8_F32 ? 32 : 64;  // columns of a box
+  static constexpr int NBOX = 64 / BC;
+  static constexpr int STAGES = OUT == FP8_F32 ? 4 : 5;
   static constexpr int A_BYTES = TM * 128, B_BYTES = N / 2 * 128;
   static constexpr int NB = (N + 127) / 128;
   static constexpr int SF_BYTES = 512 * (1 + NB), SF_COLS = 4 * (1 + NB), SF_COL = 2 * N;
-  static constexpr int OFF_SF = EPI * NBOX * BOX, OFF_BIAS = OFF_SF + SF_RING * SF_BYTES;
-  static constexpr int OFF_BAR = OFF_BIAS + EPI * COLS * 4;
-  static constexpr int OFF_BOX = 0, OFF_A = (OFF_BAR + 512 + 1023) / 1024 * 1024;  // then the operands, in what is left
-  static constexpr int ROOM = 227 * 1024 - 1024 - OFF_A;
-  static int stages(int kb) {
-    const int n = STAT ? (ROOM - kb * B_BYTES) / (BPS * A_BYTES) : ROOM / (A_BYTES + B_BYTES);
-    return n < MAX_STAGES ? n : MAX_STAGES;
-  }
+  static constexpr int OFF_B = STAGES * A_BYTES, OFF_BOX = OFF_B + STAGES * B_BYTES;
+  static constexpr int OFF_SF = OFF_BOX + EPI * NBOX * BOX, OFF_BIAS = OFF_SF + SF_RING * SF_BYTES;
+  static constexpr int OFF_BAR = OFF_BIAS + EPI * 64 * 4;
+  static constexpr int SMEM = OFF_BAR + 512 + 1024;
   static_assert(SF_COL + SF_RING * SF_COLS <= 512, "TMEM columns");
-  static_assert(ROOM >= (STAT ? KB_MAX * B_BYTES + 2 * BPS * A_BYTES : 4 * (A_BYTES + B_BYTES)), "shared memory");
-  static_assert(!STAT || KB_MAX <= 4 * (SF_RING / 2), "a tile's scale groups fit half the ring");
+  static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
-template <int OUT, bool RES, bool STAT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TileShape<OUT, RES, STAT>::THREADS, 1)
+template <int OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TileShape<OUT>::THREADS, 1)
     fp8_linear_tile_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
                            const __grid_constant__ CUtensorMap ymap, const __grid_constant__ CUtensorMap rmap,
                            const __grid_constant__ TcFp8Args p) {
-  using S = TileShape<OUT, RES, STAT>;
-  constexpr bool Q = OUT == FP8_E4M3;
+  using S = TileShape<OUT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint64_t* full = (uint64_t*)(smem + S::OFF_BAR);
-  uint64_t *empty = full + S::MAX_STAGES, *sf_full = empty + S::MAX_STAGES, *sf_empty = sf_full + SF_RING;
+  uint64_t *empty = full + S::STAGES, *sf_full = empty + S::STAGES, *sf_empty = sf_full + SF_RING;
   uint64_t *acc_full = sf_empty + SF_RING, *acc_free = acc_full + 2;
   uint64_t* res_full = acc_free + 2;  // [EPI][NBOX]
   uint32_t* tmem_slot = (uint32_t*)(res_full + S::EPI * S::NBOX);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t off_a = S::OFF_A, off_b = S::OFF_A + p.stages * S::BPS * S::A_BYTES;  // the operands: x, then W
   const uint32_t rank = cta_rank();
   const Fp8Linear& a = p.a;
   int* err = p.err ? p.err : &g_fp8_wait_error;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S::MAX_STAGES; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
+    for (int i = 0; i < S::STAGES; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     for (int i = 0; i < SF_RING; i++) mbar_init(sf_full + i, rank == 0 ? 2 : 1), mbar_init(sf_empty + i, 1);
-    for (int i = 0; i < 2; i++) mbar_init(acc_full + i, 1), mbar_init(acc_free + i, Q ? S::EPI : 2 * S::EPI);
+    for (int i = 0; i < 2; i++) mbar_init(acc_full + i, 1), mbar_init(acc_free + i, 2 * S::EPI);
     for (int i = 0; i < S::EPI * S::NBOX; i++) mbar_init(res_full + i, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -766,53 +755,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TileShape<OUT, RES, 
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int kb = p.kb, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  // STAT: a pair keeps column pair % n_tiles of the tiles and takes every (pairs / n_tiles)-th row of it, so that
-  // all columns of a row of tiles are worked on at about the same time and x comes from HBM once
-  const int first = STAT ? pair / p.n_tiles : pair, step = STAT ? pairs / p.n_tiles : pairs;
-  const int tiles = STAT ? p.m_tiles : p.m_tiles * p.n_tiles;
-  auto tile = [&](int t, int* mt, int* nt) {
-    if (STAT)
-      *mt = t, *nt = pair % p.n_tiles;
-    else
-      tile_at(p, t, mt, nt);
-  };
+  const int tiles = p.m_tiles * p.n_tiles, kb = p.kb;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
   if (warp == 0) {
     {
       const bool lead = elect_one();
       uint32_t it = 0, s = 0, ph = 1;
-      const uint32_t stages = p.stages;
       bool ok = true;
       for (int t = first; ok && t < tiles; t += step) {
         int mt, nt;
-        tile(t, &mt, &nt);
+        tile_at(p, t, &mt, &nt);
         const int m0 = mt * 2 * TM + (int)rank * TM, n0 = nt * S::N + (int)rank * (S::N / 2);
-        const bool load_w = !STAT || t == first;
-        for (int b = 0; b < kb; b += S::BPS, it++) {
-          if (it >= stages && !warp_wait(empty + s, ph, abort_flag, err)) {
+        for (int b = 0; b < kb; b++, it++) {
+          if (it >= S::STAGES && !warp_wait(empty + s, ph, abort_flag, err)) {
             ok = false;
             break;
           }
           if (lead) {
-            const int blocks = min(S::BPS, kb - b);
-            if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * blocks * (S::A_BYTES + (load_w ? S::B_BYTES : 0)));
+            if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * (S::A_BYTES + S::B_BYTES));
             const uint32_t bar = map_rank(full + s, 0);
-#pragma unroll
-            for (int i = 0; i < S::BPS; i++) {
-              if (i >= blocks) break;
-              tma_load_2d_pair(smem + off_a + (s * S::BPS + i) * S::A_BYTES, &xmap, (b + i) * 128, m0, bar);
-              if (load_w) tma_load_2d_pair(smem + off_b + (STAT ? b + i : s) * S::B_BYTES, &wmap, (b + i) * 128, n0, bar);
-            }
+            tma_load_2d_pair(smem + s * S::A_BYTES, &xmap, b * 128, m0, bar);
+            tma_load_2d_pair(smem + S::OFF_B + s * S::B_BYTES, &wmap, b * 128, n0, bar);
           }
-          if (++s == stages) s = 0, ph ^= 1;
+          if (++s == S::STAGES) s = 0, ph ^= 1;
         }
       }
       // After an expired wait, loads still in flight land before the shared memory goes: the first CTA sees them
       // complete, the second, whose loads complete there, waits far longer than a load takes.
       if (!ok) {
         if (rank == 0) {
-          for (uint32_t i = it > stages ? it - stages : 0; i < it; i++) mbar_drain(full + i % stages, (i / stages) & 1);
+          for (uint32_t i = it > S::STAGES ? it - S::STAGES : 0; i < it; i++)
+            mbar_drain(full + i % S::STAGES, (i / S::STAGES) & 1);
         } else {
           const unsigned long long t0 = tc_now();
           while (tc_now() - t0 < 1000000ull) __nanosleep(1000);
@@ -822,9 +796,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TileShape<OUT, RES, 
   } else if (warp == 1) {
     if (rank == 0) {
       const bool lead = elect_one();
-      const uint64_t da0 = sdesc_sw128(smem_u32(smem + off_a)), db0 = sdesc_sw128(smem_u32(smem + off_b));
+      const uint64_t da0 = sdesc_sw128(smem_u32(smem)), db0 = sdesc_sw128(smem_u32(smem + S::OFF_B));
       const uint64_t dsf0 = sdesc(smem_u32(smem + S::OFF_SF), 128, 128);
-      MmaFeed f{full, sf_full, p.stages, abort_flag, err};
+      MmaFeed f{full, sf_full, S::STAGES, abort_flag, err};
       uint32_t tile_n = 0;
       bool ok = true;
       for (int t = first; ok && t < tiles; t += step, tile_n++) {
@@ -832,242 +806,156 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TileShape<OUT, RES, 
         if (tile_n > 1 && !warp_wait_cluster(acc_free + buf, ((tile_n >> 1) + 1) & 1, abort_flag, err)) break;
         tc_fence_after();
         const uint32_t d = tmem + buf * S::N;
-        if constexpr (STAT) {
-          // all of the tile's scales, then its stages: few waits and commits a tile, because they, not the MMAs, are
-          // what takes this warp's time
-          ok = warp_wait_cluster(sf_full + buf, (tile_n >> 1) & 1, abort_flag, err);
+        for (int b0 = 0; ok && b0 < kb; b0 += 4) {
+          ok = f.scales();
           if (!ok) break;
-          const uint32_t sf0 = tmem + S::SF_COL + buf * (SF_RING / 2) * S::SF_COLS;
+          const uint32_t sfa = tmem + S::SF_COL + f.slot * S::SF_COLS;
           if (lead) {
-            for (int g = 0; 4 * g < kb; g++) {
-              const uint64_t dsf = dsf0 + (buf * (SF_RING / 2) + g) * (S::SF_BYTES >> 4);
+            const uint64_t dsf = dsf0 + f.slot * (S::SF_BYTES >> 4);
 #pragma unroll
-              for (int i = 0; i < 1 + S::NB; i++) tmem_cp_scales_pair(sf0 + g * S::SF_COLS + 4 * i, dsf + (512 >> 4) * i);
-            }
+            for (int i = 0; i < 1 + S::NB; i++) tmem_cp_scales_pair(sfa + 4 * i, dsf + (512 >> 4) * i);
           }
-#pragma unroll 4
-          for (int b = 0; b < kb; b += S::BPS) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            if (b0 + j >= kb) break;
             ok = f.stage();
             if (!ok) break;
             if (lead) {
+              const uint64_t da = da0 + f.s * (S::A_BYTES >> 4), db = db0 + f.s * (S::B_BYTES >> 4);
 #pragma unroll
-              for (int i = 0; i < S::BPS; i++) {
-                if (b + i >= kb) break;
-                const uint64_t da = da0 + (f.s * S::BPS + i) * (S::A_BYTES >> 4), db = db0 + (b + i) * (S::B_BYTES >> 4);
-                const uint32_t sfa = sf0 + ((b + i) >> 2) * S::SF_COLS, sel = (b + i) & 3;
-                const uint32_t id = idesc_mxf8(2 * TM, S::N, 0) | (sel << 4) | (sel << 29);
-#pragma unroll
-                for (int j = 0; j < 4; j++) mma_mxf8_pair(d, da + 2 * j, db + 2 * j, id, sfa, sfa + 4, j > 0 || b + i > 0);
-              }
+              for (int k = 0; k < 4; k++)
+                mma_mxf8_pair(d, da + 2 * k, db + 2 * k, idesc_mxf8(2 * TM, S::N, j), sfa, sfa + 4, j > 0 || k > 0 || b0 > 0);
               mma_commit_pair(empty + f.s);
             }
             f.next_stage();
           }
-        } else {
-          for (int b0 = 0; ok && b0 < kb; b0 += 4) {
-            ok = f.scales();
-            if (!ok) break;
-            const uint32_t sfa = tmem + S::SF_COL + f.slot * S::SF_COLS;
-            if (lead) {
-              const uint64_t dsf = dsf0 + f.slot * (S::SF_BYTES >> 4);
-  #pragma unroll
-              for (int i = 0; i < 1 + S::NB; i++) tmem_cp_scales_pair(sfa + 4 * i, dsf + (512 >> 4) * i);
-            }
-  #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              if (b0 + j >= kb) break;
-              ok = f.stage();
-              if (!ok) break;
-              if (lead) {
-                const uint64_t da = da0 + f.s * (S::A_BYTES >> 4), db = db0 + (STAT ? b0 + j : f.s) * (S::B_BYTES >> 4);
-  #pragma unroll
-                for (int k = 0; k < 4; k++)
-                  mma_mxf8_pair(d, da + 2 * k, db + 2 * k, idesc_mxf8(2 * TM, S::N, j), sfa, sfa + 4, j > 0 || k > 0 || b0 > 0);
-                mma_commit_pair(empty + f.s);
-              }
-              f.next_stage();
-            }
-            if (ok && lead) mma_commit_pair(sf_empty + f.slot);
-            f.next_scales();
-          }
+          if (ok && lead) mma_commit_pair(sf_empty + f.slot);
+          f.next_scales();
         }
         if (ok && lead) mma_commit_pair(acc_full + buf);
       }
       if (*abort_flag && f.any) mbar_drain(empty + f.last, f.last_ph);  // MMAs in flight end before their operands and TMEM go
     } else if (first < tiles) {
-      const long n = (tiles - first + step - 1) / step;
-      if (STAT)
-        forward_scales<2>(n, sf_full, lane, abort_flag, err);
-      else
-        forward_scales<SF_RING>(n * ((kb + 3) / 4), sf_full, lane, abort_flag, err);
+      forward_scales<SF_RING>((long)((tiles - first + step - 1) / step) * ((kb + 3) / 4), sf_full, lane, abort_flag, err);
     }
   } else if (warp == 2) {
-    ScaleFeed<SF_RING, S::N, STAT> feed{a, smem_u32(smem + S::OFF_SF), sf_full, STAT ? acc_full : sf_empty, abort_flag, err, lane};
+    ScaleFeed<SF_RING, S::N> feed{a, smem_u32(smem + S::OFF_SF), sf_full, sf_empty, abort_flag, err, lane};
     feed.run(first, step, tiles, 0, kb, [&](int t, long* m0, long* n0) {
       int mt, nt;
-      tile(t, &mt, &nt);
+      tile_at(p, t, &mt, &nt);
       *m0 = (long)mt * 2 * TM + rank * TM, *n0 = (long)nt * S::N;
     });
-  } else if (warp >= 4) {
-    const int ew = warp - 4, group = ew >> 2, q = ew & 3;
-    constexpr int PB = S::COLS / 32;  // bias values of a lane
-    float* bias_s = (float*)(smem + S::OFF_BIAS) + ew * S::COLS;
+  } else {
+    const int ew = warp - CTRL_WARPS, cg = ew >> 2, q4 = warp & 3;  // 64 columns; the TMEM lane quarter a warp reaches
+    float* bias_s = (float*)(smem + S::OFF_BIAS) + ew * 64;
     uint8_t* box = smem + S::OFF_BOX + ew * S::NBOX * BOX;
     const uint32_t row_s = smem_u32(box) + lane * 128;  // this thread's row of a box; 16-byte units swizzled by row
-    const int col = Q ? 0 : group * S::COLS;            // of the tile
     uint32_t tile_n = 0, nres = 0;
     bool ok = true;
-    float bias_r[PB];
-    auto load_bias_r = [&](int t) {
+    float2 bias_r = make_float2(0.0f, 0.0f);
+    if (first < tiles) {
       int mt, nt;
-      tile(t, &mt, &nt);
-      const long c = (long)nt * S::N + col + PB * lane;
-#pragma unroll
-      for (int i = 0; i < PB; i++) bias_r[i] = a.bias && c + i < a.n ? a.bias[c + i] : 0.0f;
-    };
-    // e4m3: this group takes every second tile of the pair's
-    const int t0 = Q ? first + group * step : first, tstep = Q ? 2 * step : step;
-    if (t0 < tiles) load_bias_r(t0);
-    tile_n = Q ? group : 0;
-    for (int t = t0; ok && t < tiles; t += tstep, tile_n += Q ? 2 : 1) {
+      tile_at(p, first, &mt, &nt);
+      bias_r = load_bias2(a, (long)nt * S::N + cg * 64 + 2 * lane);
+    }
+    for (int t = first; ok && t < tiles; t += step, tile_n++) {
       int mt, nt;
-      tile(t, &mt, &nt);
-      const long r0 = (long)mt * 2 * TM + rank * TM + q * 32;
-      const long c0 = (long)nt * S::N + col;
+      tile_at(p, t, &mt, &nt);
+      const long r0 = (long)mt * 2 * TM + rank * TM + q4 * 32;
+      const long c0 = (long)nt * S::N + cg * 64;
       const uint32_t buf = tile_n & 1;
       // boxes with columns, and how many of them go by TMA
       const int live = r0 < a.m && c0 < a.n ? (int)min((long)S::NBOX, (a.n - c0 + S::BC - 1) / S::BC) : 0;
       const int boxes = !p.tma_y || live == 0 ? 0 : (p.tma_edge ? live : (int)min((long)live, (a.n - c0) / S::BC));
       if (lane == 0) bulk_wait_all_read();  // the boxes are free once the last tile's stores have read them
-      if constexpr (RES) {                  // the residual comes while the tile's MMAs run
-        if (lane == 0) {
-          for (int i = 0; i < boxes; i++) {
-            mbar_arrive_expect_tx(res_full + ew * S::NBOX + i, BOX);
-            tma_load_2d(box + i * BOX, &rmap, (int)c0 + i * S::BC, (int)r0, res_full + ew * S::NBOX + i);
-          }
+      if (lane == 0) {                      // the residual comes while the tile's MMAs run
+        for (int i = 0; i < boxes; i++) {
+          mbar_arrive_expect_tx(res_full + ew * S::NBOX + i, BOX);
+          tma_load_2d(box + i * BOX, &rmap, (int)c0 + i * S::BC, (int)r0, res_full + ew * S::NBOX + i);
         }
       }
       __syncwarp();
-#pragma unroll
-      for (int i = 0; i < PB; i++) bias_s[PB * lane + i] = bias_r[i];
+      *reinterpret_cast<float2*>(bias_s + 2 * lane) = bias_r;
       __syncwarp();
-      if (!STAT && t + tstep < tiles) load_bias_r(t + tstep);  // the next tile's arrives during this one
+      if (t + step < tiles) {  // the next tile's, which arrives during this one
+        int mt1, nt1;
+        tile_at(p, t + step, &mt1, &nt1);
+        bias_r = load_bias2(a, (long)nt1 * S::N + cg * 64 + 2 * lane);
+      }
       ok = warp_wait(acc_full + buf, (tile_n >> 1) & 1, abort_flag, err);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t d = tmem + ((uint32_t)q << 21) + buf * S::N + col;
+      const uint32_t d = tmem + ((uint32_t)q4 << 21) + buf * S::N + cg * 64;
       const uint32_t free0 = map_rank(acc_free + buf, 0);
-      if constexpr (Q) {
-        float v[128];
-        tmem_ld64(d, v);
-        tmem_ld64(d + 64, v + 64);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_relaxed(free0);
 #pragma unroll
-        for (int i = 0; i < 4; i++) add_bias32(v + 32 * i, bias_s + 32 * i);
+      for (int h = 0; h < 2; h++) {  // 32 columns at a time
+        const int c = 32 * h, bx = c / S::BC;
+        const bool on = bx < live, tma = bx < boxes;
+        float v[32];
+        tmem_ld32(d + c, v);
+        if (h == 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(free0);
+        }
+        if (!on) continue;
+        add_bias32(v, bias_s + c);
         if (a.gelu) {
 #pragma unroll
-          for (int i = 0; i < 128; i += 2) gelu_fast2(v[i], v[i + 1]);
+          for (int j = 0; j < 32; j += 16) gelu_fast<16>(v + j);
         }
-        if (live) {
-          uint32_t u[32];
-          const int e = quantize_block(v, u);
-          if (r0 + lane < a.m) a.q.e[(r0 + lane) * a.q.lde + (c0 >> 7)] = (uint8_t)e;
-          if (boxes) {
+        if (!tma) {
+          if (c0 + c < a.n) {
+            if constexpr (OUT == FP8_F32)
+              store_any<float>(a, v, r0, c0 + c, lane);
+            else
+              store_any<__nv_bfloat16>(a, v, r0, c0 + c, lane);
+          }
+          continue;
+        }
+        if (c % S::BC == 0) {
+          ok = warp_wait(res_full + ew * S::NBOX + bx, (nres >> bx) & 1, abort_flag, err);
+          if (!ok) break;
+          nres ^= 1u << bx;
+        }
+        const uint32_t row_b = row_s + bx * BOX;
+        if constexpr (OUT == FP8_F32) {
 #pragma unroll
-            for (int k = 0; k < 8; k++)
-              sts_u4(row_s + ((k ^ (lane & 7)) << 4), make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]));
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&ymap, (int)c0, (int)r0, box);
-              bulk_commit();
+          for (int k = 0; k < 8; k++) {
+            const uint32_t at = row_b + ((k ^ (lane & 7)) << 4);
+            float4 o = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+            const float4 r = lds_f4(at);
+            o.x += r.x, o.y += r.y, o.z += r.z, o.w += r.w;
+            sts_u4(at, make_uint4(__float_as_uint(o.x), __float_as_uint(o.y), __float_as_uint(o.z), __float_as_uint(o.w)));
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const uint32_t at = row_b + (((4 * h + k) ^ (lane & 7)) << 4);
+            const float4 r = lds_f4(at);
+            const uint32_t u[4] = {__float_as_uint(r.x), __float_as_uint(r.y), __float_as_uint(r.z), __float_as_uint(r.w)};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              v[8 * k + 2 * i] += __uint_as_float(u[i] << 16);
+              v[8 * k + 2 * i + 1] += __uint_as_float(u[i] & 0xFFFF0000u);
             }
-          } else if (r0 + lane < a.m) {  // the last columns
-            uint8_t* row = a.q.v + (r0 + lane) * a.q.ldv + c0;
-#pragma unroll
-            for (int i = 0; i < 128; i++)
-              if (c0 + i < a.n) row[i] = (uint8_t)(u[i >> 2] >> (8 * (i & 3)));
+            sts_u4(at, make_uint4(bf16x2(v[8 * k], v[8 * k + 1]), bf16x2(v[8 * k + 2], v[8 * k + 3]),
+                                  bf16x2(v[8 * k + 4], v[8 * k + 5]), bf16x2(v[8 * k + 6], v[8 * k + 7])));
           }
         }
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {  // 32 columns at a time
-          const int c = 32 * h, bx = c / S::BC;
-          const bool on = bx < live, tma = bx < boxes;
-          float v[32];
-          tmem_ld32(d + c, v);
-          if (h == 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster_relaxed(free0);
-          }
-          if (!on) continue;
-          add_bias32(v, bias_s + c);
-          if (a.gelu) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) gelu_fast2(v[j], v[j + 1]);
-          }
-          if (!tma) {
-            if (c0 + c < a.n) {
-              if constexpr (OUT == FP8_F32)
-                store_any<float>(a, v, r0, c0 + c, lane);
-              else
-                store_any<__nv_bfloat16>(a, v, r0, c0 + c, lane);
-            }
-            continue;
-          }
-          if constexpr (RES) {
-            if (c % S::BC == 0) {
-              ok = warp_wait(res_full + ew * S::NBOX + bx, (nres >> bx) & 1, abort_flag, err);
-              if (!ok) break;
-              nres ^= 1u << bx;
-            }
-          }
-          const uint32_t row_b = row_s + bx * BOX;
-          if constexpr (OUT == FP8_F32) {
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-              const uint32_t at = row_b + ((k ^ (lane & 7)) << 4);
-              float4 o = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-              if constexpr (RES) {
-                const float4 r = lds_f4(at);
-                o.x += r.x, o.y += r.y, o.z += r.z, o.w += r.w;
-              }
-              sts_u4(at, make_uint4(__float_as_uint(o.x), __float_as_uint(o.y), __float_as_uint(o.z), __float_as_uint(o.w)));
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-              const uint32_t at = row_b + (((4 * h + k) ^ (lane & 7)) << 4);
-              if constexpr (RES) {
-                const float4 r = lds_f4(at);
-                const uint32_t u[4] = {__float_as_uint(r.x), __float_as_uint(r.y), __float_as_uint(r.z), __float_as_uint(r.w)};
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                  v[8 * k + 2 * i] += __uint_as_float(u[i] << 16);
-                  v[8 * k + 2 * i + 1] += __uint_as_float(u[i] & 0xFFFF0000u);
-                }
-              }
-              sts_u4(at, make_uint4(bf16x2(v[8 * k], v[8 * k + 1]), bf16x2(v[8 * k + 2], v[8 * k + 3]),
-                                    bf16x2(v[8 * k + 4], v[8 * k + 5]), bf16x2(v[8 * k + 6], v[8 * k + 7])));
-            }
-          }
-          if ((c + 32) % S::BC == 0) {
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&ymap, (int)c0 + bx * S::BC, (int)r0, box + bx * BOX);
-              bulk_commit();
-            }
+        if ((c + 32) % S::BC == 0) {
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&ymap, (int)c0 + bx * S::BC, (int)r0, box + bx * BOX);
+            bulk_commit();
           }
         }
       }
       tc_fence_before();
     }
     if (lane == 0) {
-      if (!ok && RES) {  // residual boxes still in flight land before the shared memory goes
+      if (!ok) {  // residual boxes still in flight land before the shared memory goes
         const unsigned long long w0 = tc_now();
         while (tc_now() - w0 < 1000000ull) __nanosleep(1000);
       }
@@ -1300,7 +1188,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) v[i] += bias_r[i];
-    if (a.gelu) gelu_fast2(v[0], v[1]), gelu_fast2(v[2], v[3]);
+    if (a.gelu) gelu_fast<4>(v);
     if (OUT != FP8_E4M3) {
 #pragma unroll
       for (int i = 0; i < 4; i++) v[i] += res_r[i];
@@ -1443,35 +1331,25 @@ static cudaError_t launch_pair(const Fp8Linear& a, int* err, cudaStream_t st) {
   const long tiles = (long)p.m_tiles * p.n_tiles;
   const int pairs = num_sms() / 2;
   if (pairs <= 0) return cudaErrorInvalidDevice;
-  kernel<<<2 * (unsigned)(tiles < pairs ? tiles : pairs), PAIR_THREADS, S::SMEM, st>>>(m.x, m.w, m.y, p);
+  kernel<<<2 * (unsigned)(tiles < pairs ? tiles : pairs), S::THREADS, S::SMEM, st>>>(m.x, m.w, m.y, p);
   return cudaGetLastError();
 }
 
-template <int OUT, bool RES, bool STAT>
+template <int OUT>
 static cudaError_t launch_tile(const Fp8Linear& a, int* err, cudaStream_t st) {
-  using S = TileShape<OUT, RES, STAT>;
+  using S = TileShape<OUT>;
   TcFp8Args p;
   PairMaps m;
   p.err = err;
   if (!make_pair_maps(a, S::N, &p, &m)) return cudaErrorInvalidValue;
-  const auto kernel = fp8_linear_tile_kernel<OUT, RES, STAT>;
+  const auto kernel = fp8_linear_tile_kernel<OUT>;
   static std::atomic<uint64_t> allowed{0};
-  const cudaError_t e = allow_smem(kernel, 227 * 1024, &allowed);
+  const cudaError_t e = allow_smem(kernel, S::SMEM, &allowed);
   if (e != cudaSuccess) return e;
+  const long tiles = (long)p.m_tiles * p.n_tiles;
   const int pairs = num_sms() / 2;
   if (pairs <= 0) return cudaErrorInvalidDevice;
-  p.stages = S::stages(p.kb);
-  const int smem = 1024 + S::OFF_A + p.stages * S::BPS * S::A_BYTES + (STAT ? p.kb : p.stages) * S::B_BYTES;
-  long used;
-  if (STAT) {  // whole columns of tiles, no more pairs to a column than it has rows
-    const long per = pairs / p.n_tiles;
-    if (per == 0 || p.kb > S::KB_MAX) return cudaErrorInvalidValue;
-    used = (per < p.m_tiles ? per : p.m_tiles) * p.n_tiles;
-  } else {
-    const long tiles = (long)p.m_tiles * p.n_tiles;
-    used = tiles < pairs ? tiles : pairs;
-  }
-  kernel<<<2 * (unsigned)used, S::THREADS, smem, st>>>(m.x, m.w, m.y, m.r, p);
+  kernel<<<2 * (unsigned)(tiles < pairs ? tiles : pairs), S::THREADS, S::SMEM, st>>>(m.x, m.w, m.y, m.r, p);
   return cudaGetLastError();
 }
 
@@ -1535,12 +1413,10 @@ static cudaError_t launch_out(const Fp8Linear& a, int* err, cudaStream_t st) {
       if (narrow) return launch_split<64, OUT>(a, splits, err, st);
     return launch_split<128, OUT>(a, splits, err, st);
   }
-  using T = TileShape<OUT, false, true>;
-  const bool stat = (a.k + 127) / 128 <= T::KB_MAX && (a.n + T::N - 1) / T::N <= sms / 2;
   if constexpr (OUT != FP8_E4M3) {
-    if (a.res) return stat ? launch_tile<OUT, true, true>(a, err, st) : launch_tile<OUT, true, false>(a, err, st);
+    if (a.res) return launch_tile<OUT>(a, err, st);
   }
-  return stat ? launch_tile<OUT, false, true>(a, err, st) : launch_pair<OUT>(a, err, st);
+  return launch_pair<OUT>(a, err, st);
 }
 
 cudaError_t launch_fp8_linear(const Fp8Linear& a, int* err, cudaStream_t st) {

@@ -85,22 +85,39 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
   return u;
 }
 
-// gelu_new(x) = x / 2 (1 + tanh(u)) = x / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3), with the
-// hardware exponential and reciprocal: about 2^-21 relative near 0 and above. (The bf16 layers use the
-// hardware tanh, 2^-11; here the result may be kept in 32 bits, or be rounded to e4m3, where an error of
-// 2^-11 moves one value in a hundred to the neighbouring code.)
-__device__ __forceinline__ void gelu_fast2(float& a, float& b) {
-  constexpr float c = -2.0f * 0.797884560802865355f * 1.44269504088896341f;  // -2 sqrt(2 / pi) log2(e)
-  const uint64_t x = pack2(a, b);
-  const uint64_t z = mul2(x, fma2(mul2(x, x), pack2(0.044715f * c, 0.044715f * c), pack2(c, c)));
-  float t0, t1, r0, r1;
-  unpack2(z, t0, t1);
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(t0));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(t1));
-  add2(t0, t1, 1.0f, 1.0f);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(t0));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(t1));
-  unpack2(mul2(x, pack2(r0, r1)), a, b);
+// gelu_new(x) = x / 2 (1 + tanh(u)) = x / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3), of four values,
+// with the hardware exponential and one reciprocal for the four: 1 / a = b c d / (a b c d). The exponential and
+// reciprocal unit gives 4 results a clock to a quarter of the SM, so at two a value it, not the MMAs, would bound a
+// layer of 768 columns. Values below -5.6, where gelu_new is above -2.7e-9, count as -5.6, so that the product of the
+// four denominators stays finite; NaN stays NaN. About 2^-20 relative near 0 and above. (The bf16 layers use the
+// hardware tanh, 2^-11; here the result may be kept in 32 bits, or be rounded to e4m3, where an error of 2^-11 moves
+// one value in a hundred to the neighbouring code.)
+template <int N>  // a multiple of 4; the steps of all N values side by side, because each step waits for the one before
+__device__ __forceinline__ void gelu_fast(float* v) {
+  constexpr float k = -2.0f * 0.797884560802865355f * 1.44269504088896341f;  // -2 sqrt(2 / pi) log2(e)
+  const uint64_t k1 = pack2(0.044715f * k, 0.044715f * k), k0 = pack2(k, k);
+  float t[N], r[N / 2];
+#pragma unroll
+  for (int i = 0; i < N; i++) asm("max.NaN.f32 %0, %1, %2;" : "=f"(v[i]) : "f"(v[i]), "f"(-5.6f));
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const uint64_t x = pack2(v[i], v[i + 1]);
+    unpack2(mul2(x, fma2(mul2(x, x), k1, k0)), t[i], t[i + 1]);
+  }
+#pragma unroll
+  for (int i = 0; i < N; i++) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t[i]) : "f"(t[i]));
+#pragma unroll
+  for (int i = 0; i < N; i += 2) add2(t[i], t[i + 1], 1.0f, 1.0f);
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const float p0 = t[i] * t[i + 1], p1 = t[i + 2] * t[i + 3];
+    float q;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(p0 * p1));
+    r[i / 2] = q * p1, r[i / 2 + 1] = q * p0;  // 1 / p0, 1 / p1
+  }
+#pragma unroll
+  for (int i = 0; i < N; i += 2)
+    unpack2(mul2(pack2(v[i], v[i + 1]), mul2(pack2(t[i + 1], t[i]), pack2(r[i / 2], r[i / 2]))), v[i], v[i + 1]);
 }
 
 }  // namespace kk
