@@ -171,6 +171,45 @@ def test_linear_nan_reaches_its_row_only(kk):
         assert y[3].isnan().all() and not y[:3].isnan().any() and not y[4:].isnan().any()
 
 
+@pytest.mark.parametrize("m, n, k", [(5, 300, 256), (700, 640, 520), (4800, 1000, 300), (4800, 1000, 1700)])
+@pytest.mark.parametrize("act", [None, "gelu"])
+def test_linear_nan_column(kk, m, n, k, act):
+    """A NaN or an infinity in one column's bias, or in a weight, stays in that column."""
+    rng = np.random.default_rng(11)
+    fp8 = kk.fp8
+    x = fp8.quantize(torch.from_numpy(rng.standard_normal((m, k)).astype(np.float32)).cuda())
+    w = (rng.standard_normal((n, k)) / np.sqrt(k)).astype(np.float32)
+    w[17, 3] = np.nan
+    w = fp8.quantize(torch.from_numpy(w).cuda(), block_rows=128)
+    bias = torch.zeros(n, device="cuda")
+    bias[130], bias[131], bias[n - 1] = float("nan"), float("inf"), float("-inf")
+    res = torch.ones(m, n, device="cuda")
+    fine = torch.ones(n, dtype=torch.bool, device="cuda")
+    fine[[17, 130, 131, n - 1]] = False
+    for dtype in (torch.float32, torch.bfloat16, E4M3):
+        for r in (None, res) if dtype != E4M3 else (None,):
+            y = fp8.linear(x, w, bias, act=act, out_dtype=dtype, residual=None if r is None else r.to(dtype))
+            y = fp8.dequantize(y) if dtype == E4M3 else y.float()
+            assert y[:, fine].isfinite().all()
+            assert y[:, [17, 130]].isnan().all()
+            assert (y[:, 131].isnan() if dtype == E4M3 else y[:, 131] == float("inf")).all()
+
+
+@pytest.mark.parametrize("m, n", [(3, 128), (300, 256), (5000, 1024)])
+def test_gelu_over_its_range(kk, m, n):
+    """GELU of given values, through a layer whose product is zero: |error| <= 2^-20 |y| + 2^-27 (values below -5.6
+    count as -5.6, 2.7e-9) in 32 bits."""
+    rng = np.random.default_rng(m)
+    bias = np.concatenate([np.linspace(-12, 12, n - 8), [0.0, 1e-30, -1e-30, 30.0, -30.0, 1e4, -1e4, 3e38]]).astype(np.float32)
+    bias[:-8] = rng.permutation(bias[:-8])
+    x = kk.fp8.quantize(torch.zeros(m, 128, device="cuda"))
+    w = kk.fp8.quantize(torch.zeros(n, 128, device="cuda"), block_rows=128)
+    got = kk.fp8.linear(x, w, torch.from_numpy(bias).cuda(), act="gelu").double().cpu().numpy()
+    with np.errstate(over="ignore"):
+        want = ref.gelu(bias.astype(np.float64))
+    assert (np.abs(got - want) <= 2.0 ** -20 * np.abs(want) + 2.0 ** -27).all(), np.abs(got - want).max(0)
+
+
 def test_linear_far_apart_scales(kk):
     """Rows of zeros, of 1e-30 and of 1e30 in one tile: each keeps its own relative accuracy."""
     rng = np.random.default_rng(4)
