@@ -1397,20 +1397,29 @@ static cudaError_t launch_split(const Fp8Linear& a, int splits, int* err, cudaSt
   return cudaLaunchKernelEx(&cfg, kernel, xm, wm, p);
 }
 
+// Which kernel, by the number of tiles and of blocks of K (times of launches in a row, us).
+//  * Split kernel up to two CTAs an SM, one when K is long: rows x K -> n 2048 x 768 -> 2304 (288 tiles of 128) 9.1
+//    against 9.4 with pairs, 4096 x 768 -> 2304 (576) 16.1 against 12.9; 1024 x 4096 -> 4096 (256) 19.8 against 17.7.
+//  * Its tiles are 64 columns wide while those are few (up to 1.5 an SM): 512 x 768 -> 2304 (144) 5.9 against 6.8 with
+//    128, 2048 x 768 -> 768 (192) 8.6 against 9.6, 1024 x 768 -> 2304 (288) 7.4 against 7.1; 128 wide for an e4m3 result,
+//    whose blocks are, and when K is long, where a CTA has more of W on its way: 1 x 8192 -> 8192 11.3 against 14.4.
+//  * K is split (a cluster costs about 0.5 us to start and more the more there are) into shares of four blocks or more,
+//    as far as every CTA has an SM of its own, or half of one when K is long: 1 x 2048 -> 768 5.4 in four shares against
+//    7.4 in one, 1 x 768 -> 2304 5.1 in one against 5.5 in two, 512 x 2048 -> 768 8.0 in two (96 CTAs) against 9.3 in one
+//    and 14.5 in eight (384).
 template <int OUT>
 static cudaError_t launch_out(const Fp8Linear& a, int* err, cudaStream_t st) {
-  const int sms = num_sms();
+  const int sms = num_sms(), kb = (int)((a.k + 127) / 128);
   if (sms <= 0) return cudaErrorInvalidDevice;
-  const long rows = (a.m + TM - 1) / TM, t128 = rows * ((a.n + 127) / 128);
-  if (t128 <= 2 * sms) {
-    const int kb = (int)((a.k + 127) / 128);
-    const long t64 = rows * ((a.n + 63) / 64);
-    const bool narrow = OUT != FP8_E4M3 && t64 <= sms;
-    const long tiles = narrow ? t64 : t128;
+  const long rows = (a.m + TM - 1) / TM, t128 = rows * ((a.n + 127) / 128), t64 = rows * ((a.n + 63) / 64);
+  if (t128 <= (kb > 16 ? sms : 2 * sms)) {
+    const bool long_k = kb > 32, narrow = OUT != FP8_E4M3 && !long_k && t64 <= sms + sms / 2;
+    const long tiles = narrow ? t64 : t128, room = long_k ? 2 * sms : sms;
     int splits = 1;
-    while (splits < 8 && 2 * splits <= kb && tiles * 2 * splits <= 2 * sms) splits *= 2;
-    if constexpr (OUT != FP8_E4M3)
+    while (splits < 8 && 4 * 2 * splits <= kb && tiles * 2 * splits <= room) splits *= 2;
+    if constexpr (OUT != FP8_E4M3) {
       if (narrow) return launch_split<64, OUT>(a, splits, err, st);
+    }
     return launch_split<128, OUT>(a, splits, err, st);
   }
   if constexpr (OUT != FP8_E4M3) {

@@ -94,22 +94,17 @@ class Fp8Tensor:
         self._args = (at, ldv, at + rows * ldv, lde)
         return self
 
-    def _views(self) -> None:
-        (rows, k), (_, ldv, _, lde) = self.shape, self._args
-        n = rows * ldv
-        self._values = self._buf[:n].view(E4M3).view(rows, ldv)[:, :k]
-        self._exps = self._buf[n:].view(-(-rows // self.block_rows), lde)[:, : -(-k // 128)]
-
     @property
     def values(self) -> torch.Tensor:
         if self._values is None:
-            self._views()
+            self._values = self._buf.view(E4M3).as_strided(self.shape, (self._args[1], 1))
         return self._values
 
     @property
     def exps(self) -> torch.Tensor:
         if self._exps is None:
-            self._views()
+            (rows, k), (_, ldv, _, lde) = self.shape, self._args
+            self._exps = self._buf.as_strided((-(-rows // self.block_rows), -(-k // 128)), (lde, 1), rows * ldv)
         return self._exps
 
     def __getitem__(self, rows: slice) -> "Fp8Tensor":
