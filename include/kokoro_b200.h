@@ -376,7 +376,8 @@ KK_API const char* kk_conv_selftest_error(void);
  * lde of 4; values are 16-byte and exps 4-byte aligned. A block's E is the smallest integer >= 0 with
  * max |x| <= 448 * 2^(E - 127) over its finite values; values are rounded to nearest even; infinities and
  * NaN are held as NaN, which e4m3 has, and so reach every result that reads them. Nothing but the rows x k
- * values and their exps is written: not the bytes between k and ldv, nor rows behind the last.
+ * values and their exps is written: not the bytes between k and ldv, nor rows behind the last. (kk_fp8_linear
+ * reads exps by whole 4-byte words.)
  *
  * All pointers are device pointers of device `cuda_ordinal`; `stream` is a cudaStream_t of that device
  * (NULL: its legacy default stream). The calls only enqueue work (they may be captured into a graph),
@@ -396,7 +397,8 @@ KK_API kk_status kk_fp8_dequantize(int cuda_ordinal, void* stream, const uint8_t
 /*
  * y = act(x w^T + bias) + residual: x a store of m rows (block_rows 1), w a store of n rows (block_rows
  * 128), both of k columns; bias [n] or NULL; sums in 32 bits. y_type KK_FP8_F32 / KK_FP8_BF16: y [m][n],
- * ldy elements apart, residual of the same type (ldr elements apart; NULL: none; it may be y itself).
+ * ldy elements apart, residual of the same type (ldr elements apart; NULL: none; it may be y itself, or not
+ * overlap it).
  * y_type KK_FP8_E4M3: y / ldy and y_exps / ldye are a store (block_rows 1) that the result is quantised
  * into, without a residual. y may not overlap x or w.
  */

@@ -1,7 +1,6 @@
 // C entries of the 8-bit operators: argument checks, the caller's device and stream, status codes.
 #include <cuda_runtime.h>
 #include <atomic>
-#include <exception>
 #include <string>
 
 #include "../../include/kokoro_b200.h"
@@ -11,8 +10,14 @@ namespace {
 
 thread_local std::string g_fp8_error;
 
-kk_status fail(kk_status s, const std::string& m) {
-  g_fp8_error = m;
+// the status, its message kept for kk_fp8_error (nothing is thrown across the C boundary)
+kk_status fail(kk_status s, const char* what, const char* message = "") noexcept {
+  try {
+    g_fp8_error = what;
+    g_fp8_error += message;
+  } catch (...) {
+    g_fp8_error.clear();
+  }
   return s;
 }
 
@@ -82,21 +87,15 @@ int device_kind(int ordinal) {
 }
 
 kk_status run(int ordinal, const char* what, cudaError_t (*f)(const void*, cudaStream_t), const void* arg, void* stream) {
-  try {
-    const int kind = device_kind(ordinal);
-    if (kind == 3) return fail(KK_ERR_INVALID_ARG, "CUDA device ordinal out of range");
-    if (kind == 2) return fail(KK_ERR_CUDA, "device is not compute capability 10.x (sm_100a)");
-    DeviceGuard g(ordinal);
-    if (g.err != cudaSuccess) return fail(KK_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(g.err));
-    const cudaError_t e = f(arg, (cudaStream_t)stream);
-    if (e != cudaSuccess) {
-      cudaGetLastError();
-      return fail(e == cudaErrorMemoryAllocation ? KK_ERR_OOM : KK_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
-    }
-    return KK_OK;
-  } catch (const std::exception& x) {
-    return fail(KK_ERR_CUDA, x.what());
-  }
+  const int kind = device_kind(ordinal);
+  if (kind == 3) return fail(KK_ERR_INVALID_ARG, "CUDA device ordinal out of range");
+  if (kind == 2) return fail(KK_ERR_CUDA, "device is not compute capability 10.x (sm_100a)");
+  DeviceGuard g(ordinal);
+  if (g.err != cudaSuccess) return fail(KK_ERR_CUDA, what, cudaGetErrorString(g.err));
+  const cudaError_t e = f(arg, (cudaStream_t)stream);
+  if (e == cudaSuccess) return KK_OK;
+  cudaGetLastError();
+  return fail(e == cudaErrorMemoryAllocation ? KK_ERR_OOM : KK_ERR_CUDA, what, cudaGetErrorString(e));
 }
 
 struct QuantArgs {
@@ -121,7 +120,7 @@ kk_status kk_fp8_quantize(int cuda_ordinal, void* stream, const void* x, int typ
   if (const char* m = bad_rows(x, type, k, ldx)) return fail(KK_ERR_INVALID_ARG, m);
   if (const char* m = bad_store(values, ldv, exps, lde, k)) return fail(KK_ERR_INVALID_ARG, m);
   QuantArgs a{x, type, (long)rows, (long)k, (long)ldx, block_rows, {values, (long)ldv, exps, (long)lde}};
-  return run(cuda_ordinal, "kk_fp8_quantize", [](const void* p, cudaStream_t st) {
+  return run(cuda_ordinal, "kk_fp8_quantize: ", [](const void* p, cudaStream_t st) {
     const QuantArgs& a = *(const QuantArgs*)p;
     return kk::launch_fp8_quantize(a.x, a.type, a.rows, a.k, a.ld, a.block_rows, a.q, st);
   }, &a, stream);
@@ -136,7 +135,7 @@ kk_status kk_fp8_dequantize(int cuda_ordinal, void* stream, const uint8_t* value
   if (const char* m = bad_store(values, ldv, exps, lde, k)) return fail(KK_ERR_INVALID_ARG, m);
   QuantArgs a{y, type, (long)rows, (long)k, (long)ldy, block_rows,
               {const_cast<uint8_t*>(values), (long)ldv, const_cast<uint8_t*>(exps), (long)lde}};
-  return run(cuda_ordinal, "kk_fp8_dequantize", [](const void* p, cudaStream_t st) {
+  return run(cuda_ordinal, "kk_fp8_dequantize: ", [](const void* p, cudaStream_t st) {
     const QuantArgs& a = *(const QuantArgs*)p;
     return kk::launch_fp8_dequantize(a.q, a.rows, a.k, a.block_rows, const_cast<void*>(a.x), a.type, a.ld, st);
   }, &a, stream);
@@ -153,16 +152,16 @@ kk_status kk_fp8_linear(int cuda_ordinal, void* stream, int64_t m, int64_t n, in
   if (y_type != KK_FP8_F32 && y_type != KK_FP8_BF16 && y_type != KK_FP8_E4M3)
     return fail(KK_ERR_INVALID_ARG, "unknown output type");
   if (m == 0) return KK_OK;
-  if (const char* s = bad_store(x, ldx, x_exps, ldxe, k)) return fail(KK_ERR_INVALID_ARG, std::string("x: ") + s);
-  if (const char* s = bad_store(w, ldw, w_exps, ldwe, k)) return fail(KK_ERR_INVALID_ARG, std::string("w: ") + s);
+  if (const char* s = bad_store(x, ldx, x_exps, ldxe, k)) return fail(KK_ERR_INVALID_ARG, "x: ", s);
+  if (const char* s = bad_store(w, ldw, w_exps, ldwe, k)) return fail(KK_ERR_INVALID_ARG, "w: ", s);
   if (!aligned(bias, 4)) return fail(KK_ERR_INVALID_ARG, "bias must be 4-byte aligned");
   if (y_type == KK_FP8_E4M3) {
     if (residual) return fail(KK_ERR_INVALID_ARG, "an e4m3 result takes no residual");
-    if (const char* s = bad_store(y, ldy, y_exps, ldye, n)) return fail(KK_ERR_INVALID_ARG, std::string("y: ") + s);
+    if (const char* s = bad_store(y, ldy, y_exps, ldye, n)) return fail(KK_ERR_INVALID_ARG, "y: ", s);
   } else {
-    if (const char* s = bad_rows(y, y_type, n, ldy)) return fail(KK_ERR_INVALID_ARG, std::string("y: ") + s);
+    if (const char* s = bad_rows(y, y_type, n, ldy)) return fail(KK_ERR_INVALID_ARG, "y: ", s);
     if (residual)
-      if (const char* s = bad_rows(residual, y_type, n, ldr)) return fail(KK_ERR_INVALID_ARG, std::string("residual: ") + s);
+      if (const char* s = bad_rows(residual, y_type, n, ldr)) return fail(KK_ERR_INVALID_ARG, "residual: ", s);
   }
   struct Args {
     kk::Fp8Linear a;
@@ -175,7 +174,7 @@ kk_status kk_fp8_linear(int cuda_ordinal, void* stream, int64_t m, int64_t n, in
     g.a.q = {(uint8_t*)y, (long)ldy, y_exps, (long)ldye};
   else
     g.a.y = y, g.a.ldy = (long)ldy;
-  return run(cuda_ordinal, "kk_fp8_linear", [](const void* p, cudaStream_t st) {
+  return run(cuda_ordinal, "kk_fp8_linear: ", [](const void* p, cudaStream_t st) {
     return kk::launch_fp8_linear(((const Args*)p)->a, nullptr, st);
   }, &g, stream);
 }
@@ -183,10 +182,10 @@ kk_status kk_fp8_linear(int cuda_ordinal, void* stream, int64_t m, int64_t n, in
 kk_status kk_fp8_check(int cuda_ordinal, void* stream) {
   int flag = 0;
   int* const out = &flag;
-  const kk_status s = run(cuda_ordinal, "kk_fp8_check", [](const void* p, cudaStream_t st) {
+  const kk_status s = run(cuda_ordinal, "kk_fp8_check: ", [](const void* p, cudaStream_t st) {
     return kk::fp8_take_wait_error(*(int* const*)p, st);
   }, &out, stream);
-  if (s == KK_OK && flag) return fail(KK_ERR_TIMEOUT, "a bounded wait of kk_fp8_linear expired (code " + std::to_string(flag) + ")");
+  if (s == KK_OK && flag) return fail(KK_ERR_TIMEOUT, "a bounded pipeline wait of kk_fp8_linear expired");
   return s;
 }
 

@@ -623,62 +623,66 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<OUT>::THRE
           }
         }
       } else {
-        constexpr int BC = OUT == FP8_F32 ? 32 : 64, NCH = S::COLS / BC;  // columns of a box, boxes of a warp
-        const int ch0 = shares && cg != 0 ? NCH - 64 / BC : 0;  // the boxes of the shared columns come first
+        constexpr int BC = OUT == FP8_F32 ? 32 : 64;  // columns of a box
+        // 64 columns at a time, the shared ones first, all read (and handed on) before anything is done with them
 #pragma unroll 1
-        for (int i = 0; i < NCH; i++) {
-          const int ch = (i + ch0) % NCH;
-          const long cx = c0 + ch * BC;  // the box's first column
-          const bool on = live && cx < a.n, tma = on && p.tma_y && (p.tma_edge || cx + BC <= a.n);
-          if (tma) {
-            if (lane == 0) bulk_wait_all_read();
+        for (int i = 0; i < S::COLS / 64; i++) {
+          const int half = shares && cg != 0 ? S::COLS / 64 - 1 - i : i;
+          float v[64];
+          tmem_ld64(d + 64 * half, v);
+          if (shares && i == 0) {
+            tc_fence_before();
             __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(acc_free0);
           }
 #pragma unroll
-          for (int h = 0; h < BC / 32; h++) {
-            const int c = ch * BC + 32 * h;
-            float v[32];
-            tmem_ld32(d + c, v);
-            if (shares && (BC == 32 ? i == 1 : i == 0 && h == 1)) {
-              tc_fence_before();
+          for (int b = 0; b < 64 / BC; b++) {
+            const int c = 64 * half + BC * b;  // of the warp's columns
+            const long cx = c0 + c;            // the box's first column
+            if (!live || cx >= a.n) continue;
+            const bool tma = p.tma_y && (p.tma_edge || cx + BC <= a.n);
+            if (tma) {
+              if (lane == 0) bulk_wait_all_read();
               __syncwarp();
-              if (lane == 0) mbar_arrive_cluster_relaxed(acc_free0);
             }
-            if (!on) continue;
-            add_bias32(v, bias_s + c);
-            if (a.gelu) {
 #pragma unroll
-              for (int j = 0; j < 32; j += 16) gelu_fast<16>(v + j);
-            }
-            if (!tma) {
-              if (c0 + c < a.n) {
-                if constexpr (OUT == FP8_F32)
-                  store_any<float>(a, v, r0, c0 + c, lane);
-                else
-                  store_any<__nv_bfloat16>(a, v, r0, c0 + c, lane);
+            for (int h = 0; h < BC / 32; h++) {
+              float* w = v + BC * b + 32 * h;
+              add_bias32(w, bias_s + c + 32 * h);
+              if (a.gelu) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 16) gelu_fast<16>(w + j);
               }
-              continue;
-            }
-            if constexpr (OUT == FP8_F32) {
+              if (!tma) {
+                if (cx + 32 * h < a.n) {
+                  if constexpr (OUT == FP8_F32)
+                    store_any<float>(a, w, r0, cx + 32 * h, lane);
+                  else
+                    store_any<__nv_bfloat16>(a, w, r0, cx + 32 * h, lane);
+                }
+                continue;
+              }
+              if constexpr (OUT == FP8_F32) {
 #pragma unroll
-              for (int q = 0; q < 8; q++)
-                sts_u4(row_s + ((q ^ (lane & 7)) << 4),
-                       make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]),
-                                  __float_as_uint(v[4 * q + 3])));
-            } else {
+                for (int q = 0; q < 8; q++)
+                  sts_u4(row_s + ((q ^ (lane & 7)) << 4),
+                         make_uint4(__float_as_uint(w[4 * q]), __float_as_uint(w[4 * q + 1]), __float_as_uint(w[4 * q + 2]),
+                                    __float_as_uint(w[4 * q + 3])));
+              } else {
 #pragma unroll
-              for (int q = 0; q < 4; q++)
-                sts_u4(row_s + (((4 * h + q) ^ (lane & 7)) << 4),
-                       make_uint4(bf16x2(v[8 * q], v[8 * q + 1]), bf16x2(v[8 * q + 2], v[8 * q + 3]),
-                                  bf16x2(v[8 * q + 4], v[8 * q + 5]), bf16x2(v[8 * q + 6], v[8 * q + 7])));
+                for (int q = 0; q < 4; q++)
+                  sts_u4(row_s + (((4 * h + q) ^ (lane & 7)) << 4),
+                         make_uint4(bf16x2(w[8 * q], w[8 * q + 1]), bf16x2(w[8 * q + 2], w[8 * q + 3]),
+                                    bf16x2(w[8 * q + 4], w[8 * q + 5]), bf16x2(w[8 * q + 6], w[8 * q + 7])));
+              }
             }
-          }
-          if (!tma) continue;
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&ymap, (int)cx, (int)r0, box);
-            bulk_commit();
+            if (!tma) continue;
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&ymap, (int)cx, (int)r0, box);
+              bulk_commit();
+            }
           }
         }
       }
@@ -1403,10 +1407,11 @@ static cudaError_t launch_split(const Fp8Linear& a, int splits, int* err, cudaSt
 //  * Its tiles are 64 columns wide while those are few (up to 1.5 an SM): 512 x 768 -> 2304 (144) 5.9 against 6.8 with
 //    128, 2048 x 768 -> 768 (192) 8.6 against 9.6, 1024 x 768 -> 2304 (288) 7.4 against 7.1; 128 wide for an e4m3 result,
 //    whose blocks are, and when K is long, where a CTA has more of W on its way: 1 x 8192 -> 8192 11.3 against 14.4.
-//  * K is split (a cluster costs about 0.5 us to start and more the more there are) into shares of four blocks or more,
-//    as far as every CTA has an SM of its own, or half of one when K is long: 1 x 2048 -> 768 5.4 in four shares against
-//    7.4 in one, 1 x 768 -> 2304 5.1 in one against 5.5 in two, 512 x 2048 -> 768 8.0 in two (96 CTAs) against 9.3 in one
-//    and 14.5 in eight (384).
+//  * K is split (a cluster costs about 0.5 us to start and more the more there are) into shares of four blocks or more
+//    (one for an e4m3 result, whose epilogue the shares split too: 256 x 768 -> 2048 8.1 in four against 9.4), as far as
+//    every CTA has an SM of its own, or half of one when K is long: 1 x 2048 -> 768 5.4 in four shares against 7.4 in
+//    one, 1 x 768 -> 2304 5.1 in one against 5.5 in two, 512 x 2048 -> 768 8.0 in two (96 CTAs) against 9.3 in one and
+//    14.5 in eight (384).
 template <int OUT>
 static cudaError_t launch_out(const Fp8Linear& a, int* err, cudaStream_t st) {
   const int sms = num_sms(), kb = (int)((a.k + 127) / 128);
@@ -1416,7 +1421,8 @@ static cudaError_t launch_out(const Fp8Linear& a, int* err, cudaStream_t st) {
     const bool long_k = kb > 32, narrow = OUT != FP8_E4M3 && !long_k && t64 <= sms + sms / 2;
     const long tiles = narrow ? t64 : t128, room = long_k ? 2 * sms : sms;
     int splits = 1;
-    while (splits < 8 && 4 * 2 * splits <= kb && tiles * 2 * splits <= room) splits *= 2;
+    const int least = OUT == FP8_E4M3 ? 1 : 4;  // blocks of a share
+    while (splits < 8 && least * 2 * splits <= kb && tiles * 2 * splits <= room) splits *= 2;
     if constexpr (OUT != FP8_E4M3) {
       if (narrow) return launch_split<64, OUT>(a, splits, err, st);
     }

@@ -142,7 +142,8 @@ def check_linear(got, y, S, rms, K, act, dtype):
 SIZES = [(1, 1, 1), (1, 16, 128), (1, 768, 768), (2, 130, 100), (7, 128, 129), (16, 2304, 768), (17, 50, 512), (33, 257, 300),
          (64, 512, 768), (65, 96, 640), (66, 2048, 768), (128, 768, 2048), (129, 255, 16), (200, 1090, 514), (300, 769, 1100),
          (512, 768, 2048), (700, 640, 520), (4800, 1000, 384), (9501, 513, 640), (2600, 2304, 768),
-         (3, 20000, 4700), (140, 1000, 2500), (4800, 1000, 1700), (5003, 1157, 2100), (4900, 1024, 1030)]
+         (3, 20000, 4700), (140, 1000, 2500), (4800, 1000, 1700), (5003, 1157, 2100), (4900, 1024, 1030), (40000, 1, 130),
+         (20000, 300, 33)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, E4M3])
@@ -275,12 +276,15 @@ def test_linear_result_store_within_a_larger_one(kk):
         assert (e[:2] == 0x66).all() and (e[m + 2:] == 0x66).all() and (e[:, 3:] == 0x66).all()
 
 
-def test_rows_do_not_depend_on_the_batch_they_are_in(kk):
-    """Same inputs, same bits; and twice the same."""
+@pytest.mark.parametrize("m, n, k", [(3, 768, 2048), (700, 768, 2048), (5000, 1024, 768)])
+def test_linear_twice_the_same(kk, m, n, k):
+    """Same inputs, same bits (shares of K are added in their order)."""
     rng = np.random.default_rng(10)
-    xq, wq, _, _ = make(rng, 700, 768, 2048, kk.fp8)
-    a, b = kk.fp8.linear(xq, wq), kk.fp8.linear(xq, wq)
-    assert torch.equal(a, b)
+    xq, wq, _, _ = make(rng, m, n, k, kk.fp8)
+    r = torch.randn(m, n, device="cuda")
+    for res in (None, r):
+        a, b = kk.fp8.linear(xq, wq, residual=res), kk.fp8.linear(xq, wq, residual=res)
+        assert torch.equal(a, b)
 
 
 def feed_forward(fp8, x, w1, b1, w2, b2, residual):
@@ -400,3 +404,66 @@ def test_no_rows(kk):
 def test_no_wait_has_expired(kk):
     kk.fp8.check()
     kk.fp8.check("cuda:0")
+
+
+FIRST_CALL_IN_A_CAPTURE = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+import conftest
+fp8 = conftest.import_package().fp8
+x, w = torch.randn(300, 768, device="cuda"), torch.randn(2048, 768, device="cuda") / 30
+b = torch.randn(2048, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    wq = fp8.quantize(w, block_rows=128)
+    y = fp8.dequantize(fp8.linear(fp8.quantize(x), wq, b, act="gelu", out_dtype=torch.float8_e4m3fn))
+x.copy_(torch.randn(300, 768, device="cuda"))
+g.replay()
+want = fp8.dequantize(fp8.linear(fp8.quantize(x), fp8.quantize(w, 128), b, act="gelu", out_dtype=torch.float8_e4m3fn))
+assert torch.equal(y, want)
+fp8.check()
+print("fine")
+"""
+
+
+def test_first_call_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_CAPTURE, os.path.dirname(os.path.abspath(__file__))],
+                       capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+def test_calls_of_several_host_threads_at_once(kk):
+    import threading
+    fp8 = kk.fp8
+    torch.manual_seed(1)
+    x = torch.randn(2000, 768, device="cuda")
+    w1, w2 = (fp8.quantize(torch.randn(s, device="cuda") / 30, block_rows=128) for s in ((2048, 768), (768, 2048)))
+    b1, b2 = torch.randn(2048, device="cuda"), torch.randn(768, device="cuda")
+    sizes = (1, 40, 300, 2000)
+    want = [feed_forward(fp8, x[:n], w1, b1, w2, b2, x[:n]) for n in sizes]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    n = sizes[i]
+                    y = feed_forward(fp8, x[:n], w1, b1, w2, b2, x[:n])
+                    torch.cuda.current_stream().synchronize()
+                    if not torch.equal(y, want[i]):
+                        bad.append(i)
+        except Exception as e:  # noqa: BLE001
+            bad.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+    fp8.check()
