@@ -88,27 +88,37 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
 // gelu_new(x) = x / 2 (1 + tanh(u)) = x / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3), with the hardware
 // exponential and reciprocal: about 2^-20 relative near 0 and above. (The bf16 layers use the hardware tanh, 2^-11; here
 // the result may be kept in 32 bits, or be rounded to e4m3, where an error of 2^-11 moves one value in a hundred to the
-// neighbouring code.) The epilogues that call it are bound by the instructions they issue, so taking work off the unit
-// for exponentials and reciprocals pays little: exponentials on the FMA pipe measured 5% slower, one reciprocal for four
-// values 4% faster, for which a NaN reaches its neighbours and large negative values have to be clamped.
-template <int N>  // even; the steps of all N values side by side, because each step waits for the one before
+// neighbouring code.) The unit for both gives 16 results a clock and SM, which at two a value bounds a layer of 768
+// columns, so one reciprocal serves four values: 1 / a = b c d / (a b c d), 11% of the layer. For that the denominators
+// have to stay finite: values below -5.6, where gelu_new is above -2.7e-9, count as -5.6, and a NaN is kept from its
+// neighbours' product (fminf takes the number) but stays NaN itself. (Exponentials on the FMA pipe measured slower:
+// then it is the instructions.)
+template <int N>  // a multiple of 4; the steps of all N values side by side, because each step waits for the one before
 __device__ __forceinline__ void gelu_fast(float* v) {
   constexpr float k = -2.0f * 0.797884560802865355f * 1.44269504088896341f;  // -2 sqrt(2 / pi) log2(e)
   const uint64_t k1 = pack2(0.044715f * k, 0.044715f * k), k0 = pack2(k, k);
-  float t[N];
+  float t[N], r[N / 2];
+#pragma unroll
+  for (int i = 0; i < N; i++) asm("max.NaN.f32 %0, %1, %2;" : "=f"(v[i]) : "f"(v[i]), "f"(-5.6f));
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
     const uint64_t x = pack2(v[i], v[i + 1]);
-    unpack2(mul2(x, fma2(mul2(x, x), k1, k0)), t[i], t[i + 1]);
+    unpack2(mul2(x, fma2(mul2(x, x), k1, k0)), t[i], t[i + 1]);  // at most 30.97
   }
 #pragma unroll
-  for (int i = 0; i < N; i++) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t[i]) : "f"(t[i]));
+  for (int i = 0; i < N; i++) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t[i]) : "f"(fminf(t[i], 31.0f)));
 #pragma unroll
   for (int i = 0; i < N; i += 2) add2(t[i], t[i + 1], 1.0f, 1.0f);
 #pragma unroll
-  for (int i = 0; i < N; i++) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t[i]) : "f"(t[i]));
+  for (int i = 0; i < N; i += 4) {
+    const float p0 = t[i] * t[i + 1], p1 = t[i + 2] * t[i + 3];
+    float q;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(p0 * p1));
+    r[i / 2] = q * p1, r[i / 2 + 1] = q * p0;  // 1 / p0, 1 / p1
+  }
 #pragma unroll
-  for (int i = 0; i < N; i += 2) unpack2(mul2(pack2(v[i], v[i + 1]), pack2(t[i], t[i + 1])), v[i], v[i + 1]);
+  for (int i = 0; i < N; i += 2)
+    unpack2(mul2(pack2(v[i], v[i + 1]), mul2(pack2(t[i + 1], t[i]), pack2(r[i / 2], r[i / 2]))), v[i], v[i + 1]);
 }
 
 }  // namespace kk
