@@ -157,6 +157,11 @@ __device__ __forceinline__ bool warp_wait_cluster(uint64_t* b, uint32_t parity, 
   return __all_sync(0xFFFFFFFFu, mbar_wait_cluster(b, parity, abort_flag, err));
 }
 
+__device__ __forceinline__ void pause_1ms() {
+  const unsigned long long t0 = tc_now();
+  while (tc_now() - t0 < 1000000ull) __nanosleep(1000);
+}
+
 constexpr int SF_RING = 4;  // scale groups (4 blocks of K each) of a pair, in shared memory and TMEM
 
 // ---- scales
@@ -280,7 +285,7 @@ struct TcFp8Args {
   int tma_edge;        // so can their last columns: TMA writes whole 16-byte units, so n has to end on one
 };
 
-// ---- large layers: a pair of CTAs per tile of 256 rows x 256 columns
+// ---- large layers: persistent pairs of CTAs, a tile of 256 rows x 256 columns at a time
 //
 // Bound by the tensor cores from about K = 1000 on, by HBM below. One CTA with a 128 x 256 tile reads 96 bytes of
 // L2 per SM and clock at the full MMA rate, more than L2 gives; a pair shares the 256 rows of W (each CTA loads
@@ -298,11 +303,12 @@ struct PairShape {
   // several at once: 10% slower with GELU)
   static constexpr int EPI = Q ? 16 : 8, COLS = Q ? 64 : 128;
   static constexpr int THREADS = 32 * (CTRL_WARPS + EPI);
-  static constexpr int STAGES = 5;
-  static constexpr int A_BYTES = TM * 128, B_BYTES = TN / 2 * 128;
-  static constexpr int SF_BYTES = 512 * 3;
-  // TMEM columns: the two accumulators share columns 192..255 (see the epilogue); scales behind them
-  static constexpr int D1 = 192, SF_COL = D1 + TN, SF_COLS = 12;
+  static constexpr int N = TN, STAGES = 5;
+  static constexpr int A_BYTES = TM * 128, B_BYTES = N / 2 * 128;
+  static constexpr int NB = N / 128, SF_BYTES = 512 * (1 + NB);
+  // TMEM columns: the two accumulators share columns 192..255 (see the epilogue), so one barrier each way goes for
+  // both; scales behind them
+  static constexpr int D1 = 192, ACC = 1, SF_COL = D1 + N, SF_COLS = 4 * (1 + NB);
   static constexpr int BOXES = 8;  // e4m3: two warps share one
   static constexpr int OFF_B = STAGES * A_BYTES, OFF_BOX = OFF_B + STAGES * B_BYTES;
   static constexpr int OFF_SF = OFF_BOX + BOXES * BOX, OFF_BIAS = OFF_SF + SF_RING * SF_BYTES;
@@ -398,140 +404,189 @@ __device__ __forceinline__ void tile_at(const TcFp8Args& p, int t, int* mt, int*
   *mt = g * G + (r - *nt * h);
 }
 
-// Persistent pairs. In each CTA warp 0 loads its boxes of x and W (128 bytes x 128 rows, 128-byte swizzle) into a
-// ring of stages, warp 2 brings the scales, four blocks of K at a time, into shared memory in the layout of the
-// TMEM copy, the last 16 are the epilogue (a thread holds 64 columns of one row; with 128 columns, which a block of an
-// e4m3 result would suggest, too few registers are left to work on several at once); warp 1 of the first CTA issues
-// the pair's MMAs. Barriers that the MMA warp waits on live in the first CTA; those it commits to, in both.
+// ---- the main loop of a pair
+//
+// In each CTA warp 0 loads its boxes of x and W (128 bytes x 128 rows, or half the tile's columns; 128-byte swizzle)
+// into a ring of stages, and warp 2 brings the scales, four blocks of K at a time; warp 1 of the first CTA issues the
+// pair's MMAs, that of the second hands its CTA's scales on. Barriers that the MMA warp waits on live in the first
+// CTA; those it commits to, in both.
+template <class S>
+struct PairLoop {
+  const TcFp8Args& p;
+  uint8_t* smem;
+  uint64_t *full, *empty, *sf_full, *sf_empty, *acc_full, *acc_free, *more;  // more: the first barrier behind these
+  volatile int* abort_flag;
+  int* err;
+  uint32_t *tmem_slot, tmem, rank;
+  int warp, lane, tiles, first, step;
+
+  __device__ __forceinline__ PairLoop(const TcFp8Args& args, uint8_t* raw) : p(args) {
+    smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    tmem_slot = (uint32_t*)(smem + S::OFF_BAR);
+    abort_flag = (volatile int*)(tmem_slot + 1);
+    full = (uint64_t*)(tmem_slot + 2);
+    empty = full + S::STAGES, sf_full = empty + S::STAGES, sf_empty = sf_full + SF_RING;
+    acc_full = sf_empty + SF_RING, acc_free = acc_full + S::ACC, more = acc_free + S::ACC;
+    err = p.err ? p.err : &g_fp8_wait_error;
+    warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    rank = cta_rank();
+    tiles = p.m_tiles * p.n_tiles, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  }
+  // one thread; the kernel's own barriers come with it
+  __device__ __forceinline__ void init_barriers() {
+    for (int i = 0; i < S::STAGES; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
+    for (int i = 0; i < SF_RING; i++) mbar_init(sf_full + i, rank == 0 ? 2 : 1), mbar_init(sf_empty + i, 1);
+    for (int i = 0; i < S::ACC; i++) mbar_init(acc_full + i, 1), mbar_init(acc_free + i, 2 * S::EPI);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __device__ __forceinline__ void begin() {
+    if (warp == 0) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    tmem = *tmem_slot;
+  }
+  __device__ __forceinline__ void end() {
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 0) {
+      tc_fence_after();
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+  }
+
+  __device__ __forceinline__ void loads(const CUtensorMap* xmap, const CUtensorMap* wmap) {
+    const bool lead = elect_one();
+    uint32_t it = 0, s = 0, ph = 1;  // ph: of the wait for the stage's last use
+    bool ok = true;
+    for (int t = first; ok && t < tiles; t += step) {
+      int mt, nt;
+      tile_at(p, t, &mt, &nt);
+      const int m0 = mt * 2 * TM + (int)rank * TM, n0 = nt * S::N + (int)rank * (S::N / 2);
+      for (int b = 0; b < p.kb; b++, it++) {
+        if (it >= S::STAGES && !warp_wait(empty + s, ph, abort_flag, err)) {
+          ok = false;
+          break;
+        }
+        if (lead) {
+          if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * (S::A_BYTES + S::B_BYTES));
+          const uint32_t bar = map_rank(full + s, 0);
+          tma_load_2d_pair(smem + s * S::A_BYTES, xmap, b * 128, m0, bar);
+          tma_load_2d_pair(smem + S::OFF_B + s * S::B_BYTES, wmap, b * 128, n0, bar);
+        }
+        if (++s == S::STAGES) s = 0, ph ^= 1;
+      }
+    }
+    // After an expired wait, loads still in flight land before the shared memory goes: the first CTA sees them
+    // complete, the second, whose loads complete there, waits far longer than a load takes.
+    if (!ok) {
+      if (rank == 0) {
+        for (uint32_t i = it > S::STAGES ? it - S::STAGES : 0; i < it; i++)
+          mbar_drain(full + i % S::STAGES, (i / S::STAGES) & 1);
+      } else {
+        pause_1ms();
+      }
+    }
+  }
+
+  // The whole warp runs this loop, so that its control flow and addresses stay uniform, and one elected lane issues.
+  // What it does for each block of K (a wait, four MMAs, a commit) has to take less than the block's 512 MMA cycles:
+  // with one divergent lane it took 870.
+  __device__ __forceinline__ void mmas() {
+    const bool lead = elect_one();
+    const uint64_t da0 = sdesc_sw128(smem_u32(smem)), db0 = sdesc_sw128(smem_u32(smem + S::OFF_B));
+    const uint64_t dsf0 = sdesc(smem_u32(smem + S::OFF_SF), 128, 128);
+    MmaFeed f{full, sf_full, S::STAGES, abort_flag, err};
+    uint32_t tile_n = 0;
+    bool ok = true;
+    for (int t = first; ok && t < tiles; t += step, tile_n++) {
+      const uint32_t bar = tile_n % S::ACC, use = tile_n / S::ACC;
+      if (use > 0 && !warp_wait_cluster(acc_free + bar, (use - 1) & 1, abort_flag, err)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + (tile_n & 1) * S::D1;
+      for (int b0 = 0; ok && b0 < p.kb; b0 += 4) {
+        ok = f.scales();
+        if (!ok) break;
+        const uint32_t sfa = tmem + S::SF_COL + f.slot * S::SF_COLS;
+        if (lead) {
+          const uint64_t dsf = dsf0 + f.slot * (S::SF_BYTES >> 4);
+#pragma unroll
+          for (int i = 0; i < 1 + S::NB; i++) tmem_cp_scales_pair(sfa + 4 * i, dsf + (512 >> 4) * i);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          if (b0 + j >= p.kb) break;
+          ok = f.stage();
+          if (!ok) break;
+          if (lead) {
+            const uint64_t da = da0 + f.s * (S::A_BYTES >> 4), db = db0 + f.s * (S::B_BYTES >> 4);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+              mma_mxf8_pair(d, da + 2 * k, db + 2 * k, idesc_mxf8(2 * TM, S::N, j), sfa, sfa + 4, j > 0 || k > 0 || b0 > 0);
+            mma_commit_pair(empty + f.s);
+          }
+          f.next_stage();
+        }
+        if (ok && lead) mma_commit_pair(sf_empty + f.slot);
+        f.next_scales();
+      }
+      if (ok && lead) mma_commit_pair(acc_full + bar);
+    }
+    if (*abort_flag && f.any) mbar_drain(empty + f.last, f.last_ph);  // MMAs in flight end before their operands and TMEM go
+  }
+
+  __device__ __forceinline__ void scales() {
+    ScaleFeed<SF_RING, S::N> feed{p.a, smem_u32(smem + S::OFF_SF), sf_full, sf_empty, abort_flag, err, lane};
+    feed.run(first, step, tiles, 0, p.kb, [&](int t, long* m0, long* n0) {
+      int mt, nt;
+      tile_at(p, t, &mt, &nt);
+      *m0 = (long)mt * 2 * TM + rank * TM, *n0 = (long)nt * S::N;
+    });
+  }
+  // what the control warps do
+  __device__ __forceinline__ void control(const CUtensorMap* xmap, const CUtensorMap* wmap) {
+    if (warp == 0)
+      loads(xmap, wmap);
+    else if (warp == 2)
+      scales();
+    else if (rank == 0)
+      mmas();
+    else if (first < tiles)
+      forward_scales<SF_RING>((long)((tiles - first + step - 1) / step) * ((p.kb + 3) / 4), sf_full, lane, abort_flag, err);
+  }
+};
+
+// The epilogue: COLS columns of one row a thread.
 template <int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<OUT>::THREADS, 1)
     fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
                            const __grid_constant__ CUtensorMap ymap, const __grid_constant__ TcFp8Args p) {
   using S = PairShape<OUT>;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint64_t* full = (uint64_t*)(smem + S::OFF_BAR);
-  uint64_t *empty = full + S::STAGES, *sf_full = empty + S::STAGES, *sf_empty = sf_full + SF_RING;
-  uint64_t *acc_full = sf_empty + SF_RING, *acc_free = acc_full + 1;
-  uint64_t *max_in = acc_free + 1, *box_in = max_in + S::BOXES;  // e4m3: of the two warps of a box
-  uint32_t* tmem_slot = (uint32_t*)(box_in + S::BOXES);
-  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cta_rank();
-  const Fp8Linear& a = p.a;
-  int* err = p.err ? p.err : &g_fp8_wait_error;
+  PairLoop<S> loop(p, smem_raw);
+  uint8_t* smem = loop.smem;
+  uint64_t *max_in = loop.more, *box_in = max_in + S::BOXES;  // e4m3: of the two warps of a box
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S::STAGES; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
-    for (int i = 0; i < SF_RING; i++) mbar_init(sf_full + i, rank == 0 ? 2 : 1), mbar_init(sf_empty + i, 1);
-    mbar_init(acc_full, 1);
-    mbar_init(acc_free, 2 * S::EPI);
     if (S::Q)
       for (int i = 0; i < S::BOXES; i++) mbar_init(max_in + i, 2), mbar_init(box_in + i, 2);
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    loop.init_barriers();
   }
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-  }
-  tc_fence_before();
-  __syncthreads();
-  cluster_sync();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const int tiles = p.m_tiles * p.n_tiles, kb = p.kb;
-  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
-
-  if (warp == 0) {
-    {
-      const bool lead = elect_one();
-      uint32_t it = 0, s = 0, ph = 1;  // ph: of the wait for the stage's last use
-      bool ok = true;
-      for (int t = first; ok && t < tiles; t += step) {
-        int mt, nt;
-        tile_at(p, t, &mt, &nt);
-        const int m0 = mt * 2 * TM + (int)rank * TM, n0 = nt * TN + (int)rank * (TN / 2);
-        for (int b = 0; b < kb; b++, it++) {
-          if (it >= S::STAGES && !warp_wait(empty + s, ph, abort_flag, err)) {
-            ok = false;
-            break;
-          }
-          if (lead) {
-            if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * (S::A_BYTES + S::B_BYTES));
-            const uint32_t bar = map_rank(full + s, 0);
-            tma_load_2d_pair(smem + s * S::A_BYTES, &xmap, b * 128, m0, bar);
-            tma_load_2d_pair(smem + S::OFF_B + s * S::B_BYTES, &wmap, b * 128, n0, bar);
-          }
-          if (++s == S::STAGES) s = 0, ph ^= 1;
-        }
-      }
-      // After an expired wait, loads still in flight land before the shared memory goes: the first CTA sees them
-      // complete, the second, whose loads complete there, waits far longer than a load takes.
-      if (!ok) {
-        if (rank == 0) {
-          for (uint32_t i = it > S::STAGES ? it - S::STAGES : 0; i < it; i++)
-            mbar_drain(full + i % S::STAGES, (i / S::STAGES) & 1);
-        } else {
-          const unsigned long long t0 = tc_now();
-          while (tc_now() - t0 < 1000000ull) __nanosleep(1000);
-        }
-      }
-    }
-  } else if (warp == 1) {
-    if (rank == 0) {
-      // The whole warp runs this loop, so that its control flow and addresses stay uniform, and one elected lane
-      // issues. What the loop does for each block of K (a wait, four MMAs, a commit) has to take less than the
-      // block's 512 MMA cycles: with one divergent lane it took 870.
-      const bool lead = elect_one();
-      const uint64_t da0 = sdesc_sw128(smem_u32(smem)), db0 = sdesc_sw128(smem_u32(smem + S::OFF_B));
-      const uint64_t dsf0 = sdesc(smem_u32(smem + S::OFF_SF), 128, 128);
-      MmaFeed f{full, sf_full, S::STAGES, abort_flag, err};
-      uint32_t tile_n = 0;
-      bool ok = true;
-      for (int t = first; ok && t < tiles; t += step, tile_n++) {
-        if (tile_n > 0 && !warp_wait_cluster(acc_free, (tile_n - 1) & 1, abort_flag, err)) break;
-        tc_fence_after();
-        const uint32_t d = tmem + (tile_n & 1) * S::D1;
-        for (int b0 = 0; ok && b0 < kb; b0 += 4) {
-          ok = f.scales();
-          if (!ok) break;
-          const uint32_t sfa = tmem + S::SF_COL + f.slot * S::SF_COLS;
-          if (lead) {
-            const uint64_t dsf = dsf0 + f.slot * (S::SF_BYTES >> 4);
-            tmem_cp_scales_pair(sfa, dsf);
-            tmem_cp_scales_pair(sfa + 4, dsf + (512 >> 4));
-            tmem_cp_scales_pair(sfa + 8, dsf + (1024 >> 4));
-          }
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            if (b0 + j >= kb) break;
-            ok = f.stage();
-            if (!ok) break;
-            if (lead) {
-              const uint64_t da = da0 + f.s * (S::A_BYTES >> 4), db = db0 + f.s * (S::B_BYTES >> 4);
-#pragma unroll
-              for (int k = 0; k < 4; k++)
-                mma_mxf8_pair(d, da + 2 * k, db + 2 * k, idesc_mxf8(2 * TM, TN, j), sfa, sfa + 4, j > 0 || k > 0 || b0 > 0);
-              mma_commit_pair(empty + f.s);
-            }
-            f.next_stage();
-          }
-          if (ok && lead) mma_commit_pair(sf_empty + f.slot);
-          f.next_scales();
-        }
-        if (ok && lead) mma_commit_pair(acc_full);
-      }
-      if (*abort_flag && f.any) mbar_drain(empty + f.last, f.last_ph);  // MMAs in flight end before their operands and TMEM go
-    } else if (first < tiles) {
-      forward_scales<SF_RING>((long)((tiles - first + step - 1) / step) * ((kb + 3) / 4), sf_full, lane, abort_flag, err);
-    }
-  } else if (warp == 2) {
-    ScaleFeed<SF_RING, TN> feed{a, smem_u32(smem + S::OFF_SF), sf_full, sf_empty, abort_flag, err, lane};
-    feed.run(first, step, tiles, 0, kb, [&](int t, long* m0, long* n0) {
-      int mt, nt;
-      tile_at(p, t, &mt, &nt);
-      *m0 = (long)mt * 2 * TM + rank * TM, *n0 = (long)nt * TN;
-    });
+  loop.begin();
+  const Fp8Linear& a = p.a;
+  const int warp = loop.warp, lane = loop.lane, tiles = loop.tiles, first = loop.first, step = loop.step;
+  const uint32_t rank = loop.rank, tmem = loop.tmem;
+  uint64_t *acc_full = loop.acc_full, *acc_free = loop.acc_free;
+  volatile int* abort_flag = loop.abort_flag;
+  int* err = loop.err;
+  if (warp < CTRL_WARPS) {
+    loop.control(&xmap, &wmap);
   } else {
     const int ew = warp - CTRL_WARPS, cg = ew >> 2, q4 = warp & 3;  // COLS columns; the TMEM lane quarter a warp reaches
     float* bias_s = (float*)(smem + S::OFF_BIAS) + ew * S::COLS;
@@ -690,14 +745,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<OUT>::THRE
     }
     if (lane == 0) bulk_wait_all();
   }
-  __syncwarp();
-  tc_fence_before();
-  __syncthreads();
-  cluster_sync();
-  if (warp == 0) {
-    tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
-  }
+  loop.end();
 }
 
 // ---- large layers with a residual: two whole accumulators and a box for every column
@@ -715,7 +763,8 @@ struct TileShape {
   static constexpr int STAGES = OUT == FP8_F32 ? 4 : 5;
   static constexpr int A_BYTES = TM * 128, B_BYTES = N / 2 * 128;
   static constexpr int NB = (N + 127) / 128;
-  static constexpr int SF_BYTES = 512 * (1 + NB), SF_COLS = 4 * (1 + NB), SF_COL = 2 * N;
+  static constexpr int SF_BYTES = 512 * (1 + NB), SF_COLS = 4 * (1 + NB);
+  static constexpr int D1 = N, ACC = 2, SF_COL = 2 * N;  // two accumulators, a barrier each way for each
   static constexpr int OFF_B = STAGES * A_BYTES, OFF_BOX = OFF_B + STAGES * B_BYTES;
   static constexpr int OFF_SF = OFF_BOX + EPI * NBOX * BOX, OFF_BIAS = OFF_SF + SF_RING * SF_BYTES;
   static constexpr int OFF_BAR = OFF_BIAS + EPI * 64 * 4;
@@ -731,124 +780,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TileShape<OUT>::THRE
                            const __grid_constant__ TcFp8Args p) {
   using S = TileShape<OUT>;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint64_t* full = (uint64_t*)(smem + S::OFF_BAR);
-  uint64_t *empty = full + S::STAGES, *sf_full = empty + S::STAGES, *sf_empty = sf_full + SF_RING;
-  uint64_t *acc_full = sf_empty + SF_RING, *acc_free = acc_full + 2;
-  uint64_t* res_full = acc_free + 2;  // [EPI][NBOX]
-  uint32_t* tmem_slot = (uint32_t*)(res_full + S::EPI * S::NBOX);
-  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cta_rank();
-  const Fp8Linear& a = p.a;
-  int* err = p.err ? p.err : &g_fp8_wait_error;
+  PairLoop<S> loop(p, smem_raw);
+  uint8_t* smem = loop.smem;
+  uint64_t* res_full = loop.more;  // [EPI][NBOX]
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S::STAGES; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
-    for (int i = 0; i < SF_RING; i++) mbar_init(sf_full + i, rank == 0 ? 2 : 1), mbar_init(sf_empty + i, 1);
-    for (int i = 0; i < 2; i++) mbar_init(acc_full + i, 1), mbar_init(acc_free + i, 2 * S::EPI);
     for (int i = 0; i < S::EPI * S::NBOX; i++) mbar_init(res_full + i, 1);
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    loop.init_barriers();
   }
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-  }
-  tc_fence_before();
-  __syncthreads();
-  cluster_sync();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const int tiles = p.m_tiles * p.n_tiles, kb = p.kb;
-  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
-
-  if (warp == 0) {
-    {
-      const bool lead = elect_one();
-      uint32_t it = 0, s = 0, ph = 1;
-      bool ok = true;
-      for (int t = first; ok && t < tiles; t += step) {
-        int mt, nt;
-        tile_at(p, t, &mt, &nt);
-        const int m0 = mt * 2 * TM + (int)rank * TM, n0 = nt * S::N + (int)rank * (S::N / 2);
-        for (int b = 0; b < kb; b++, it++) {
-          if (it >= S::STAGES && !warp_wait(empty + s, ph, abort_flag, err)) {
-            ok = false;
-            break;
-          }
-          if (lead) {
-            if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * (S::A_BYTES + S::B_BYTES));
-            const uint32_t bar = map_rank(full + s, 0);
-            tma_load_2d_pair(smem + s * S::A_BYTES, &xmap, b * 128, m0, bar);
-            tma_load_2d_pair(smem + S::OFF_B + s * S::B_BYTES, &wmap, b * 128, n0, bar);
-          }
-          if (++s == S::STAGES) s = 0, ph ^= 1;
-        }
-      }
-      // After an expired wait, loads still in flight land before the shared memory goes: the first CTA sees them
-      // complete, the second, whose loads complete there, waits far longer than a load takes.
-      if (!ok) {
-        if (rank == 0) {
-          for (uint32_t i = it > S::STAGES ? it - S::STAGES : 0; i < it; i++)
-            mbar_drain(full + i % S::STAGES, (i / S::STAGES) & 1);
-        } else {
-          const unsigned long long t0 = tc_now();
-          while (tc_now() - t0 < 1000000ull) __nanosleep(1000);
-        }
-      }
-    }
-  } else if (warp == 1) {
-    if (rank == 0) {
-      const bool lead = elect_one();
-      const uint64_t da0 = sdesc_sw128(smem_u32(smem)), db0 = sdesc_sw128(smem_u32(smem + S::OFF_B));
-      const uint64_t dsf0 = sdesc(smem_u32(smem + S::OFF_SF), 128, 128);
-      MmaFeed f{full, sf_full, S::STAGES, abort_flag, err};
-      uint32_t tile_n = 0;
-      bool ok = true;
-      for (int t = first; ok && t < tiles; t += step, tile_n++) {
-        const uint32_t buf = tile_n & 1;
-        if (tile_n > 1 && !warp_wait_cluster(acc_free + buf, ((tile_n >> 1) + 1) & 1, abort_flag, err)) break;
-        tc_fence_after();
-        const uint32_t d = tmem + buf * S::N;
-        for (int b0 = 0; ok && b0 < kb; b0 += 4) {
-          ok = f.scales();
-          if (!ok) break;
-          const uint32_t sfa = tmem + S::SF_COL + f.slot * S::SF_COLS;
-          if (lead) {
-            const uint64_t dsf = dsf0 + f.slot * (S::SF_BYTES >> 4);
-#pragma unroll
-            for (int i = 0; i < 1 + S::NB; i++) tmem_cp_scales_pair(sfa + 4 * i, dsf + (512 >> 4) * i);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            if (b0 + j >= kb) break;
-            ok = f.stage();
-            if (!ok) break;
-            if (lead) {
-              const uint64_t da = da0 + f.s * (S::A_BYTES >> 4), db = db0 + f.s * (S::B_BYTES >> 4);
-#pragma unroll
-              for (int k = 0; k < 4; k++)
-                mma_mxf8_pair(d, da + 2 * k, db + 2 * k, idesc_mxf8(2 * TM, S::N, j), sfa, sfa + 4, j > 0 || k > 0 || b0 > 0);
-              mma_commit_pair(empty + f.s);
-            }
-            f.next_stage();
-          }
-          if (ok && lead) mma_commit_pair(sf_empty + f.slot);
-          f.next_scales();
-        }
-        if (ok && lead) mma_commit_pair(acc_full + buf);
-      }
-      if (*abort_flag && f.any) mbar_drain(empty + f.last, f.last_ph);  // MMAs in flight end before their operands and TMEM go
-    } else if (first < tiles) {
-      forward_scales<SF_RING>((long)((tiles - first + step - 1) / step) * ((kb + 3) / 4), sf_full, lane, abort_flag, err);
-    }
-  } else if (warp == 2) {
-    ScaleFeed<SF_RING, S::N> feed{a, smem_u32(smem + S::OFF_SF), sf_full, sf_empty, abort_flag, err, lane};
-    feed.run(first, step, tiles, 0, kb, [&](int t, long* m0, long* n0) {
-      int mt, nt;
-      tile_at(p, t, &mt, &nt);
-      *m0 = (long)mt * 2 * TM + rank * TM, *n0 = (long)nt * S::N;
-    });
+  loop.begin();
+  const Fp8Linear& a = p.a;
+  const int warp = loop.warp, lane = loop.lane, tiles = loop.tiles, first = loop.first, step = loop.step;
+  const uint32_t rank = loop.rank, tmem = loop.tmem;
+  uint64_t *acc_full = loop.acc_full, *acc_free = loop.acc_free;
+  volatile int* abort_flag = loop.abort_flag;
+  int* err = loop.err;
+  if (warp < CTRL_WARPS) {
+    loop.control(&xmap, &wmap);
   } else {
     const int ew = warp - CTRL_WARPS, cg = ew >> 2, q4 = warp & 3;  // 64 columns; the TMEM lane quarter a warp reaches
     float* bias_s = (float*)(smem + S::OFF_BIAS) + ew * 64;
@@ -871,8 +818,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TileShape<OUT>::THRE
       // boxes with columns, and how many of them go by TMA
       const int live = r0 < a.m && c0 < a.n ? (int)min((long)S::NBOX, (a.n - c0 + S::BC - 1) / S::BC) : 0;
       const int boxes = !p.tma_y || live == 0 ? 0 : (p.tma_edge ? live : (int)min((long)live, (a.n - c0) / S::BC));
-      if (lane == 0) bulk_wait_all_read();  // the boxes are free once the last tile's stores have read them
-      if (lane == 0) {                      // the residual comes while the tile's MMAs run
+      if (lane == 0) {  // the residual comes while the tile's MMAs run
+        bulk_wait_all_read();  // (the boxes are free once the last tile's stores have read them)
         for (int i = 0; i < boxes; i++) {
           mbar_arrive_expect_tx(res_full + ew * S::NBOX + i, BOX);
           tma_load_2d(box + i * BOX, &rmap, (int)c0 + i * S::BC, (int)r0, res_full + ew * S::NBOX + i);
@@ -959,21 +906,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TileShape<OUT>::THRE
       tc_fence_before();
     }
     if (lane == 0) {
-      if (!ok) {  // residual boxes still in flight land before the shared memory goes
-        const unsigned long long w0 = tc_now();
-        while (tc_now() - w0 < 1000000ull) __nanosleep(1000);
-      }
+      if (!ok) pause_1ms();  // residual boxes still in flight land before the shared memory goes
       bulk_wait_all();
     }
   }
-  __syncwarp();
-  tc_fence_before();
-  __syncthreads();
-  cluster_sync();
-  if (warp == 0) {
-    tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
-  }
+  loop.end();
 }
 
 // ---- small layers: one CTA per tile of 128 rows x NT columns and share of K
