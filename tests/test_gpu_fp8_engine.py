@@ -93,14 +93,15 @@ def test_fp8_encoder_rows(eng8, cases, oracle, oracle8):
 def test_fp8_durations(eng8, cases, oracle, oracle8):
     """Durations against the 8-bit oracle's (within a frame), and how many differ from the plain oracle's."""
     outs = eng8.forward_batch(cases)
-    n = diff = 0
+    n = diff = most = 0
     for it, o in zip(cases, outs):
         r8 = oracle8.forward(it.ids, it.ref_s, 1.0, seed=it.noise.seed, want=("dur_q",))
         r = oracle.forward(it.ids, it.ref_s, 1.0, seed=it.noise.seed, want=("dur_q",))
         assert np.abs(o.pred_dur - r8["dur"]).max() <= 1
         assert o.audio.shape[0] == 600 * int(o.pred_dur.sum()) and np.isfinite(o.audio).all()
         n, diff = n + len(r["dur"]), diff + int((o.pred_dur != r["dur"]).sum())
-    print(f"{diff} of {n} durations differ from the plain oracle's")
+        most = max(most, int(np.abs(o.pred_dur - r["dur"]).max()))
+    print(f"{diff} of {n} durations differ from the plain oracle's, by at most {most}")
 
 
 def test_fp8_twice_the_same_and_gap_rows_stay_out(kk, eng8, cases):
