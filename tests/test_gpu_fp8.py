@@ -467,3 +467,61 @@ def test_calls_of_several_host_threads_at_once(kk):
         t.join()
     assert not bad
     fp8.check()
+
+
+@pytest.mark.parametrize("m, n, k", [(5, 130, 200), (700, 640, 520), (4800, 1000, 300)])
+def test_what_lies_behind_a_row_is_not_read(kk, m, n, k):
+    """Values behind column k that are NaN, and scales behind the last block that are NaN, change nothing."""
+    rng = np.random.default_rng(13)
+    fp8 = kk.fp8
+    xq, wq, _, _ = make(rng, m, n, k, fp8)
+    want = fp8.linear(xq, wq)
+
+    def within(q):
+        rows, kb = q.shape[0], q.exps.shape[1]
+        ldv, lde = -(-k // 16) * 16 + 32, -(-kb // 4) * 4 + 4
+        v = torch.full((rows + 3, ldv), 0x7F, device="cuda", dtype=torch.uint8)
+        e = torch.full((q.exps.shape[0] + 3, lde), 0xFF, device="cuda", dtype=torch.uint8)
+        v[:rows, :k] = q.values.view(torch.uint8)
+        e[: q.exps.shape[0], :kb] = q.exps
+        return fp8.Fp8Tensor(v.view(E4M3)[:rows, :k], e[: q.exps.shape[0], :kb], q.block_rows)
+
+    x2, w2 = within(xq), within(wq)
+    assert torch.equal(fp8.linear(x2, w2), want)
+    assert torch.equal(fp8.linear(x2, w2, out_dtype=torch.bfloat16), fp8.linear(xq, wq, out_dtype=torch.bfloat16))
+    a, b = fp8.linear(x2, w2, out_dtype=E4M3), fp8.linear(xq, wq, out_dtype=E4M3)
+    assert np.array_equal(bits(a.values), bits(b.values)) and torch.equal(a.exps, b.exps)
+    assert torch.equal(fp8.dequantize(x2), fp8.dequantize(xq)) and torch.equal(fp8.dequantize(w2), fp8.dequantize(wq))
+
+
+def test_offsets_past_32_bits(kk):
+    """Rows that begin past 2^31 elements and 2^32 bytes: the last ones equal those of a small call."""
+    fp8 = kk.fp8
+    torch.manual_seed(14)
+    # Two orders of adding 128 products, whose magnitudes add up to 130 at most here, differ by 2 * 128 * 2^-24 * 130.
+    tol = 2.0 * 128 * 2.0 ** -24 * 130
+    rows, k = 20000, 120000  # 2.4e9 elements
+    x = torch.zeros(rows, k, device="cuda", dtype=torch.bfloat16)
+    x[-3:] = torch.randn(3, k, device="cuda")
+    q = fp8.quantize(x)
+    small = fp8.quantize(x[-3:].clone())
+    assert torch.equal(q[rows - 3:].values.view(torch.uint8), small.values.view(torch.uint8))
+    assert torch.equal(q[rows - 3:].exps, small.exps)
+    x.fill_(1.0)
+    fp8.dequantize(q, torch.bfloat16, out=x)
+    assert torch.equal(x[-3:], fp8.dequantize(small, torch.bfloat16)) and (x[:-3] == 0).all()
+    del x, q
+    m, n = 300000, 8192  # 2.5e9 results
+    xq = fp8.quantize(torch.randn(m, 128, device="cuda"))
+    wq = fp8.quantize(torch.randn(n, 128, device="cuda"), block_rows=128)
+    res = torch.zeros(m, n, device="cuda")
+    res[-5:] = 1.0
+    want = fp8.linear(xq[m - 5:], wq)
+    y = fp8.linear(xq, wq)
+    assert torch.allclose(y[-5:], want, rtol=0, atol=tol)
+    fp8.linear(xq, wq, residual=res, out=res)
+    assert torch.allclose(res[-5:], want + 1.0, rtol=0, atol=tol) and torch.allclose(res[:1000], y[:1000], rtol=0, atol=tol)
+    del res
+    h = fp8.linear(xq, wq, out_dtype=E4M3)
+    tail = fp8.dequantize(h[m - 5:])
+    assert ((tail - want).abs() <= 2.0 ** -4 * want.abs() + want.abs().amax() * 2.0 ** -10 / 224 + tol).all()
