@@ -382,7 +382,9 @@ KK_API const char* kk_conv_selftest_error(void);
  * All pointers are device pointers of device `cuda_ordinal`; `stream` is a cudaStream_t of that device
  * (NULL: its legacy default stream). The calls only enqueue work (they may be captured into a graph),
  * allocate nothing, keep nothing, and may run at once on several streams and host threads. The caller's
- * current device is left as it was. rows / m = 0 is a no-op. Rows, columns and blocks stay below 2^31.
+ * current device is left as it was. rows / m = 0 is a no-op. Rows and blocks stay below 2^31, columns below 2^30.
+ * What a call writes may not overlap what it reads, but for a residual that is the result itself: such calls are
+ * refused, as are those whose rows of two pitches lie in one range of addresses.
  */
 typedef enum { KK_FP8_F32 = 0, KK_FP8_BF16 = 1, KK_FP8_E4M3 = 2 } kk_fp8_type;
 typedef enum { KK_FP8_ACT_NONE = 0, KK_FP8_ACT_GELU = 1 /* gelu_new, kernels/kokoro.cu:84-90 */ } kk_fp8_act;
@@ -400,7 +402,7 @@ KK_API kk_status kk_fp8_dequantize(int cuda_ordinal, void* stream, const uint8_t
  * ldy elements apart, residual of the same type (ldr elements apart; NULL: none; it may be y itself, or not
  * overlap it).
  * y_type KK_FP8_E4M3: y / ldy and y_exps / ldye are a store (block_rows 1) that the result is quantised
- * into, without a residual. y may not overlap x or w.
+ * into, without a residual. y may not overlap x, w or bias.
  */
 KK_API kk_status kk_fp8_linear(int cuda_ordinal, void* stream, int64_t m, int64_t n, int64_t k, const uint8_t* x,
                                int64_t ldx, const uint8_t* x_exps, int64_t ldxe, const uint8_t* w, int64_t ldw,
@@ -408,8 +410,8 @@ KK_API kk_status kk_fp8_linear(int cuda_ordinal, void* stream, int64_t m, int64_
                                int64_t ldr, int y_type, void* y, int64_t ldy, uint8_t* y_exps, int64_t ldye);
 /*
  * Waits for the stream and reports (KK_ERR_TIMEOUT, once) whether a bounded in-kernel wait of a
- * kk_fp8_linear on this device gave up since the last check; its results are then not valid. Not inside
- * a capture.
+ * kk_fp8_linear on this device gave up since the last check; its results are then not valid. Refused
+ * (KK_ERR_CUDA) while the stream is being captured.
  */
 KK_API kk_status kk_fp8_check(int cuda_ordinal, void* stream);
 /* Message of the last kk_fp8_* failure on this thread. */

@@ -41,7 +41,7 @@ cudaError_t launch_fp8_dequantize(Fp8Store q, long rows, long k, int block_rows,
                                   cudaStream_t st);
 // err receives 2 if a bounded pipeline wait expires; null: the device's own flag, for fp8_take_wait_error
 cudaError_t launch_fp8_linear(const Fp8Linear& a, int* err, cudaStream_t st);
-// Waits for the stream; *flag = the current device's flag, which is cleared.
+// Waits for the stream (an error while it is being captured); *flag = the current device's flag, which is cleared.
 cudaError_t fp8_take_wait_error(int* flag, cudaStream_t st);
 
 }  // namespace kk

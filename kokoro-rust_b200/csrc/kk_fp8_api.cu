@@ -68,6 +68,39 @@ const char* bad_extent(int64_t rows, int64_t k) {
   return nullptr;
 }
 
+// Rows of `width` bytes, `pitch` bytes apart.
+struct Span {
+  const void* p;
+  int64_t rows, width, pitch;
+};
+
+// Whether two spans share a byte. Columns of one buffer, rows of the same pitch, are told apart; spans of other pitches
+// count as sharing where their address ranges do.
+bool overlap(Span a, Span b) {
+  if (!a.p || !b.p) return false;
+  const uint64_t pa = (uint64_t)(uintptr_t)a.p, pb = (uint64_t)(uintptr_t)b.p;
+  const uint64_t ea = pa + (uint64_t)(a.rows - 1) * a.pitch + a.width, eb = pb + (uint64_t)(b.rows - 1) * b.pitch + b.width;
+  if (ea <= pb || eb <= pa) return false;
+  if (a.rows == 1) a.pitch = b.pitch;
+  if (b.rows == 1) b.pitch = a.pitch;
+  if (a.rows == 1 && b.rows == 1) return true;
+  if (a.pitch != b.pitch || a.width > a.pitch || b.width > b.pitch) return true;
+  if (pb < pa) return overlap(b, a);
+  // b begins r bytes into the pitch that a's row s begins: its rows meet a's row s or, round the corner, the next
+  const uint64_t s = (pb - pa) / (uint64_t)a.pitch, r = (pb - pa) % (uint64_t)a.pitch;
+  return (r < (uint64_t)a.width && s < (uint64_t)a.rows) ||
+         (r + b.width > (uint64_t)a.pitch && s + 1 < (uint64_t)a.rows);
+}
+
+Span value_span(const void* v, int64_t ldv, int64_t rows, int64_t k) { return {v, rows, k, ldv}; }
+Span exps_span(const void* e, int64_t lde, int64_t rows, int64_t k, int block_rows) {
+  return {e, (rows + block_rows - 1) / block_rows, (k + 127) / 128, lde};
+}
+Span row_span(const void* x, int type, int64_t ld, int64_t rows, int64_t k) {
+  const int64_t es = type == KK_FP8_F32 ? 4 : 2;
+  return {x, rows, k * es, ld * es};
+}
+
 // What a device ordinal is, looked up once: 1 compute capability 10.x, 2 another device, 3 none.
 int device_kind(int ordinal) {
   static std::atomic<int> cache[64];
@@ -119,6 +152,10 @@ kk_status kk_fp8_quantize(int cuda_ordinal, void* stream, const void* x, int typ
   if (rows == 0) return KK_OK;
   if (const char* m = bad_rows(x, type, k, ldx)) return fail(KK_ERR_INVALID_ARG, m);
   if (const char* m = bad_store(values, ldv, exps, lde, k)) return fail(KK_ERR_INVALID_ARG, m);
+  const Span xs = row_span(x, type, ldx, rows, k), vs = value_span(values, ldv, rows, k);
+  const Span es = exps_span(exps, lde, rows, k, block_rows);
+  if (overlap(xs, vs) || overlap(xs, es) || overlap(vs, es))
+    return fail(KK_ERR_INVALID_ARG, "the rows, the values and the exponents must not overlap");
   QuantArgs a{x, type, (long)rows, (long)k, (long)ldx, block_rows, {values, (long)ldv, exps, (long)lde}};
   return run(cuda_ordinal, "kk_fp8_quantize: ", [](const void* p, cudaStream_t st) {
     const QuantArgs& a = *(const QuantArgs*)p;
@@ -133,6 +170,9 @@ kk_status kk_fp8_dequantize(int cuda_ordinal, void* stream, const uint8_t* value
   if (rows == 0) return KK_OK;
   if (const char* m = bad_rows(y, type, k, ldy)) return fail(KK_ERR_INVALID_ARG, m);
   if (const char* m = bad_store(values, ldv, exps, lde, k)) return fail(KK_ERR_INVALID_ARG, m);
+  const Span ys = row_span(y, type, ldy, rows, k);
+  if (overlap(ys, value_span(values, ldv, rows, k)) || overlap(ys, exps_span(exps, lde, rows, k, block_rows)))
+    return fail(KK_ERR_INVALID_ARG, "the rows must not overlap the store");
   QuantArgs a{y, type, (long)rows, (long)k, (long)ldy, block_rows,
               {const_cast<uint8_t*>(values), (long)ldv, const_cast<uint8_t*>(exps), (long)lde}};
   return run(cuda_ordinal, "kk_fp8_dequantize: ", [](const void* p, cudaStream_t st) {
@@ -163,6 +203,16 @@ kk_status kk_fp8_linear(int cuda_ordinal, void* stream, int64_t m, int64_t n, in
     if (residual)
       if (const char* s = bad_rows(residual, y_type, n, ldr)) return fail(KK_ERR_INVALID_ARG, "residual: ", s);
   }
+  const bool q = y_type == KK_FP8_E4M3;
+  const Span ys = q ? value_span(y, ldy, m, n) : row_span(y, y_type, ldy, m, n);
+  const Span qs = q ? exps_span(y_exps, ldye, m, n, 1) : Span{nullptr, 0, 0, 0};
+  const Span in[5] = {value_span(x, ldx, m, k), exps_span(x_exps, ldxe, m, k, 1), value_span(w, ldw, n, k),
+                      exps_span(w_exps, ldwe, n, k, 128), Span{bias, 1, n * 4, n * 4}};
+  for (const Span& s : in)
+    if (overlap(ys, s) || overlap(qs, s)) return fail(KK_ERR_INVALID_ARG, "y must not overlap x, w or bias");
+  if (overlap(ys, qs)) return fail(KK_ERR_INVALID_ARG, "y: the values and the exponents must not overlap");
+  if (residual && !(residual == y && (ldr == ldy || m == 1)) && overlap(ys, row_span(residual, y_type, ldr, m, n)))
+    return fail(KK_ERR_INVALID_ARG, "residual must be y itself or not overlap it");
   struct Args {
     kk::Fp8Linear a;
   } g{};

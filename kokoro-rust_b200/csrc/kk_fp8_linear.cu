@@ -1379,7 +1379,10 @@ cudaError_t launch_fp8_linear(const Fp8Linear& a, int* err, cudaStream_t st) {
 
 cudaError_t fp8_take_wait_error(int* err, cudaStream_t st) {
   int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbolAsync(err, g_fp8_wait_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(st, &capture);
+  if (e == cudaSuccess && capture != cudaStreamCaptureStatusNone) e = cudaErrorStreamCaptureUnsupported;
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(err, g_fp8_wait_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   if (e == cudaSuccess && *err) {
     e = cudaMemcpyToSymbolAsync(g_fp8_wait_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);

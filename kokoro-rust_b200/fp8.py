@@ -88,6 +88,8 @@ class Fp8Tensor:
         self = cls.__new__(cls)
         # one allocation: the values, then the exponents; the views are made when they are asked for
         self._buf = torch.empty(rows * ldv + -(-rows // block_rows) * lde, dtype=torch.uint8, device=device)
+        if not self._buf.is_cuda:
+            _refuse("a store is held on a CUDA device")
         at = self._buf.data_ptr()
         self.shape, self.block_rows, self.device = torch.Size((rows, k)), block_rows, self._buf.device
         self._values = self._exps = None
@@ -164,8 +166,8 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
            out: Union[torch.Tensor, Fp8Tensor, None] = None) -> Union[torch.Tensor, Fp8Tensor]:
     """act(x w^T + bias) + residual: x [m, k] a store with block_rows 1, w [n, k] one with block_rows
     128, bias float32 [n], act None or "gelu" (the tanh form). The result is float32, bfloat16 (with a
-    residual of the same type, which may be ``out`` itself), or with float8_e4m3fn a store that the next
-    layer reads (without a residual)."""
+    residual of the same type, which may be ``out`` itself or not overlap it), or with float8_e4m3fn a store that the next
+    layer reads (without a residual). ``out`` may not overlap x, w or bias."""
     if not isinstance(x, Fp8Tensor) or x.block_rows != 1:
         _refuse("x: a store with block_rows 1 is wanted")
     if not isinstance(w, Fp8Tensor) or w.block_rows != 128:
@@ -183,7 +185,7 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
         _one_device(dev, w.device)
     b = None
     if bias is not None:
-        if bias.dtype is not _F32 or bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
+        if not isinstance(bias, torch.Tensor) or bias.dtype is not _F32 or bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
             _refuse(f"bias: adjacent float32 [{n}] is wanted")
         if bias.requires_grad and torch.is_grad_enabled():
             _refuse("bias: the 8-bit operators have no gradient")
@@ -223,7 +225,8 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
 
 def check(device=None) -> None:
     """Waits for the current stream and raises if a bounded in-kernel wait of a linear layer on this
-    device gave up since the last check (its results are then not valid)."""
+    device gave up since the last check (its results are then not valid). Refused while the stream is
+    being captured."""
     dev = torch.device("cuda") if device is None else torch.device(device)
     idx = torch.cuda.current_device() if dev.index is None else dev.index
     _run(load_library().kk_fp8_check(idx, _stream(idx)))

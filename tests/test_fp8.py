@@ -89,6 +89,60 @@ def test_linear_refusals(kk, kw, word):
     assert word in lib.kk_fp8_error().decode()
 
 
+def overlaps(a, b):
+    """Whether two lists of (address, rows, bytes of a row, pitch) share a byte, byte by byte."""
+    cells = lambda p, rows, width, pitch: {p + i * pitch + j for i in range(rows) for j in range(width)}
+    return bool(cells(*a) & cells(*b))
+
+
+def test_overlap_is_refused(kk):
+    """Residual and result in one buffer, a row pitch apart or columns of it, against their bytes counted out."""
+    lib, n, m, ld = kk.load_library(), 5, 3, 16
+    base = 1 << 20
+    far = dict(m=m, n=n, x=1 << 30, xe=1 << 31, w=1 << 32, we=1 << 33, y=base, ldy=ld, ldr=ld, dev=99)
+    seen = set()
+    for d in range(-70, 71):  # elements between the two
+        for yt, es in ((0, 4), (1, 2)):
+            want = d != 0 and overlaps((base, m, n * es, ld * es), (base + d * es, m, n * es, ld * es))
+            assert lib.kk_fp8_linear(*l_args(**far, yt=yt, res=base + d * es)) != kk.engine.KK_OK
+            assert ("residual must be" in lib.kk_fp8_error().decode()) == want, (d, yt)
+            seen.add(want)
+    assert seen == {True, False}
+    # another pitch, and the same address at another pitch
+    for kw in (dict(res=base, ldr=ld + 4), dict(res=base + 4 * n, ldr=8)):
+        assert lib.kk_fp8_linear(*l_args(**{**far, **kw})) == kk.engine.KK_ERR_INVALID_ARG
+        assert "residual must be" in lib.kk_fp8_error().decode()
+    # one row: only its bytes count
+    for d, want in ((0, False), (4 * n, False), (4, True)):
+        lib.kk_fp8_linear(*l_args(**{**far, "m": 1, "res": base + d, "ldr": n}))
+        assert ("residual must be" in lib.kk_fp8_error().decode()) == want
+
+
+@pytest.mark.parametrize("kw, word", [
+    (dict(y=1 << 30), "y must not"), (dict(y=1 << 31), "y must not"), (dict(y=(1 << 32) + 64), "y must not"),
+    (dict(y=1 << 33), "y must not"), (dict(y=1 << 34, bias=(1 << 34) + 1020), "y must not"),
+    (dict(yt=2, y=1 << 30, ldy=128, n=128, ye=1 << 35, ldye=4), "y must not"),
+    (dict(yt=2, y=1 << 34, ye=1 << 31, ldye=4), "y must not"), (dict(yt=2, y=1 << 34, ye=(1 << 34) + 252, ldye=4), "y: the values"),
+])
+def test_result_over_its_inputs_is_refused(kk, kw, word):
+    lib = kk.load_library()
+    a = dict(x=1 << 30, xe=1 << 31, w=1 << 32, we=1 << 33)
+    assert lib.kk_fp8_linear(*l_args(**{**a, **kw})) == kk.engine.KK_ERR_INVALID_ARG
+    assert word in lib.kk_fp8_error().decode()
+
+
+def test_quantize_over_its_input_is_refused(kk):
+    lib = kk.load_library()
+    x, v, e = 1 << 30, 1 << 31, 1 << 32
+    for kw in (dict(v=x), dict(e=x), dict(e=v), dict(v=x + 1024 * 3 + 1008)):
+        a = q_args(**{**dict(x=x, v=v, e=e), **kw})
+        assert lib.kk_fp8_quantize(*a) == kk.engine.KK_ERR_INVALID_ARG and "overlap" in lib.kk_fp8_error().decode()
+        if kw == dict(e=v):
+            continue  # (a store that overlaps itself is not read back)
+        a = [a[0], a[1], a[8], a[9], a[10], a[11], a[7], a[4], a[5], a[2], a[3], a[6]]
+        assert lib.kk_fp8_dequantize(*a) == kk.engine.KK_ERR_INVALID_ARG and "overlap" in lib.kk_fp8_error().decode()
+
+
 def test_no_rows_is_a_no_op(kk):
     lib = kk.load_library()
     assert lib.kk_fp8_quantize(*q_args(rows=0, x=None, v=None, e=None)) == kk.engine.KK_OK
@@ -119,6 +173,7 @@ def test_torch_refusals(kk):
     assert "adjacent" in refused(kk, fp8.quantize, torch.zeros(128, 4).t())
     assert "store is wanted" in refused(kk, fp8.dequantize, torch.zeros(4, 128))
     assert "block_rows 1" in refused(kk, fp8.linear, torch.zeros(4, 128), torch.zeros(4, 128))
+    assert "CUDA device" in refused(kk, fp8.Fp8Tensor.empty, 4, 128, device="cpu")
     v = torch.zeros(4, 128, dtype=torch.uint8).view(torch.float8_e4m3fn)
     assert "CUDA tensor" in refused(kk, fp8.Fp8Tensor, v, torch.zeros(4, 1, dtype=torch.uint8))
     assert "values" in refused(kk, fp8.Fp8Tensor, v.view(torch.uint8), torch.zeros(4, 1, dtype=torch.uint8))

@@ -525,3 +525,61 @@ def test_offsets_past_32_bits(kk):
     h = fp8.linear(xq, wq, out_dtype=E4M3)
     tail = fp8.dequantize(h[m - 5:])
     assert ((tail - want).abs() <= 2.0 ** -4 * want.abs() + want.abs().amax() * 2.0 ** -10 / 224 + tol).all()
+
+
+def test_check_inside_a_capture_is_refused(kk):
+    """...and leaves the capture as it was."""
+    fp8 = kk.fp8
+    rng = np.random.default_rng(15)
+    xq, wq, _, _ = make(rng, 200, 256, 256, fp8)
+    want = fp8.linear(xq, wq)
+    y = torch.zeros_like(want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        fp8.linear(xq, wq, out=y)
+        with pytest.raises(kk.KokoroError):
+            fp8.check()
+        fp8.linear(xq, wq, out=y)
+    g.replay()
+    fp8.check()
+    assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 1, (1 << 30) - 3), (3, 130, (1 << 28) + 200)])
+def test_longest_rows(kk, m, n, k):
+    """The whole sum of the longest rows waits for one CTA's (or one cluster's) loads."""
+    fp8 = kk.fp8
+    rng = np.random.default_rng(16)
+    at = np.unique(np.concatenate([rng.integers(0, k, 60), [0, k - 1]]))
+    xv, wv = fp8.Fp8Tensor.empty(m, k), fp8.Fp8Tensor.empty(n, k, 128)
+    for q in (xv, wv):
+        q._buf.zero_()
+        q.exps.fill_(127)
+    # powers of two at some columns: sums of at most 62 products 2^-4 .. 2^4 are exact in 24 bits
+    x = 2.0 ** rng.integers(-2, 3, (m, len(at))) * rng.choice((-1, 1), (m, len(at)))
+    w = 2.0 ** rng.integers(-2, 3, (n, len(at))) * rng.choice((-1, 1), (n, len(at)))
+    idx = torch.tensor(at, device="cuda")
+    xv.values.view(torch.uint8)[:, idx] = torch.tensor(x, device="cuda", dtype=torch.float32).to(E4M3).view(torch.uint8)
+    wv.values.view(torch.uint8)[:, idx] = torch.tensor(w, device="cuda", dtype=torch.float32).to(E4M3).view(torch.uint8)
+    y = fp8.linear(xv, wv)
+    fp8.check()
+    assert np.array_equal(y.cpu().numpy(), (x @ w.T).astype(np.float32))
+
+
+def test_most_rows(kk):
+    """2^31 - 1 rows, the most a call takes: the quantiser's, the read-back's and the layer's row indices."""
+    fp8 = kk.fp8
+    rows = (1 << 31) - 1
+    at = torch.tensor([0, 1, (1 << 30) - 1, 1 << 30, rows - 2, rows - 1], device="cuda")
+    vals = torch.tensor([1.0, -2.0, 3.0, 0.5, -7.0, 448.0], device="cuda")[:, None]
+    x = torch.zeros(rows, 1, device="cuda")
+    x[at] = vals
+    q = fp8.quantize(x)
+    x.fill_(5.0)
+    fp8.dequantize(q, out=x)
+    assert torch.equal(x[at], vals) and torch.count_nonzero(x).item() == len(at)
+    w = fp8.quantize(torch.full((1, 1), 2.0, device="cuda"), block_rows=128)
+    x.fill_(5.0)
+    fp8.linear(q, w, out=x)
+    fp8.check()
+    assert torch.equal(x[at], 2.0 * vals) and torch.count_nonzero(x).item() == len(at)
