@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <atomic>
+#include <type_traits>
 
 #include "kk_fp8.h"
 #include "kk_fp8_math.cuh"
@@ -318,38 +319,93 @@ struct PairShape {
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
-// 32 x 32 transpose over a warp: lane r's v[c] becomes lane c's v[r].
-__device__ __forceinline__ void warp_transpose(float* v, int lane) {
+// Rows at strides or offsets that TMA does not take: a warp's box of 32 rows (the thread's row at row_s, written as for
+// TMA) leaves row by row, its columns side by side, so that a store instruction still fills whole sectors. What it takes
+// is instructions, so whole boxes have loops of their own without a test in them: 33,104 x 768 -> 2306 bf16 69 us
+// (119 with a test at each row, 58 for 2304 by TMA), 768 -> 769 f32 44 (31 for 768), with a residual 69 (46; 224 with
+// the residual's rows loaded one after the other).
+//
+// 32 columns in 32 bits, one a lane: residual columns of the 32 rows from r0, all on their way at once (as raw bits:
+// widened here, they would be waited for here)...
+template <typename T>
+__device__ __forceinline__ void load_rows(const Fp8Linear& a, long r0, long c, int lane, uint32_t* res) {
+  using U = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+  const U* r = (const U*)a.res + r0 * a.ldr + c + lane;
+  const bool in = c + lane < a.n;
+  if (r0 + 32 <= a.m) {
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) {
-    const bool up = lane & s;
+    for (int j = 0; j < 32; j++, r += a.ldr) res[j] = in ? *r : 0;
+  } else {
 #pragma unroll
-    for (int i = 0; i < 32; i++) {
-      if (i & s) continue;
-      const float x = __shfl_xor_sync(0xFFFFFFFFu, up ? v[i] : v[i | s], s);
-      if (up)
-        v[i] = x;
-      else
-        v[i | s] = x;
-    }
+    for (int j = 0; j < 32; j++, r += a.ldr) res[j] = in && r0 + j < a.m ? *r : 0;
   }
 }
-
-// Rows at strides or offsets that TMA does not take: 32 columns from c of the 32 rows from r0 (lane = row). The
-// warp transposes the square and reads and writes a row's 32 columns together.
-template <typename T>
-__device__ __forceinline__ void store_any(const Fp8Linear& a, float* v, long r0, long c, int lane) {
-  T* y = (T*)a.y;
-  const T* res = (const T*)a.res;
-  warp_transpose(v, lane);
-  if (c + lane >= a.n) return;
+__device__ __forceinline__ void stage_rows(const float* v, uint32_t row_s, int lane) {
 #pragma unroll
-  for (int j = 0; j < 32; j++) {
-    if (r0 + j >= a.m) break;
-    float o = v[j];
-    if (res) o += (float)res[(r0 + j) * a.ldr + c + lane];
-    y[(r0 + j) * a.ldy + c + lane] = (T)o;
+  for (int q = 0; q < 8; q++)
+    sts_u4(row_s + ((q ^ (lane & 7)) << 4),
+           make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]),
+                      __float_as_uint(v[4 * q + 3])));
+}
+// ...and the staged rows, the residual added, into y.
+template <typename T, bool RES>
+__device__ __forceinline__ void store_rows(const Fp8Linear& a, const uint8_t* box, long r0, long c, int lane,
+                                           const uint32_t* res) {
+  __syncwarp();
+  T* y = (T*)a.y + r0 * a.ldy + c + lane;
+  auto row = [&](int j) {
+    float o = *reinterpret_cast<const float*>(box + j * 128 + ((((lane >> 2) ^ (j & 7)) << 4) | ((lane & 3) << 2)));
+    if (RES) o += __uint_as_float(sizeof(T) == 4 ? res[j] : res[j] << 16);
+    return (T)o;
+  };
+  if (c + lane < a.n) {
+    if (r0 + 32 <= a.m) {
+#pragma unroll
+      for (int j = 0; j < 32; j++, y += a.ldy) *y = row(j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; j++, y += a.ldy)
+        if (r0 + j < a.m) *y = row(j);
+    }
   }
+  __syncwarp();  // the box is free
+}
+// 64 bf16 columns: two a lane where the row is 4-byte aligned, else one in each half.
+__device__ __forceinline__ void store_rows_bf16(const Fp8Linear& a, const uint8_t* box, long r0, long c, int lane) {
+  __syncwarp();
+  uint16_t* const y = (uint16_t*)a.y + r0 * a.ldy + c;
+  const int in = (lane & 7) << 1, unit = lane >> 3;
+  auto pair = [&](int j) {
+    return *reinterpret_cast<const uint32_t*>(box + j * 128 + ((((lane >> 2) ^ (j & 7)) << 4) | ((lane & 3) << 2)));
+  };
+  auto one = [&](int j, int half) {
+    return *reinterpret_cast<const uint16_t*>(box + j * 128 + ((((unit + 4 * half) ^ (j & 7)) << 4) | in));
+  };
+  if (r0 + 32 <= a.m && c + 64 <= a.n) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {  // every other row: all of one alignment
+      uint16_t* r = y + i * a.ldy;
+      if (((uintptr_t)r & 3) == 0) {
+        r += 2 * lane;
+#pragma unroll
+        for (int j = i; j < 32; j += 2, r += 2 * a.ldy) *reinterpret_cast<uint32_t*>(r) = pair(j);
+      } else {
+        r += lane;
+#pragma unroll
+        for (int j = i; j < 32; j += 2, r += 2 * a.ldy) r[0] = one(j, 0), r[32] = one(j, 1);
+      }
+    }
+  } else {
+    uint16_t* r = y + lane;
+    const bool in0 = c + lane < a.n, in1 = c + lane + 32 < a.n;
+#pragma unroll 8
+    for (int j = 0; j < 32; j++, r += a.ldy) {
+      if (r0 + j >= a.m) break;
+      if (in0) r[0] = one(j, 0);
+      if (in1) r[32] = one(j, 1);
+    }
+  }
+  __syncwarp();
 }
 
 // The largest finite magnitude of a thread's 64 columns, as bits; *infinite: one of them is infinite.
@@ -696,10 +752,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<OUT>::THRE
             const long cx = c0 + c;            // the box's first column
             if (!live || cx >= a.n) continue;
             const bool tma = p.tma_y && (p.tma_edge || cx + BC <= a.n);
-            if (tma) {
-              if (lane == 0) bulk_wait_all_read();
-              __syncwarp();
-            }
+            if (lane == 0) bulk_wait_all_read();
+            __syncwarp();
 #pragma unroll
             for (int h = 0; h < BC / 32; h++) {
               float* w = v + BC * b + 32 * h;
@@ -708,21 +762,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<OUT>::THRE
 #pragma unroll
                 for (int j = 0; j < 32; j += 16) gelu_fast<16>(w + j);
               }
-              if (!tma) {
-                if (cx + 32 * h < a.n) {
-                  if constexpr (OUT == FP8_F32)
-                    store_any<float>(a, w, r0, cx + 32 * h, lane);
-                  else
-                    store_any<__nv_bfloat16>(a, w, r0, cx + 32 * h, lane);
-                }
-                continue;
-              }
               if constexpr (OUT == FP8_F32) {
-#pragma unroll
-                for (int q = 0; q < 8; q++)
-                  sts_u4(row_s + ((q ^ (lane & 7)) << 4),
-                         make_uint4(__float_as_uint(w[4 * q]), __float_as_uint(w[4 * q + 1]), __float_as_uint(w[4 * q + 2]),
-                                    __float_as_uint(w[4 * q + 3])));
+                stage_rows(w, row_s, lane);
               } else {
 #pragma unroll
                 for (int q = 0; q < 4; q++)
@@ -731,7 +772,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<OUT>::THRE
                                     bf16x2(w[8 * q + 4], w[8 * q + 5]), bf16x2(w[8 * q + 6], w[8 * q + 7])));
               }
             }
-            if (!tma) continue;
+            if (!tma) {
+              if constexpr (OUT == FP8_F32)
+                store_rows<float, false>(a, box, r0, cx, lane, nullptr);
+              else
+                store_rows_bf16(a, box, r0, cx, lane);
+              continue;
+            }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
@@ -833,6 +880,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TileShape<OUT>::THRE
         tile_at(p, t + step, &mt1, &nt1);
         bias_r = load_bias2(a, (long)nt1 * S::N + cg * 64 + 2 * lane);
       }
+      using T = typename std::conditional<OUT == FP8_F32, float, __nv_bfloat16>::type;
+      uint32_t res[2][32];  // of the columns that do not go by TMA, 32 at a time
+      if (boxes == 0 && live > 0) load_rows<T>(a, r0, c0, lane, res[0]);
       ok = warp_wait(acc_full + buf, (tile_n >> 1) & 1, abort_flag, err);
       if (!ok) break;
       tc_fence_after();
@@ -857,10 +907,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TileShape<OUT>::THRE
         }
         if (!tma) {
           if (c0 + c < a.n) {
-            if constexpr (OUT == FP8_F32)
-              store_any<float>(a, v, r0, c0 + c, lane);
-            else
-              store_any<__nv_bfloat16>(a, v, r0, c0 + c, lane);
+            stage_rows(v, row_s + bx * BOX, lane);
+            if (h == 0 && c0 + 32 < a.n) load_rows<T>(a, r0, c0 + 32, lane, res[1]);  // arrives while these are stored
+            if (h == 1 && boxes == 1) load_rows<T>(a, r0, c0 + 32, lane, res[1]);     // (the last columns, after a box by TMA)
+            store_rows<T, true>(a, box + bx * BOX, r0, c0 + c, lane, res[h]);
+            fence_proxy_async();  // (the box's next residual comes by TMA)
+            __syncwarp();
           }
           continue;
         }

@@ -583,3 +583,29 @@ def test_most_rows(kk):
     fp8.linear(q, w, out=x)
     fp8.check()
     assert torch.equal(x[at], 2.0 * vals) and torch.count_nonzero(x).item() == len(at)
+
+
+@pytest.mark.parametrize("m, n, k", [(4900, 1010, 200), (4867, 1037, 300), (4900, 1024, 140)])
+@pytest.mark.parametrize("ldy_pad, off", [(1, 0), (2, 1), (4, 4), (8, 0), (0, 3), (6, 0), (2, 0), (0, 0)])
+def test_linear_any_strides_without_residual(kk, m, n, k, ldy_pad, off):
+    """The same for the kernel without a residual, and a residual that is the result itself against one that is not."""
+    rng = np.random.default_rng(m + n + ldy_pad + 1)
+    fp8 = kk.fp8
+    xq, wq, xd, wd = make(rng, m, n, k, fp8)
+    want, S = ref.linear(xd, wd)
+    rms = np.sqrt((xd ** 2) @ (wd ** 2).T + want ** 2)
+    for dtype in (torch.float32, torch.bfloat16):
+        def view(buf):
+            return buf[off:off + m * (n + ldy_pad)].view(m, n + ldy_pad)[:, :n]
+
+        buf = torch.full((off + (m + 2) * (n + ldy_pad),), 7.0, device="cuda", dtype=dtype)
+        y = view(buf)
+        fp8.linear(xq, wq, out_dtype=dtype, out=y)
+        check_linear(y, want, S, rms, k, None, dtype)
+        r = torch.randn(m, n, device="cuda").to(dtype)
+        other = fp8.linear(xq, wq, residual=r, out_dtype=dtype)
+        y.copy_(r)
+        fp8.linear(xq, wq, residual=y, out_dtype=dtype, out=y)
+        assert torch.equal(y, other)
+        view(buf).fill_(7.0)
+        assert (buf == 7.0).all()
