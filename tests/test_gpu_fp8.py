@@ -609,3 +609,21 @@ def test_linear_any_strides_without_residual(kk, m, n, k, ldy_pad, off):
         assert torch.equal(y, other)
         view(buf).fill_(7.0)
         assert (buf == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows, k", [(1, 1), (3, 3), (5, 130), (40, 255), (9, 1027), (6000, 770), (300, 16301)])
+def test_read_back_into_any_rows(kk, dtype, rows, k):
+    """Rows at every offset and stride from a 16-byte boundary; nothing is written beside them."""
+    rng = np.random.default_rng(rows + k)
+    x = torch.from_numpy(rng.standard_normal((rows, k)).astype(np.float32)).cuda()
+    for block_rows in (1, 128):
+        q = kk.fp8.quantize(x, block_rows=block_rows)
+        want = torch.from_numpy(ref.dequantize(bits(q.values), q.exps.cpu().numpy(), block_rows).astype(np.float32)).cuda().to(dtype)
+        for pad, off in ((0, 0), (1, 0), (2, 1), (3, 3), (4, 5), (5, 2), (6, 7), (7, 4), (8, 6)):
+            buf = torch.full((off + rows * (k + pad) + 9,), 7.0, device="cuda", dtype=dtype)
+            y = buf[off:off + rows * (k + pad)].view(rows, k + pad)[:, :k]
+            kk.fp8.dequantize(q, dtype, out=y)
+            assert torch.equal(y, want)
+            y.fill_(7.0)
+            assert (buf == 7.0).all()
