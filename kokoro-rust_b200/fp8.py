@@ -79,12 +79,18 @@ class Fp8Tensor:
 
     @classmethod
     def empty(cls, rows: int, k: int, block_rows: int = 1, device="cuda") -> "Fp8Tensor":
-        """A store with its rows padded to the alignment that the operators want; not initialised."""
+        """A store with its rows padded to the alignment that the operators want (or do best with); not initialised."""
         if block_rows != 1 and block_rows != 128:
             _refuse("block_rows must be 1 or 128")
         if rows < 0 or k < 0:
             _refuse("rows and columns must not be negative")
+        # Rows of values begin on the largest of 128, 64 or 32 bytes that pads them by at most an eighth: L2 gives whole
+        # sectors of 32 (33,104 x 770 -> 2304: 81 us in rows of 784 bytes, 69 in 800, 66 in 832, 64 in 896).
         ldv, lde = -(-k // 16) * 16, -(-k // 512) * 4
+        for unit in (128, 64, 32):
+            if -k % unit * 8 <= k:
+                ldv = -(-k // unit) * unit
+                break
         self = cls.__new__(cls)
         # one allocation: the values, then the exponents; the views are made when they are asked for
         self._buf = torch.empty(rows * ldv + -(-rows // block_rows) * lde, dtype=torch.uint8, device=device)
