@@ -1392,26 +1392,30 @@ static cudaError_t launch_split(const Fp8Linear& a, int splits, int* err, cudaSt
 
 // Which kernel, by the number of tiles and of blocks of K (times of launches in a row, us).
 //  * Split kernel up to two CTAs an SM, one when K is long: rows x K -> n 2048 x 768 -> 2304 (288 tiles of 128) 9.1
-//    against 9.4 with pairs, 4096 x 768 -> 2304 (576) 16.1 against 12.9; 1024 x 4096 -> 4096 (256) 19.8 against 17.7.
+//    against 9.4 with pairs, 4096 x 768 -> 2304 (576) 16.1 against 12.9; 1024 x 4096 -> 4096 (256) 19.8 against 17.7. One
+//    for an e4m3 result too, whose epilogue has twice the warps with pairs: 1024 x 768 -> 2048 (128) 9.2 against 9.9,
+//    1280 (160) 11.8 against 10.0, 2048 (256) with GELU 13.3 against 11.9.
 //  * Its tiles are 64 columns wide while those are few (up to 1.5 an SM): 512 x 768 -> 2304 (144) 5.9 against 6.8 with
 //    128, 2048 x 768 -> 768 (192) 8.6 against 9.6, 1024 x 768 -> 2304 (288) 7.4 against 7.1; 128 wide for an e4m3 result,
 //    whose blocks are, and when K is long, where a CTA has more of W on its way: 1 x 8192 -> 8192 11.3 against 14.4.
 //  * K is split (a cluster costs about 0.5 us to start and more the more there are) into shares of four blocks or more
 //    (one for an e4m3 result, whose epilogue the shares split too: 256 x 768 -> 2048 8.1 in four against 9.4), as far as
-//    every CTA has an SM of its own, or half of one when K is long: 1 x 2048 -> 768 5.4 in four shares against 7.4 in
-//    one, 1 x 768 -> 2304 5.1 in one against 5.5 in two, 512 x 2048 -> 768 8.0 in two (96 CTAs) against 9.3 in one and
-//    14.5 in eight (384).
+//    every CTA has an SM of its own, or half of one when K is long (seven eighths of the halves with clusters of four or
+//    more, which do not divide every GPC's SMs: 9458 x 4352 -> 68, 74 tiles, 18.2 in two against 24.6 in four): 1 x 2048
+//    -> 768 5.4 in four shares against 7.4 in one, 1 x 768 -> 2304 5.1 in one against 5.5 in two, 512 x 2048 -> 768 8.0
+//    in two (96 CTAs) against 9.3 in one and 14.5 in eight (384).
 template <int OUT>
 static cudaError_t launch_out(const Fp8Linear& a, int* err, cudaStream_t st) {
   const int sms = num_sms(), kb = (int)((a.k + 127) / 128);
   if (sms <= 0) return cudaErrorInvalidDevice;
   const long rows = (a.m + TM - 1) / TM, t128 = rows * ((a.n + 127) / 128), t64 = rows * ((a.n + 63) / 64);
-  if (t128 <= (kb > 16 ? sms : 2 * sms)) {
+  if (t128 <= (kb > 16 || OUT == FP8_E4M3 ? sms : 2 * sms)) {
     const bool long_k = kb > 32, narrow = OUT != FP8_E4M3 && !long_k && t64 <= sms + sms / 2;
     const long tiles = narrow ? t64 : t128, room = long_k ? 2 * sms : sms;
     int splits = 1;
     const int least = OUT == FP8_E4M3 ? 1 : 4;  // blocks of a share
-    while (splits < 8 && least * 2 * splits <= kb && tiles * 2 * splits <= room) splits *= 2;
+    while (splits < 8 && least * 2 * splits <= kb && tiles * 2 * splits <= (long_k && splits > 1 ? room - room / 8 : room))
+      splits *= 2;
     if constexpr (OUT != FP8_E4M3) {
       if (narrow) return launch_split<64, OUT>(a, splits, err, st);
     }
