@@ -718,10 +718,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<OUT>::THRE
             sts_u4(row_s + (((4 * odd + q) ^ (lane & 7)) << 4), make_uint4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]));
           fence_proxy_async();
         } else if (live && r0 + lane < a.m) {  // the last columns
-          uint8_t* row = a.q.v + (r0 + lane) * a.q.ldv + c0;
+          uint8_t* row = a.q.v + (r0 + lane) * a.q.ldv + c0;  // (16-byte aligned)
+          const int cols = (int)min(64l, a.n - c0);
 #pragma unroll
-          for (int i = 0; i < 64; i++)
-            if (c0 + i < a.n) row[i] = (uint8_t)(u[i >> 2] >> (8 * (i & 3)));
+          for (int q = 0; q < 4; q++) {
+            if (16 * q + 16 <= cols) {
+              *reinterpret_cast<uint4*>(row + 16 * q) = make_uint4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]);
+            } else {
+#pragma unroll
+              for (int i = 16 * q; i < 16 * q + 16; i++)
+                if (i < cols) row[i] = (uint8_t)(u[i >> 2] >> (8 * (i & 3)));
+            }
+          }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(box_in + bx);

@@ -97,7 +97,7 @@ template <int N>  // a multiple of 4; the steps of all N values side by side, be
 __device__ __forceinline__ void gelu_fast(float* v) {
   constexpr float k = -2.0f * 0.797884560802865355f * 1.44269504088896341f;  // -2 sqrt(2 / pi) log2(e)
   const uint64_t k1 = pack2(0.044715f * k, 0.044715f * k), k0 = pack2(k, k);
-  float t[N], r[N / 2];
+  float t[N];
 #pragma unroll
   for (int i = 0; i < N; i++) asm("max.NaN.f32 %0, %1, %2;" : "=f"(v[i]) : "f"(v[i]), "f"(-5.6f));
 #pragma unroll
@@ -110,15 +110,15 @@ __device__ __forceinline__ void gelu_fast(float* v) {
 #pragma unroll
   for (int i = 0; i < N; i += 2) add2(t[i], t[i + 1], 1.0f, 1.0f);
 #pragma unroll
-  for (int i = 0; i < N; i += 4) {
-    const float p0 = t[i] * t[i + 1], p1 = t[i + 2] * t[i + 3];
-    float q;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(p0 * p1));
-    r[i / 2] = q * p1, r[i / 2 + 1] = q * p0;  // 1 / p0, 1 / p1
+  for (int i = 0; i < N; i += 4) {  // in pairs that need no swap: 1 / a and 1 / b are c and d times 1 / (a c), 1 / (b d)
+    const uint64_t ab = pack2(t[i], t[i + 1]), cd = pack2(t[i + 2], t[i + 3]);
+    float ac, bd, q;
+    unpack2(mul2(ab, cd), ac, bd);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(ac * bd));
+    const uint64_t r = pack2(q * bd, q * ac);
+    unpack2(mul2(pack2(v[i], v[i + 1]), mul2(cd, r)), v[i], v[i + 1]);
+    unpack2(mul2(pack2(v[i + 2], v[i + 3]), mul2(ab, r)), v[i + 2], v[i + 3]);
   }
-#pragma unroll
-  for (int i = 0; i < N; i += 2)
-    unpack2(mul2(pack2(v[i], v[i + 1]), mul2(pack2(t[i + 1], t[i]), pack2(r[i / 2], r[i / 2]))), v[i], v[i + 1]);
 }
 
 }  // namespace kk
