@@ -1061,6 +1061,35 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
   float bias_r[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) bias_r[i] = a.bias && n0 + c + i < a.n ? a.bias[n0 + c + i] : 0.0f;
+  // and the residual of its first unit; from then on a unit's comes while the one before it is worked on
+  const int units = rows * UNITS, stride = splits * SPLIT_THREADS, first = share * SPLIT_THREADS + threadIdx.x;
+  uint32_t res[4] = {0, 0, 0, 0};  // bits of y's type; two bf16 in a word where rows are loaded so
+  auto load_res = [&](int u) {
+    if (OUT == FP8_E4M3 || !a.res || u >= units) return;
+    const long m = m0 + u / UNITS, n = n0 + c;
+    if (OUT == FP8_F32) {
+      const uint32_t* rr = (const uint32_t*)a.res + m * a.ldr + n;
+      if (p.vec_res && n + 4 <= a.n) {
+        const uint4 f = *reinterpret_cast<const uint4*>(rr);
+        res[0] = f.x, res[1] = f.y, res[2] = f.z, res[3] = f.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (n + i < a.n) res[i] = rr[i];
+      }
+    } else {
+      const uint16_t* rr = (const uint16_t*)a.res + m * a.ldr + n;
+      if (p.vec_res && n + 4 <= a.n) {
+        const uint2 f = *reinterpret_cast<const uint2*>(rr);
+        res[0] = f.x, res[1] = f.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (n + i < a.n) res[i] = rr[i];
+      }
+    }
+  };
+  load_res(first);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -1145,34 +1174,18 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::TMEM_COLS));
   }
   const bool done = *abort_flag == 0;
-  for (int u = share * SPLIT_THREADS + threadIdx.x; done && u < rows * UNITS; u += splits * SPLIT_THREADS) {
+  for (int u = first; done && u < units; u += stride) {
     const int r = u / UNITS;
     const long m = m0 + r, n = n0 + c;
-    float res_r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (OUT != FP8_E4M3 && a.res) {
-      if (OUT == FP8_F32) {
-        const float* rr = (const float*)a.res + m * a.ldr + n;
-        if (p.vec_res && n + 4 <= a.n) {
-          const float4 f = *reinterpret_cast<const float4*>(rr);
-          res_r[0] = f.x, res_r[1] = f.y, res_r[2] = f.z, res_r[3] = f.w;
-        } else {
+    float res_r[4];
+    if (OUT == FP8_BF16 && p.vec_res && n + 4 <= a.n) {
+      res_r[0] = __uint_as_float(res[0] << 16), res_r[1] = __uint_as_float(res[0] & 0xFFFF0000u);
+      res_r[2] = __uint_as_float(res[1] << 16), res_r[3] = __uint_as_float(res[1] & 0xFFFF0000u);
+    } else {
 #pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (n + i < a.n) res_r[i] = rr[i];
-        }
-      } else {
-        const __nv_bfloat16* rr = (const __nv_bfloat16*)a.res + m * a.ldr + n;
-        if (p.vec_res && n + 4 <= a.n) {
-          const uint2 f = *reinterpret_cast<const uint2*>(rr);
-          res_r[0] = __uint_as_float(f.x << 16), res_r[1] = __uint_as_float(f.x & 0xFFFF0000u);
-          res_r[2] = __uint_as_float(f.y << 16), res_r[3] = __uint_as_float(f.y & 0xFFFF0000u);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (n + i < a.n) res_r[i] = (float)rr[i];
-        }
-      }
+      for (int i = 0; i < 4; i++) res_r[i] = __uint_as_float(OUT == FP8_F32 ? res[i] : res[i] << 16);
     }
+    load_res(u + stride);
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const float* part = (const float*)smem + r * S::PITCH + c;
     if (splits == 1) {
