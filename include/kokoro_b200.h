@@ -409,6 +409,13 @@ KK_API kk_status kk_fp8_linear(int cuda_ordinal, void* stream, int64_t m, int64_
                                const uint8_t* w_exps, int64_t ldwe, const float* bias, int act, const void* residual,
                                int64_t ldr, int y_type, void* y, int64_t ldy, uint8_t* y_exps, int64_t ldye);
 /*
+ * The calls above with their arguments, in their order, as one array of 64-bit numbers (pointers as numbers, NULL as 0;
+ * n of them): for callers whose foreign-function interface pays for each argument (ctypes: 2.6 us for the 22 of
+ * kk_fp8_linear, 0.7 so).
+ */
+typedef enum { KK_FP8_OP_QUANTIZE = 0, KK_FP8_OP_DEQUANTIZE = 1, KK_FP8_OP_LINEAR = 2 } kk_fp8_op;
+KK_API kk_status kk_fp8_call(int op, const int64_t* args, int n);
+/*
  * Waits for the stream and reports (KK_ERR_TIMEOUT, once) whether a bounded in-kernel wait of a
  * kk_fp8_linear on this device gave up since the last check; its results are then not valid. Refused
  * (KK_ERR_CUDA) while the stream is being captured.

@@ -229,6 +229,22 @@ kk_status kk_fp8_linear(int cuda_ordinal, void* stream, int64_t m, int64_t n, in
   }, &g, stream);
 }
 
+kk_status kk_fp8_call(int op, const int64_t* v, int n) {
+  if (!v) return fail(KK_ERR_INVALID_ARG, "null arguments");
+  // what does not fit an int is no type, ordinal, activation or block_rows either
+  const auto i = [v](int k) { return v[k] == (int)v[k] ? (int)v[k] : -1; };
+  const auto p = [v](int k) { return (void*)(uintptr_t)v[k]; };
+  const auto b = [v](int k) { return (uint8_t*)(uintptr_t)v[k]; };
+  if (op == KK_FP8_OP_QUANTIZE && n == 12)
+    return kk_fp8_quantize(i(0), p(1), p(2), i(3), v[4], v[5], v[6], i(7), b(8), v[9], b(10), v[11]);
+  if (op == KK_FP8_OP_DEQUANTIZE && n == 12)
+    return kk_fp8_dequantize(i(0), p(1), b(2), v[3], b(4), v[5], i(6), v[7], v[8], p(9), i(10), v[11]);
+  if (op == KK_FP8_OP_LINEAR && n == 22)
+    return kk_fp8_linear(i(0), p(1), v[2], v[3], v[4], b(5), v[6], b(7), v[8], b(9), v[10], b(11), v[12],
+                         (const float*)p(13), i(14), p(15), v[16], i(17), p(18), v[19], b(20), v[21]);
+  return fail(KK_ERR_INVALID_ARG, "unknown operation, or not its number of arguments");
+}
+
 kk_status kk_fp8_check(int cuda_ordinal, void* stream) {
   int flag = 0;
   int* const out = &flag;

@@ -14,6 +14,7 @@ refused call.
 """
 from __future__ import annotations
 
+import struct
 from typing import Optional, Union
 
 import torch
@@ -122,6 +123,10 @@ class Fp8Tensor:
         return Fp8Tensor(self.values[rows], self.exps[rows])
 
 
+# the arguments of the C calls, packed (kk_fp8_call)
+_args12, _args22 = struct.Struct("12q").pack, struct.Struct("22q").pack
+
+
 def _run(status: int) -> None:
     if status != 0:
         raise KokoroError(status, load_library().kk_fp8_error().decode())
@@ -142,8 +147,8 @@ def quantize(x: torch.Tensor, block_rows: int = 1, out: Optional[Fp8Tensor] = No
         _refuse("out: a store of x's shape and of the same block_rows is wanted")
     elif out.device != dev:
         _one_device(dev, out.device)
-    _run(load_library().kk_fp8_quantize(dev.index, _stream(dev.index), x.data_ptr(), _TYPES[x.dtype], rows, k, ld,
-                                        block_rows, *out._args))
+    _run(load_library().kk_fp8_call(0, _args12(dev.index, _stream(dev.index), x.data_ptr(), _TYPES[x.dtype], rows, k, ld,
+                                               block_rows, *out._args), 12))
     return out
 
 
@@ -162,8 +167,8 @@ def dequantize(q: Fp8Tensor, dtype: torch.dtype = torch.float32, out: Optional[t
         if out.shape != q.shape:
             _refuse("out: the store's shape is wanted")
         _one_device(dev, out.device)
-    _run(load_library().kk_fp8_dequantize(dev.index, _stream(dev.index), *q._args, q.block_rows, rows, k, out.data_ptr(),
-                                          _TYPES[dtype], ld))
+    _run(load_library().kk_fp8_call(1, _args12(dev.index, _stream(dev.index), *q._args, q.block_rows, rows, k,
+                                               out.data_ptr(), _TYPES[dtype], ld), 12))
     return out
 
 
@@ -189,7 +194,7 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
     dev = x.device
     if w.device != dev:
         _one_device(dev, w.device)
-    b = None
+    b = 0
     if bias is not None:
         if not isinstance(bias, torch.Tensor) or bias.dtype is not _F32 or bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
             _refuse(f"bias: adjacent float32 [{n}] is wanted")
@@ -198,7 +203,7 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
         if bias.device != dev:
             _one_device(dev, bias.device)
         b = bias.data_ptr()
-    res, ldr = None, 0
+    res, ldr = 0, 0
     if residual is not None:
         if out_dtype is E4M3:
             _refuse("an e4m3 result takes no residual")
@@ -216,16 +221,16 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
         y = out._args
     elif out is None:
         out = torch.empty((m, n), dtype=out_dtype, device=dev)
-        y = (out.data_ptr(), n, None, 0)
+        y = (out.data_ptr(), n, 0, 0)
     else:
         ldy = _rows(out, "out", (out_dtype,))[2]
         if out.shape != (m, n):
             _refuse(f"out: [{m}, {n}] is wanted")
-        y = (out.data_ptr(), ldy, None, 0)
+        y = (out.data_ptr(), ldy, 0, 0)
     if out.device != dev:
         _one_device(dev, out.device)
-    _run(load_library().kk_fp8_linear(dev.index, _stream(dev.index), m, n, k, *x._args, *w._args, b, _ACTS[act], res, ldr,
-                                      _TYPES[out_dtype], *y))
+    _run(load_library().kk_fp8_call(2, _args22(dev.index, _stream(dev.index), m, n, k, *x._args, *w._args, b, _ACTS[act],
+                                               res, ldr, _TYPES[out_dtype], *y), 22))
     return out
 
 

@@ -89,6 +89,38 @@ def test_linear_refusals(kk, kw, word):
     assert word in lib.kk_fp8_error().decode()
 
 
+def test_packed_calls_are_the_same_calls(kk):
+    """Each argument in its place: one is spoilt at a time, and the status and the message are those of the call itself."""
+    import struct
+    lib = kk.load_library()
+    quant = q_args(x=1 << 30, v=1 << 31, e=1 << 32, dev=99)
+    deq = [quant[0], quant[1], quant[8], quant[9], quant[10], quant[11], quant[7], quant[4], quant[5], quant[2], quant[3], quant[6]]
+    lin = l_args(x=1 << 30, xe=1 << 31, w=1 << 32, we=1 << 33, y=1 << 34, res=1 << 35, bias=1 << 36, dev=99)
+    lin8 = l_args(x=1 << 30, xe=1 << 31, w=1 << 32, we=1 << 33, y=1 << 34, yt=2, ye=1 << 35, ldye=4, bias=1 << 36, dev=99)
+    seen = set()
+    for op, f, good in ((0, lib.kk_fp8_quantize, quant), (1, lib.kk_fp8_dequantize, deq), (2, lib.kk_fp8_linear, lin),
+                        (2, lib.kk_fp8_linear, lin8)):
+        for i in [None, *range(len(good))]:
+            for bad in (-1, 1, 7, 0):
+                a = list(good)
+                if i is not None:
+                    if i < 2:
+                        continue  # (the device and the stream: this machine may have none)
+                    a[i] = bad
+                st, msg = f(*a), lib.kk_fp8_error()
+                packed = struct.pack(f"{len(a)}q", *(v or 0 for v in a))
+                assert (lib.kk_fp8_call(op, packed, len(a)), lib.kk_fp8_error()) == (st, msg)
+                seen.add(msg)
+    assert len(seen) > 15
+    packed = struct.pack("22q", *(v or 0 for v in lin))
+    for op, p, n in ((2, packed, 21), (0, packed, 22), (3, packed, 12), (-1, packed, 22), (2, None, 22)):
+        assert lib.kk_fp8_call(op, p, n) == kk.engine.KK_ERR_INVALID_ARG
+    wide = list(quant)
+    wide[3] = 1 << 32  # as an int it would be type 0
+    assert lib.kk_fp8_call(0, struct.pack("12q", *(v or 0 for v in wide)), 12) == kk.engine.KK_ERR_INVALID_ARG
+    assert "f32 or bf16" in lib.kk_fp8_error().decode()
+
+
 def overlaps(a, b):
     """Whether two lists of (address, rows, bytes of a row, pitch) share a byte, byte by byte."""
     cells = lambda p, rows, width, pitch: {p + i * pitch + j for i in range(rows) for j in range(width)}
