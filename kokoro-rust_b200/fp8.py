@@ -75,7 +75,9 @@ class Fp8Tensor:
         self.device = values.device
         if exps.device != self.device:
             _refuse("values and exps must be on one device")
-        self.shape, self.block_rows, self._values, self._exps, self._buf = values.shape, block_rows, values, exps, None
+        self.shape, self.block_rows, self._values, self._exps = values.shape, block_rows, values, exps
+        # the memory that the calls are given stays, whatever becomes of the two tensors (set_, .data)
+        self._buf = values.untyped_storage(), exps.untyped_storage()
         self._args = (values.data_ptr(), ldv, exps.data_ptr(), lde)
 
     @classmethod
@@ -115,6 +117,9 @@ class Fp8Tensor:
             (rows, k), (_, ldv, _, lde) = self.shape, self._args
             self._exps = self._buf.as_strided((-(-rows // self.block_rows), -(-k // 128)), (lde, 1), rows * ldv)
         return self._exps
+
+    def __reduce__(self):  # a copy (copy.deepcopy, torch.save) is a store over copied tensors, with addresses of its own
+        return Fp8Tensor, (self.values, self.exps, self.block_rows)
 
     def __getitem__(self, rows: slice) -> "Fp8Tensor":
         """A view of some of an activation store's rows (to read them, or to quantise into them)."""

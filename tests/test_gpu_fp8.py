@@ -627,3 +627,41 @@ def test_read_back_into_any_rows(kk, dtype, rows, k):
             assert torch.equal(y, want)
             y.fill_(7.0)
             assert (buf == 7.0).all()
+
+
+@pytest.mark.parametrize("rows, k, block_rows", [(1, 5, 1), (130, 300, 1), (130, 300, 128)])
+def test_copies_of_a_store_have_memory_of_their_own(kk, rows, k, block_rows):
+    import copy
+    import io
+    fp8 = kk.fp8
+    x = torch.randn(rows, k, device="cuda")
+    q = fp8.quantize(x, block_rows=block_rows)
+    want = fp8.dequantize(q)
+    file = io.BytesIO()
+    torch.save(q, file)
+    copies = [copy.deepcopy(q), copy.deepcopy(fp8.Fp8Tensor(q.values, q.exps, block_rows))]
+    if block_rows == 1:
+        copies.append(copy.deepcopy(q[0:rows]))
+    file.seek(0)
+    copies.append(torch.load(file, weights_only=False))
+    fp8.quantize(torch.zeros_like(x), block_rows=block_rows, out=q)
+    del q
+    torch.cuda.empty_cache()
+    for c in copies:
+        assert c.shape == (rows, k) and c.block_rows == block_rows
+        assert torch.equal(fp8.dequantize(c), want)
+        fp8.quantize(2 * x, block_rows=block_rows, out=c)
+        assert torch.equal(fp8.dequantize(c), 2 * want)
+
+
+def test_a_store_keeps_the_memory_it_was_made_over(kk):
+    fp8 = kk.fp8
+    q = fp8.quantize(torch.randn(64, 256, device="cuda"))
+    want = fp8.dequantize(q)
+    v, e = q.values.clone(), torch.zeros(64, 4, device="cuda", dtype=torch.uint8)[:, :2]  # (rows 4 bytes apart)
+    e.copy_(q.exps)
+    s = fp8.Fp8Tensor(v, e)
+    v.set_(torch.empty(0, 0, device="cuda", dtype=E4M3))
+    e.set_(torch.empty(0, 0, device="cuda", dtype=torch.uint8))
+    torch.cuda.empty_cache()
+    assert torch.equal(fp8.dequantize(s), want)
