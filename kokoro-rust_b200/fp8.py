@@ -166,7 +166,7 @@ def dequantize(q: Fp8Tensor, dtype: torch.dtype = torch.float32, out: Optional[t
         _refuse("dtype: float32 or bfloat16 is wanted")
     (rows, k), dev = q.shape, q.device
     if out is None:
-        out, ld = torch.empty((rows, k), dtype=dtype, device=dev), k
+        out, ld = torch.empty(rows, k, dtype=dtype, device=dev), k
     else:
         ld = _rows(out, "out", (dtype,))[2]
         if out.shape != q.shape:
@@ -225,7 +225,7 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
             _refuse(f"out: a store [{m}, {n}] with block_rows 1 is wanted")
         y = out._args
     elif out is None:
-        out = torch.empty((m, n), dtype=out_dtype, device=dev)
+        out = torch.empty(m, n, dtype=out_dtype, device=dev)
         y = (out.data_ptr(), n, 0, 0)
     else:
         ldy = _rows(out, "out", (out_dtype,))[2]
