@@ -494,7 +494,14 @@ def test_what_lies_behind_a_row_is_not_read(kk, m, n, k):
     assert torch.equal(fp8.dequantize(x2), fp8.dequantize(xq)) and torch.equal(fp8.dequantize(w2), fp8.dequantize(wq))
 
 
-def test_offsets_past_32_bits(kk):
+@pytest.fixture
+def much_memory():
+    """For tests that hold tens of GB: what they leave cached goes back, for the engines of the tests after them."""
+    yield
+    torch.cuda.empty_cache()
+
+
+def test_offsets_past_32_bits(kk, much_memory):
     """Rows that begin past 2^31 elements and 2^32 bytes: the last ones equal those of a small call."""
     fp8 = kk.fp8
     torch.manual_seed(14)
@@ -546,7 +553,7 @@ def test_check_inside_a_capture_is_refused(kk):
 
 
 @pytest.mark.parametrize("m, n, k", [(1, 1, (1 << 30) - 3), (3, 130, (1 << 28) + 200)])
-def test_longest_rows(kk, m, n, k):
+def test_longest_rows(kk, much_memory, m, n, k):
     """The whole sum of the longest rows waits for one CTA's (or one cluster's) loads."""
     fp8 = kk.fp8
     rng = np.random.default_rng(16)
@@ -566,7 +573,7 @@ def test_longest_rows(kk, m, n, k):
     assert np.array_equal(y.cpu().numpy(), (x @ w.T).astype(np.float32))
 
 
-def test_most_rows(kk):
+def test_most_rows(kk, much_memory):
     """2^31 - 1 rows, the most a call takes: the quantiser's, the read-back's and the layer's row indices."""
     fp8 = kk.fp8
     rows = (1 << 31) - 1
