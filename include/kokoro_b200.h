@@ -403,6 +403,8 @@ KK_API kk_status kk_fp8_dequantize(int cuda_ordinal, void* stream, const uint8_t
  * overlap it).
  * y_type KK_FP8_E4M3: y / ldy and y_exps / ldye are a store (block_rows 1) that the result is quantised
  * into, without a residual. y may not overlap x, w or bias.
+ * KK_FP8_ACT_GELU is within 2^-20 of the value or 2.7e-9, whichever is more (values below -5.6 count as -5.6);
+ * a bias of minus infinity makes its column NaN, as the formula's -inf * 0 is.
  */
 KK_API kk_status kk_fp8_linear(int cuda_ordinal, void* stream, int64_t m, int64_t n, int64_t k, const uint8_t* x,
                                int64_t ldx, const uint8_t* x_exps, int64_t ldxe, const uint8_t* w, int64_t ldw,

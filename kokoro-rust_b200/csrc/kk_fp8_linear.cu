@@ -440,6 +440,11 @@ __device__ __forceinline__ float2 load_bias2(const Fp8Linear& a, long c) {
   if (c + 1 < a.n) b.y = a.bias[c + 1];
   return b;
 }
+// ...into a warp's row of biases, once it is there
+__device__ __forceinline__ void stage_bias2(const Fp8Linear& a, float* bias_s, float2 b) {
+  if (a.gelu) b.x = gelu_bias(b.x), b.y = gelu_bias(b.y);
+  *reinterpret_cast<float2*>(bias_s) = b;
+}
 
 __device__ __forceinline__ void add_bias32(float* v, const float* bias_s) {
 #pragma unroll
@@ -674,7 +679,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<OUT>::THRE
       if (S::Q && !odd && lane == 0) bulk_wait_all_read();  // the box is free once the last tile's store has read it
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < S::COLS / 64; i++) *reinterpret_cast<float2*>(bias_s + 64 * i + 2 * lane) = bias_r[i];
+      for (int i = 0; i < S::COLS / 64; i++) stage_bias2(a, bias_s + 64 * i + 2 * lane, bias_r[i]);
       __syncwarp();
       if (t + step < tiles) load_bias_r(t + step);  // the next tile's, which arrives during this one
       ok = warp_wait(acc_full, tile_n & 1, abort_flag, err);
@@ -881,7 +886,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TileShape<OUT>::THRE
         }
       }
       __syncwarp();
-      *reinterpret_cast<float2*>(bias_s + 2 * lane) = bias_r;
+      stage_bias2(a, bias_s + 2 * lane, bias_r);
       __syncwarp();
       if (t + step < tiles) {  // the next tile's, which arrives during this one
         int mt1, nt1;
@@ -1174,6 +1179,10 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::TMEM_COLS));
   }
   const bool done = *abort_flag == 0;
+  if (a.gelu) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) bias_r[i] = gelu_bias(bias_r[i]);
+  }
   for (int u = first; done && u < units; u += stride) {
     const int r = u / UNITS;
     const long m = m0 + r, n = n0 + c;

@@ -672,3 +672,25 @@ def test_a_store_keeps_the_memory_it_was_made_over(kk):
     e.set_(torch.empty(0, 0, device="cuda", dtype=torch.uint8))
     torch.cuda.empty_cache()
     assert torch.equal(fp8.dequantize(s), want)
+
+
+@pytest.mark.parametrize("m, n, k", [(5, 300, 256), (700, 640, 520), (4800, 1000, 300), (4800, 1000, 1700)])
+def test_gelu_of_minus_infinity(kk, m, n, k):
+    """-inf (1 + tanh(-inf)) / 2 is NaN: in its columns only, the first and the last among them, in every result type and
+    kernel, and without GELU it is minus infinity."""
+    rng = np.random.default_rng(21)
+    fp8 = kk.fp8
+    xq, wq, xd, wd = make(rng, m, n, k, fp8)
+    bias = torch.randn(n, device="cuda")
+    cols = [0, 7, 8, 200, n - 1]
+    bias[cols] = float("-inf")
+    res = torch.ones(m, n, device="cuda")
+    other = torch.ones(n, dtype=torch.bool, device="cuda")
+    other[cols] = False
+    for dtype in (torch.float32, torch.bfloat16, E4M3):
+        for r in (None, res) if dtype != E4M3 else (None,):
+            for act in ("gelu", None):
+                y = fp8.linear(xq, wq, bias, act=act, out_dtype=dtype, residual=None if r is None else r.to(dtype))
+                y = fp8.dequantize(y) if dtype == E4M3 else y.float()
+                assert y[:, other].isfinite().all()
+                assert (y[:, cols].isnan() if act or dtype == E4M3 else y[:, cols] == float("-inf")).all()
