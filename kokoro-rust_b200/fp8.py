@@ -9,8 +9,8 @@ as e4m3 values with a power-of-two scale for each block of 128, and the linear l
 Calls enqueue on the current stream of their tensors' device and allocate only their results (give
 ``out`` to have none); they may be captured into a CUDA graph. Tensors made or last used on another
 stream are the caller's to order, as for any torch operator. There is no gradient: a tensor that
-requires one is refused while gradients are being recorded. ``KokoroError`` carries the status of a
-refused call.
+requires one is refused while gradients are being recorded, and so is one with a forward-mode tangent.
+``KokoroError`` carries the status of a refused call.
 """
 from __future__ import annotations
 
@@ -18,6 +18,7 @@ import struct
 from typing import Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from .engine import KK_ERR_INVALID_ARG, KokoroError, load_library
 
@@ -39,6 +40,14 @@ def _public_stream(index: int) -> int:
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
 
 
+def _no_gradient(t: torch.Tensor, name: str):
+    if t.requires_grad and torch.is_grad_enabled():
+        _refuse(f"{name}: the 8-bit operators have no gradient")
+    # (a tangent lives inside a dual level, -1 outside of all: looking there first is 0.03 us instead of 0.5)
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        _refuse(f"{name}: the 8-bit operators have no gradient, in forward mode either")
+
+
 def _rows(t: torch.Tensor, name: str, dtypes, unit: int = 1):
     """(rows, columns, row stride) of a CUDA tensor of rows whose columns are adjacent; a single row's
     stride is whatever holds its columns."""
@@ -51,10 +60,9 @@ def _rows(t: torch.Tensor, name: str, dtypes, unit: int = 1):
     ld, inner = t.stride()
     if inner != 1 and k > 1:
         _refuse(f"{name}: a row's columns must be adjacent")
+    _no_gradient(t, name)
     if not t.is_cuda:
         _refuse(f"{name}: a CUDA tensor is wanted")
-    if t.requires_grad and torch.is_grad_enabled():
-        _refuse(f"{name}: the 8-bit operators have no gradient")
     return rows, k, ld if rows > 1 else -(-k // unit) * unit
 
 
@@ -203,8 +211,7 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
     if bias is not None:
         if not isinstance(bias, torch.Tensor) or bias.dtype is not _F32 or bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
             _refuse(f"bias: adjacent float32 [{n}] is wanted")
-        if bias.requires_grad and torch.is_grad_enabled():
-            _refuse("bias: the 8-bit operators have no gradient")
+        _no_gradient(bias, "bias")
         if bias.device != dev:
             _one_device(dev, bias.device)
         b = bias.data_ptr()

@@ -220,3 +220,24 @@ def test_fp8_error_is_per_thread(kk):
     t.start()
     t.join()
     assert lib.kk_fp8_error() and got == [b""]
+
+
+def test_forward_mode_tangents_are_refused(kk):
+    """As rows, and as the values of a store; outside of their level, or with forward mode off, there is none to lose."""
+    from torch.autograd import forward_ad
+    fp8 = kk.fp8
+    x, v = torch.randn(4, 128), torch.zeros(4, 128, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        assert "forward mode" in refused(kk, fp8.quantize, d)
+        dv = forward_ad.make_dual(v, torch.zeros_like(v))
+        assert "forward mode" in refused(kk, fp8.Fp8Tensor, dv, torch.zeros(4, 1, dtype=torch.uint8))
+        with torch.no_grad():
+            assert "forward mode" in refused(kk, fp8.quantize, d)
+        with torch.inference_mode():  # (no tangents are kept here)
+            assert "CUDA tensor" in refused(kk, fp8.quantize, d)
+        assert "CUDA tensor" in refused(kk, fp8.quantize, x)
+    assert "CUDA tensor" in refused(kk, fp8.quantize, d)
+    with pytest.raises(kk.KokoroError, match="forward mode"):
+        torch.func.jvp(fp8.quantize, (x,), (x,))
+    assert "no gradient" in refused(kk, fp8.quantize, x.clone().requires_grad_())

@@ -694,3 +694,21 @@ def test_gelu_of_minus_infinity(kk, m, n, k):
                 y = fp8.dequantize(y) if dtype == E4M3 else y.float()
                 assert y[:, other].isfinite().all()
                 assert (y[:, cols].isnan() if act or dtype == E4M3 else y[:, cols] == float("-inf")).all()
+
+
+def test_forward_mode_tangents_are_refused(kk):
+    """In every argument of a layer."""
+    from torch.autograd import forward_ad
+    fp8 = kk.fp8
+    x = fp8.quantize(torch.randn(4, 256, device="cuda"))
+    w = fp8.quantize(torch.randn(130, 256, device="cuda"), block_rows=128)
+    b, y = torch.zeros(130, device="cuda"), torch.zeros(4, 130, device="cuda")
+    want = fp8.linear(x, w, b, residual=y)
+    with forward_ad.dual_level():
+        db, dy = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (b, y))
+        for kw in (dict(bias=db), dict(residual=dy), dict(out=dy)):
+            with pytest.raises(kk.KokoroError, match="forward mode"):
+                fp8.linear(x, w, **kw)
+        with pytest.raises(kk.KokoroError, match="forward mode"):
+            fp8.dequantize(fp8.quantize(y), out=dy)
+        assert torch.equal(fp8.linear(x, w, b, residual=y), want)
