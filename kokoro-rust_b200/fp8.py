@@ -60,6 +60,8 @@ def _rows(t: torch.Tensor, name: str, dtypes, unit: int = 1):
     ld, inner = t.stride()
     if inner != 1 and k > 1:
         _refuse(f"{name}: a row's columns must be adjacent")
+    if k == 1 and t.is_neg():  # (the imaginary part of a conjugate, whose columns are never adjacent)
+        _refuse(f"{name}: its negation is still to be done (resolve_neg)")
     _no_gradient(t, name)
     if not t.is_cuda:
         _refuse(f"{name}: a CUDA tensor is wanted")
@@ -212,6 +214,8 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
         if not isinstance(bias, torch.Tensor) or bias.dtype is not _F32 or bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
             _refuse(f"bias: adjacent float32 [{n}] is wanted")
         _no_gradient(bias, "bias")
+        if n == 1 and bias.is_neg():
+            _refuse("bias: its negation is still to be done (resolve_neg)")
         if bias.device != dev:
             _one_device(dev, bias.device)
         b = bias.data_ptr()

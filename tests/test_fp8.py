@@ -241,3 +241,11 @@ def test_forward_mode_tangents_are_refused(kk):
     with pytest.raises(kk.KokoroError, match="forward mode"):
         torch.func.jvp(fp8.quantize, (x,), (x,))
     assert "no gradient" in refused(kk, fp8.quantize, x.clone().requires_grad_())
+
+
+def test_negation_still_to_be_done_is_refused(kk):
+    """The imaginary part of a conjugate holds its numbers with the other sign."""
+    c = torch.randn(5, 1, dtype=torch.complex64).conj().imag
+    assert c.is_neg()
+    assert "resolve_neg" in refused(kk, kk.fp8.quantize, c)
+    assert "CUDA tensor" in refused(kk, kk.fp8.quantize, c.resolve_neg())

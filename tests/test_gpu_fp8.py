@@ -712,3 +712,21 @@ def test_forward_mode_tangents_are_refused(kk):
         with pytest.raises(kk.KokoroError, match="forward mode"):
             fp8.dequantize(fp8.quantize(y), out=dy)
         assert torch.equal(fp8.linear(x, w, b, residual=y), want)
+
+
+def test_negation_still_to_be_done_is_refused(kk):
+    """In every argument of a layer of one column, where the imaginary part of a conjugate has adjacent columns."""
+    fp8 = kk.fp8
+    x = fp8.quantize(torch.randn(4, 256, device="cuda"))
+    w = fp8.quantize(torch.randn(1, 256, device="cuda"), block_rows=128)
+    y = torch.randn(4, 1, dtype=torch.complex64, device="cuda").conj().imag
+    b = torch.randn(1, dtype=torch.complex64, device="cuda").conj().imag
+    assert y.is_neg() and b.is_neg()
+    for kw in (dict(bias=b), dict(residual=y), dict(out=y)):
+        with pytest.raises(kk.KokoroError, match="resolve_neg"):
+            fp8.linear(x, w, **kw)
+    for f in (lambda: fp8.quantize(y), lambda: fp8.dequantize(fp8.quantize(y.resolve_neg()), out=y)):
+        with pytest.raises(kk.KokoroError, match="resolve_neg"):
+            f()
+    assert torch.equal(fp8.linear(x, w, b.resolve_neg(), residual=y.resolve_neg()),
+                       fp8.linear(x, w, b.resolve_neg().clone(), residual=y.contiguous().resolve_neg().clone()))
