@@ -255,5 +255,7 @@ def check(device=None) -> None:
     device gave up since the last check (its results are then not valid). Refused while the stream is
     being captured."""
     dev = torch.device("cuda") if device is None else torch.device(device)
+    if dev.type != "cuda":
+        _refuse(f"device: a CUDA device is wanted, not {dev}")
     idx = torch.cuda.current_device() if dev.index is None else dev.index
     _run(load_library().kk_fp8_check(idx, _stream(idx)))

@@ -249,3 +249,8 @@ def test_negation_still_to_be_done_is_refused(kk):
     assert c.is_neg()
     assert "resolve_neg" in refused(kk, kk.fp8.quantize, c)
     assert "CUDA tensor" in refused(kk, kk.fp8.quantize, c.resolve_neg())
+
+
+def test_check_of_another_kind_of_device_is_refused(kk):
+    for device in ("cpu", torch.device("cpu"), "meta"):
+        assert "CUDA device" in refused(kk, kk.fp8.check, device)
