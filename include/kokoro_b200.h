@@ -423,6 +423,13 @@ KK_API kk_status kk_fp8_call(int op, const int64_t* args, int n);
  * (KK_ERR_CUDA) while the stream is being captured.
  */
 KK_API kk_status kk_fp8_check(int cuda_ordinal, void* stream);
+/*
+ * kk_fp8_wait_selftest -- diagnostics of that failure path: one kernel on the stream waits, with the bounded waits of
+ * kk_fp8_linear (cluster = 0: on a block's own barriers, 1: on those that the other block of a pair arrives on) but a
+ * limit of limit_ns (1 us .. 100 ms), on a barrier that nothing arrives on. It gives up and returns, and the next check
+ * reports it as it would a linear layer's. Only enqueues work, as the operators do. No trap, no fault.
+ */
+KK_API kk_status kk_fp8_wait_selftest(int cuda_ordinal, void* stream, int cluster, int64_t limit_ns);
 /* Message of the last kk_fp8_* failure on this thread. */
 KK_API const char* kk_fp8_error(void);
 

@@ -43,5 +43,7 @@ cudaError_t launch_fp8_dequantize(Fp8Store q, long rows, long k, int block_rows,
 cudaError_t launch_fp8_linear(const Fp8Linear& a, int* err, cudaStream_t st);
 // Waits for the stream (an error while it is being captured); *flag = the current device's flag, which is cleared.
 cudaError_t fp8_take_wait_error(int* flag, cudaStream_t st);
+// A wait that expires (after limit_ns, in place of the waits' own limit) and raises the current device's flag.
+cudaError_t launch_fp8_wait_selftest(int cluster, unsigned long long limit_ns, cudaStream_t st);
 
 }  // namespace kk

@@ -245,6 +245,18 @@ kk_status kk_fp8_call(int op, const int64_t* v, int n) {
   return fail(KK_ERR_INVALID_ARG, "unknown operation, or not its number of arguments");
 }
 
+kk_status kk_fp8_wait_selftest(int cuda_ordinal, void* stream, int cluster, int64_t limit_ns) {
+  if (cluster != 0 && cluster != 1) return fail(KK_ERR_INVALID_ARG, "cluster must be 0 or 1");
+  if (limit_ns < 1000 || limit_ns > 100000000) return fail(KK_ERR_INVALID_ARG, "wait limit outside [1 us, 100 ms]");
+  struct Args {
+    int cluster;
+    unsigned long long limit;
+  } a{cluster, (unsigned long long)limit_ns};
+  return run(cuda_ordinal, "kk_fp8_wait_selftest: ", [](const void* p, cudaStream_t st) {
+    return kk::launch_fp8_wait_selftest(((const Args*)p)->cluster, ((const Args*)p)->limit, st);
+  }, &a, stream);
+}
+
 kk_status kk_fp8_check(int cuda_ordinal, void* stream) {
   int flag = 0;
   int* const out = &flag;

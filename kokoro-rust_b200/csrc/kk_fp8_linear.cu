@@ -130,13 +130,14 @@ __device__ __forceinline__ bool mbar_sleep_cluster(uint64_t* b, uint32_t parity)
   return ok != 0;
 }
 // mbar_wait on such a barrier
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* b, uint32_t parity, volatile int* abort_flag, int* err) {
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* b, uint32_t parity, volatile int* abort_flag, int* err,
+                                                  unsigned long long limit_ns = KK_WAIT_TIMEOUT_NS) {
   if (mbar_sleep_cluster(b, parity)) return true;
   const unsigned long long t0 = tc_now();
   while (true) {
     if (mbar_sleep_cluster(b, parity)) return true;
     if (*abort_flag) return false;
-    if (tc_now() - t0 > KK_WAIT_TIMEOUT_NS) {
+    if (tc_now() - t0 > limit_ns) {
       *abort_flag = 1;
       atomicExch(err, 2);
       return false;
@@ -1461,6 +1462,23 @@ cudaError_t launch_fp8_linear(const Fp8Linear& a, int* err, cudaStream_t st) {
   if (a.m == 0) return cudaSuccess;
   if (a.y_type == FP8_E4M3) return launch_out<FP8_E4M3>(a, err, st);
   return a.y_type == FP8_F32 ? launch_out<FP8_F32>(a, err, st) : launch_out<FP8_BF16>(a, err, st);
+}
+
+// One thread waits for the first phase of a barrier that nothing arrives on.
+__global__ void fp8_wait_selftest_kernel(int cluster, unsigned long long limit_ns) {
+  __shared__ __align__(8) uint64_t bar;
+  __shared__ int abort_flag;
+  mbar_init(&bar, 1);
+  abort_flag = 0;
+  if (cluster)
+    mbar_wait_cluster(&bar, 0, &abort_flag, &g_fp8_wait_error, limit_ns);
+  else
+    mbar_wait_lim(&bar, 0, &abort_flag, &g_fp8_wait_error, limit_ns);
+}
+
+cudaError_t launch_fp8_wait_selftest(int cluster, unsigned long long limit_ns, cudaStream_t st) {
+  fp8_wait_selftest_kernel<<<1, 1, 0, st>>>(cluster, limit_ns);
+  return cudaGetLastError();
 }
 
 cudaError_t fp8_take_wait_error(int* err, cudaStream_t st) {

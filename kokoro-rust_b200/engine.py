@@ -88,6 +88,7 @@ _SIGS = {
                                      ctypes.c_int64]),
     "kk_fp8_call": (ctypes.c_int, [ctypes.c_int, ctypes.c_char_p, ctypes.c_int]),
     "kk_fp8_check": (ctypes.c_int, [ctypes.c_int, _P]),
+    "kk_fp8_wait_selftest": (ctypes.c_int, [ctypes.c_int, _P, ctypes.c_int, ctypes.c_int64]),
     "kk_fp8_error": (ctypes.c_char_p, []),
     "kk_device_memory": (ctypes.c_int, [ctypes.c_int, _P, _P]),
 }

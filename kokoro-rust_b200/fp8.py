@@ -250,12 +250,23 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
     return out
 
 
-def check(device=None) -> None:
-    """Waits for the current stream and raises if a bounded in-kernel wait of a linear layer on this
-    device gave up since the last check (its results are then not valid). Refused while the stream is
-    being captured."""
+def _current(device):
+    """(ordinal, handle of the current stream) of a CUDA device."""
     dev = torch.device("cuda") if device is None else torch.device(device)
     if dev.type != "cuda":
         _refuse(f"device: a CUDA device is wanted, not {dev}")
     idx = torch.cuda.current_device() if dev.index is None else dev.index
-    _run(load_library().kk_fp8_check(idx, _stream(idx)))
+    return idx, _stream(idx)
+
+
+def check(device=None) -> None:
+    """Waits for the current stream and raises if a bounded in-kernel wait of a linear layer on this
+    device gave up since the last check (its results are then not valid). Refused while the stream is
+    being captured."""
+    _run(load_library().kk_fp8_check(*_current(device)))
+
+
+def wait_selftest(device=None, cluster: bool = False, limit_ns: int = 5000) -> None:
+    """Diagnostics: a kernel on the current stream waits in vain for limit_ns and gives up, which the next ``check``
+    reports (kk_fp8_wait_selftest)."""
+    _run(load_library().kk_fp8_wait_selftest(*_current(device), int(cluster), int(limit_ns)))

@@ -254,3 +254,11 @@ def test_negation_still_to_be_done_is_refused(kk):
 def test_check_of_another_kind_of_device_is_refused(kk):
     for device in ("cpu", torch.device("cpu"), "meta"):
         assert "CUDA device" in refused(kk, kk.fp8.check, device)
+
+
+def test_wait_selftest_refusals(kk):
+    lib = kk.load_library()
+    for cluster, limit, word in ((2, 5000, "cluster"), (-1, 5000, "cluster"), (0, 999, "limit"), (1, 100000001, "limit"), (0, -1, "limit")):
+        assert lib.kk_fp8_wait_selftest(0, None, cluster, limit) == kk.engine.KK_ERR_INVALID_ARG
+        assert word in lib.kk_fp8_error().decode()
+    assert "CUDA device" in refused(kk, kk.fp8.wait_selftest, "cpu")

@@ -730,3 +730,29 @@ def test_negation_still_to_be_done_is_refused(kk):
             f()
     assert torch.equal(fp8.linear(x, w, b.resolve_neg(), residual=y.resolve_neg()),
                        fp8.linear(x, w, b.resolve_neg().clone(), residual=y.contiguous().resolve_neg().clone()))
+
+
+def expired(kk):
+    """Whether a check reports an expired wait."""
+    try:
+        kk.fp8.check()
+        return False
+    except kk.KokoroError as e:
+        assert e.status == kk.engine.KK_ERR_TIMEOUT and "wait" in str(e)
+        return True
+
+
+@pytest.mark.parametrize("cluster", [False, True])
+def test_an_expired_wait_is_reported_once(kk, cluster):
+    """5 us on a barrier that nothing arrives on; the layers after it are as right as those before."""
+    rng = np.random.default_rng(22)
+    fp8 = kk.fp8
+    layers = [make(rng, m, 256, 256, fp8)[:2] for m in (5, 6000)]
+    want = [fp8.linear(*l) for l in layers]
+    assert not expired(kk)
+    fp8.wait_selftest(cluster=cluster)
+    assert expired(kk)
+    assert not expired(kk)
+    for l, y in zip(layers, want):
+        assert torch.equal(fp8.linear(*l), y)
+    assert not expired(kk)
