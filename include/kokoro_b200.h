@@ -418,16 +418,18 @@ KK_API kk_status kk_fp8_linear(int cuda_ordinal, void* stream, int64_t m, int64_
 typedef enum { KK_FP8_OP_QUANTIZE = 0, KK_FP8_OP_DEQUANTIZE = 1, KK_FP8_OP_LINEAR = 2 } kk_fp8_op;
 KK_API kk_status kk_fp8_call(int op, const int64_t* args, int n);
 /*
- * Waits for the stream and reports (KK_ERR_TIMEOUT, once) whether a bounded in-kernel wait of a
- * kk_fp8_linear on this device gave up since the last check; its results are then not valid. Refused
- * (KK_ERR_CUDA) while the stream is being captured.
+ * Waits for the stream and reports (KK_ERR_TIMEOUT) whether a bounded in-kernel wait of a kk_fp8_linear on this device
+ * gave up since this host thread last checked this stream, or since the process began where it never did; what was
+ * computed on the stream since then is not to be used. Each thread and each stream is told of every failure, one of
+ * another stream's among them: no check takes a report from another. Refused (KK_ERR_CUDA) while the stream is being
+ * captured.
  */
 KK_API kk_status kk_fp8_check(int cuda_ordinal, void* stream);
 /*
  * kk_fp8_wait_selftest -- diagnostics of that failure path: one kernel on the stream waits, with the bounded waits of
  * kk_fp8_linear (cluster = 0: on a block's own barriers, 1: on those that the other block of a pair arrives on) but a
- * limit of limit_ns (1 us .. 100 ms), on a barrier that nothing arrives on. It gives up and returns, and the next check
- * reports it as it would a linear layer's. Only enqueues work, as the operators do. No trap, no fault.
+ * limit of limit_ns (1 us .. 100 ms), on a barrier that nothing arrives on. It gives up and returns, and checks
+ * report it as they would a linear layer's. Only enqueues work, as the operators do. No trap, no fault.
  */
 KK_API kk_status kk_fp8_wait_selftest(int cuda_ordinal, void* stream, int cluster, int64_t limit_ns);
 /* Message of the last kk_fp8_* failure on this thread. */

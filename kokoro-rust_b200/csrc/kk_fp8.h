@@ -39,11 +39,12 @@ cudaError_t launch_fp8_quantize(const void* x, int type, long rows, long k, long
                                 cudaStream_t st);
 cudaError_t launch_fp8_dequantize(Fp8Store q, long rows, long k, int block_rows, void* y, int type, long ldy,
                                   cudaStream_t st);
-// err receives 2 if a bounded pipeline wait expires; null: the device's own flag, for fp8_take_wait_error
+// err receives 2 if a bounded pipeline wait expires; null: the device counts it, for fp8_wait_failures
 cudaError_t launch_fp8_linear(const Fp8Linear& a, int* err, cudaStream_t st);
-// Waits for the stream (an error while it is being captured); *flag = the current device's flag, which is cleared.
-cudaError_t fp8_take_wait_error(int* flag, cudaStream_t st);
-// A wait that expires (after limit_ns, in place of the waits' own limit) and raises the current device's flag.
+// Waits for the stream (an error while it is being captured); *count = how many blocks on the current device have given up
+// a wait since the process began.
+cudaError_t fp8_wait_failures(unsigned* count, cudaStream_t st);
+// A wait that expires (after limit_ns, in place of the waits' own limit) and is counted.
 cudaError_t launch_fp8_wait_selftest(int cluster, unsigned long long limit_ns, cudaStream_t st);
 
 }  // namespace kk

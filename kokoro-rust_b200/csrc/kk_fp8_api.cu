@@ -1,7 +1,9 @@
 // C entries of the 8-bit operators: argument checks, the caller's device and stream, status codes.
 #include <cuda_runtime.h>
 #include <atomic>
+#include <map>
 #include <string>
+#include <utility>
 
 #include "../../include/kokoro_b200.h"
 #include "kk_fp8.h"
@@ -258,13 +260,22 @@ kk_status kk_fp8_wait_selftest(int cuda_ordinal, void* stream, int cluster, int6
 }
 
 kk_status kk_fp8_check(int cuda_ordinal, void* stream) {
-  int flag = 0;
-  int* const out = &flag;
+  unsigned count = 0;
+  unsigned* const out = &count;
   const kk_status s = run(cuda_ordinal, "kk_fp8_check: ", [](const void* p, cudaStream_t st) {
-    return kk::fp8_take_wait_error(*(int* const*)p, st);
+    return kk::fp8_wait_failures(*(unsigned* const*)p, st);
   }, &out, stream);
-  if (s == KK_OK && flag) return fail(KK_ERR_TIMEOUT, "a bounded pipeline wait of kk_fp8_linear expired");
-  return s;
+  if (s != KK_OK) return s;
+  // what this thread has been told of on this stream
+  thread_local std::map<std::pair<int, void*>, unsigned> told;
+  try {
+    unsigned& t = told[{cuda_ordinal, stream}];
+    if (t == count) return KK_OK;
+    t = count;
+  } catch (...) {
+    return fail(KK_ERR_OOM, "kk_fp8_check: out of host memory");
+  }
+  return fail(KK_ERR_TIMEOUT, "a bounded pipeline wait of kk_fp8_linear expired");
 }
 
 }  // extern "C"

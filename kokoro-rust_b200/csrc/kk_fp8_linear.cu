@@ -17,8 +17,18 @@
 
 namespace kk {
 
-// Raised by a kernel of the stand-alone operators whose bounded pipeline wait expired; one per device.
-__device__ int g_fp8_wait_error;
+// Blocks of the stand-alone operators that gave up a bounded pipeline wait, since the process began; one per device. It
+// only grows, so that nobody who reads it takes a failure from another.
+__device__ unsigned g_fp8_wait_failures;
+
+// One thread of a block, once all its warps are through, if one of them gave up: raises the caller's flag, or counts.
+__device__ __forceinline__ void report_failure(int* err, const volatile int* abort_flag) {
+  if (*abort_flag == 0) return;
+  if (err)
+    atomicExch(err, 2);
+  else
+    atomicAdd(&g_fp8_wait_failures, 1u);
+}
 
 // ---- PTX of the block-scaled MMA
 
@@ -489,7 +499,7 @@ struct PairLoop {
     full = (uint64_t*)(tmem_slot + 2);
     empty = full + S::STAGES, sf_full = empty + S::STAGES, sf_empty = sf_full + SF_RING;
     acc_full = sf_empty + SF_RING, acc_free = acc_full + S::ACC, more = acc_free + S::ACC;
-    err = p.err ? p.err : &g_fp8_wait_error;
+    err = (int*)abort_flag;  // (raised outside at the end)
     warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     rank = cta_rank();
     tiles = p.m_tiles * p.n_tiles, first = blockIdx.x >> 1, step = gridDim.x >> 1;
@@ -517,6 +527,8 @@ struct PairLoop {
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0) report_failure(p.err, abort_flag);
+    __syncwarp();
     cluster_sync();
     if (warp == 0) {
       tc_fence_after();
@@ -1029,7 +1041,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
   volatile int* abort_flag = &abort_s;
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const Fp8Linear& a = p.a;
-  int* err = p.err ? p.err : &g_fp8_wait_error;
+  int* err = &abort_s;  // (raised outside at the end)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = p.splits, share = blockIdx.x % splits, tile = blockIdx.x / splits;
   const long m0 = (long)(tile / p.n_tiles) * TM, n0 = (long)(tile % p.n_tiles) * NT;
@@ -1180,6 +1192,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::TMEM_COLS));
   }
   const bool done = *abort_flag == 0;
+  if (threadIdx.x == 0) report_failure(p.err, abort_flag);
   if (a.gelu) {
 #pragma unroll
     for (int i = 0; i < 4; i++) bias_r[i] = gelu_bias(bias_r[i]);
@@ -1471,9 +1484,10 @@ __global__ void fp8_wait_selftest_kernel(int cluster, unsigned long long limit_n
   mbar_init(&bar, 1);
   abort_flag = 0;
   if (cluster)
-    mbar_wait_cluster(&bar, 0, &abort_flag, &g_fp8_wait_error, limit_ns);
+    mbar_wait_cluster(&bar, 0, &abort_flag, &abort_flag, limit_ns);
   else
-    mbar_wait_lim(&bar, 0, &abort_flag, &g_fp8_wait_error, limit_ns);
+    mbar_wait_lim(&bar, 0, &abort_flag, &abort_flag, limit_ns);
+  report_failure(nullptr, &abort_flag);
 }
 
 cudaError_t launch_fp8_wait_selftest(int cluster, unsigned long long limit_ns, cudaStream_t st) {
@@ -1481,17 +1495,12 @@ cudaError_t launch_fp8_wait_selftest(int cluster, unsigned long long limit_ns, c
   return cudaGetLastError();
 }
 
-cudaError_t fp8_take_wait_error(int* err, cudaStream_t st) {
-  int zero = 0;
+cudaError_t fp8_wait_failures(unsigned* count, cudaStream_t st) {
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   cudaError_t e = cudaStreamIsCapturing(st, &capture);
   if (e == cudaSuccess && capture != cudaStreamCaptureStatusNone) e = cudaErrorStreamCaptureUnsupported;
-  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(err, g_fp8_wait_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(count, g_fp8_wait_failures, sizeof(*count), 0, cudaMemcpyDeviceToHost, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  if (e == cudaSuccess && *err) {
-    e = cudaMemcpyToSymbolAsync(g_fp8_wait_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  }
   return e;
 }
 

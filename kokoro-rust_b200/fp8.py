@@ -261,12 +261,13 @@ def _current(device):
 
 def check(device=None) -> None:
     """Waits for the current stream and raises if a bounded in-kernel wait of a linear layer on this
-    device gave up since the last check (its results are then not valid). Refused while the stream is
-    being captured."""
+    device, of whichever stream, gave up since this host thread last checked this stream (or since the
+    process began): the stream's results since then are not valid. Every thread and stream is told.
+    Refused while the stream is being captured."""
     _run(load_library().kk_fp8_check(*_current(device)))
 
 
 def wait_selftest(device=None, cluster: bool = False, limit_ns: int = 5000) -> None:
-    """Diagnostics: a kernel on the current stream waits in vain for limit_ns and gives up, which the next ``check``
+    """Diagnostics: a kernel on the current stream waits in vain for limit_ns and gives up, which ``check``
     reports (kk_fp8_wait_selftest)."""
     _run(load_library().kk_fp8_wait_selftest(*_current(device), int(cluster), int(limit_ns)))

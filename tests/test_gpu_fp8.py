@@ -756,3 +756,42 @@ def test_an_expired_wait_is_reported_once(kk, cluster):
     for l, y in zip(layers, want):
         assert torch.equal(fp8.linear(*l), y)
     assert not expired(kk)
+
+
+def test_no_check_takes_an_expired_wait_from_another(kk):
+    """One of stream a is reported on stream b and to another thread, whoever checks first, once to each."""
+    import threading
+    fp8 = kk.fp8
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def on(stream):
+        with torch.cuda.stream(stream):
+            return expired(kk)
+
+    def elsewhere(f):
+        got = []
+        t = threading.Thread(target=lambda: got.append(f()))
+        t.start()
+        t.join()
+        return got[0]
+
+    for s in (a, b):
+        on(s)  # (a stream's first check tells of what other tests left)
+    assert not on(a) and not on(b)
+    for first, second in ((a, b), (b, a)):
+        with torch.cuda.stream(a):
+            fp8.wait_selftest()
+        a.synchronize()
+        assert on(first) and on(second)
+        assert not on(first) and not on(second)
+        assert elsewhere(lambda: (on(a), on(a))) == (True, False)  # (this thread's first check)
+        assert not on(a) and not on(b)
+    # a failure between another stream's failure and its check
+    with torch.cuda.stream(a):
+        fp8.wait_selftest()
+    with torch.cuda.stream(b):
+        fp8.wait_selftest(cluster=True)
+        b.synchronize()
+    assert on(a) and on(b) and not on(a) and not on(b)
+    expired(kk)  # (the current stream's own, for the tests after this one)
+    assert not expired(kk)
