@@ -374,8 +374,10 @@ KK_API const char* kk_conv_selftest_error(void);
  * byte per 128 columns): a block stands for value * 2^(E - 127). block_rows is 1 for activations (one
  * row of exps per row) and 128 for weights (one row of exps per 128 rows). ldv is a multiple of 16 and
  * lde of 4; values are 16-byte and exps 4-byte aligned. A block's E is the smallest integer >= 0 with
- * max |x| <= 448 * 2^(E - 127) over its finite values; values are rounded to nearest even; infinities and
- * NaN are held as NaN, which e4m3 has, and so reach every result that reads them. Nothing but the rows x k
+ * max |x| <= 448 * 2^(E - 127) over its finite values; values are rounded to nearest even (off by at most 2^-4 of
+ * the value, or by 2^-10 * 2^(E - 127) where that is more); infinities and
+ * NaN are held as NaN, which e4m3 has, and so reach every result that reads them. Magnitudes from 248 * 2^120 =
+ * 3.2965e38 on are held as 2^128, which reads back as infinity (a linear layer multiplies by 2^128). Nothing but the rows x k
  * values and their exps is written: not the bytes between k and ldv, nor rows behind the last. (kk_fp8_linear
  * reads exps by whole 4-byte words.)
  *

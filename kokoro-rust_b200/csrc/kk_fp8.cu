@@ -3,8 +3,8 @@
 //
 // Block of 128 columns of one row (activations) or 128 x 128 (weights), a = max |x| over its finite
 // values: E is the smallest integer >= 0 with a <= 448 * 2^(E - 127) (448 is e4m3's largest value), and
-// the block is held as e4m3(x * 2^(127 - E)), rounded to nearest even (off by at most 2^-4 of the value);
-// infinities and NaN are held as NaN. A power of two scales exactly, so a value is rounded once and does not
+// the block is held as e4m3(x * 2^(127 - E)), rounded to nearest even (off by at most 2^-4 of the value, or by
+// 2^-10 * 2^(E - 127), half of e4m3's smallest step, where that is more); infinities and NaN are held as NaN. A power of two scales exactly, so a value is rounded once and does not
 // depend on the order or precision of anything; against a scale of a / 448 it gives up at most one binade of
 // e4m3's 17, and it is the scale format the tensor core applies by itself.
 //
@@ -199,7 +199,8 @@ __global__ void __launch_bounds__(256) fp8_quant_blocks_kernel(const T* __restri
 }
 
 // Reading back: value * 2^(E - 127), LANES lanes per block of a row, U blocks a lane. The product is exact in 32 bits
-// (a value has 4 significant bits); bf16 keeps it exactly too unless it falls below bf16's normal numbers.
+// (a value has 4 significant bits), and in bf16 unless it falls below bf16's normal numbers; but 2^128, which numbers from
+// 248 * 2^120 = 3.2965e38 on are held as, is infinite in both.
 template <typename T, bool VEC, int U>
 __global__ void __launch_bounds__(256) fp8_dequant_kernel(Fp8Store q, long k, unsigned kb, unsigned units, int block_shift,
                                                           T* __restrict__ y, long ldy) {

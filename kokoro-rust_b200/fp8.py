@@ -169,7 +169,8 @@ def quantize(x: torch.Tensor, block_rows: int = 1, out: Optional[Fp8Tensor] = No
 
 def dequantize(q: Fp8Tensor, dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values that a store stands for, as ``dtype`` (float32 or bfloat16; both hold them exactly,
-    but for bfloat16 below its normal numbers)."""
+    but for bfloat16 below its normal numbers, and for 2^128, which magnitudes from 3.2965e38 on are held as
+    and which reads back as infinity)."""
     if not isinstance(q, Fp8Tensor):
         _refuse("q: a store is wanted")
     if dtype is not _F32 and dtype is not _BF16:

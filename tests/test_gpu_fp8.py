@@ -795,3 +795,29 @@ def test_no_check_takes_an_expired_wait_from_another(kk):
     assert on(a) and on(b) and not on(a) and not on(b)
     expired(kk)  # (the current stream's own, for the tests after this one)
     assert not expired(kk)
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_top_of_the_range_read_back(kk, block_rows):
+    """From 248 * 2^120 on (a tie, to the even code) a value is held as 256 * 2^120 = 2^128: infinite where it is read
+    back, a factor like any other in a layer."""
+    fp8 = kk.fp8
+    border = np.float32(248 * 2.0 ** 120)
+    x = np.zeros((5, 128), np.float32)
+    x[:, 0] = [border, np.nextafter(border, np.float32(0)), np.finfo(np.float32).max, -border, 232 * 2.0 ** 120]
+    # (a tie of its own; -border, the maximum and the border share the block's scale when block_rows is 128)
+    code, E = ref.quantize(x.astype(np.float64), block_rows)
+    q = fp8.quantize(torch.from_numpy(x).cuda(), block_rows=block_rows)
+    check_store(q, code, E)
+    held = ref.dequantize(code, E, block_rows)
+    assert held[0, 0] == 2.0 ** 128 and held[1, 0] == 240 * 2.0 ** 120 and held[4, 0] == 224 * 2.0 ** 120
+    for dtype in (torch.float32, torch.bfloat16):
+        got = fp8.dequantize(q, dtype).double().cpu().numpy()
+        want = np.where(np.abs(held) >= 2.0 ** 128, np.copysign(np.inf, held), held)
+        assert np.array_equal(got, want)
+    w = torch.zeros(3, 128, device="cuda")
+    w[:, 0] = torch.tensor([2.0 ** -3, -3 * 2.0 ** -20, 2.0 ** -100])
+    if block_rows == 1:
+        y = fp8.linear(q, fp8.quantize(w, block_rows=128)).double().cpu().numpy()
+        # 2^-100 is below the smallest step at the scale of the block's 2^-3: it is held as 0
+        assert np.array_equal(y, held[:, :1] * np.array([[2.0 ** -3, -3 * 2.0 ** -20, 0.0]]))
