@@ -284,7 +284,7 @@ struct Lstm {
 
 struct Model {
   float *word, *pos, *tt0, *emb_g, *emb_b;
-  Conv map_in, qkv, dense, ffn, ffn_out;
+  Conv map_in, qkv, dense, ffn, ffn_out;  // (FP8 mode: map_in alone)
   float *attn_g, *attn_b, *full_g, *full_b;
   Conv bert_enc;
   Lin8 qkv8, dense8, ffn8, ffn_out8;  // FP8 mode
@@ -397,7 +397,7 @@ struct Engine {
   Conv load_conv(const Checkpoint& ck, const std::string& p, int cin, int cout, int K, int dil, int pad, int stride,
                  bool bias);
   Conv load_linear(const Checkpoint& ck, const std::string& p, int din, int dout, bool bias = true);
-  Lin8 hold_fp8(const std::vector<float>& w, const Conv& c);
+  Lin8 hold_fp8(const std::vector<float>& w, const std::vector<float>& b);
   AdaIN load_adain(const Checkpoint& ck, const std::string& p, int c, std::vector<float>& fcw, std::vector<float>& fcb);
   ResBlk load_resblk(const Checkpoint& ck, const std::string& p, int din, int dout, bool up, std::vector<float>& fcw,
                      std::vector<float>& fcb);
@@ -598,12 +598,12 @@ Conv Engine::load_linear(const Checkpoint& ck, const std::string& p, int din, in
   return conv_from(w, bias ? b.data() : nullptr, din, dout, 1, 1, 0, 1);
 }
 
-// The weights of a loaded linear layer ([cout][cin]) in 8 bits, quantised on the device.
-Lin8 Engine::hold_fp8(const std::vector<float>& w, const Conv& c) {
+// A linear layer (w [cout][cin]) held in 8 bits alone, quantised on the device.
+Lin8 Engine::hold_fp8(const std::vector<float>& w, const std::vector<float>& b) {
   Lin8 l;
-  l.cin = c.cin, l.cout = c.cout, l.b = c.b;
-  l.w.ldv = (c.cin + 15) / 16 * 16, l.w.lde = (c.cin + 511) / 512 * 4;
-  const size_t nv = (size_t)c.cout * l.w.ldv, ne = (size_t)(c.cout + 127) / 128 * l.w.lde;
+  l.cout = (int)b.size(), l.cin = (int)(w.size() / b.size()), l.b = up(b);
+  l.w.ldv = (l.cin + 15) / 16 * 16, l.w.lde = (l.cin + 511) / 512 * 4;
+  const size_t nv = (size_t)l.cout * l.w.ldv, ne = (size_t)(l.cout + 127) / 128 * l.w.lde;
   KK_CUDA(cudaMalloc(&l.w.v, nv + ne));
   wallocs.push_back(l.w.v);
   wbytes += nv + ne;
@@ -611,7 +611,7 @@ Lin8 Engine::hold_fp8(const std::vector<float>& w, const Conv& c) {
   float* f = nullptr;
   KK_CUDA(cudaMalloc(&f, w.size() * sizeof(float)));
   cudaError_t e = cudaMemcpyAsync(f, w.data(), w.size() * sizeof(float), cudaMemcpyHostToDevice, st);
-  if (e == cudaSuccess) e = launch_fp8_quantize(f, FP8_F32, c.cout, c.cin, c.cin, 128, l.w, st);
+  if (e == cudaSuccess) e = launch_fp8_quantize(f, FP8_F32, l.cout, l.cin, l.cin, 128, l.w, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   cudaFree(f);
   KK_CUDA(e);
@@ -735,22 +735,28 @@ void Engine::load(const Checkpoint& ck) {
       w.insert(w.end(), a.begin(), a.end());
       b.insert(b.end(), c.begin(), c.end());
     }
-    m.qkv = conv_from(w, b.data(), 768, 2304, 1, 1, 0, 1);
-    if (text_fp8) m.qkv8 = hold_fp8(w, m.qkv);
+    if (text_fp8)
+      m.qkv8 = hold_fp8(w, b);
+    else
+      m.qkv = conv_from(w, b.data(), 768, 2304, 1, 1, 0, 1);
   }
-  m.dense = load_linear(ck, L + ".attention.dense", 768, 768);
+  if (text_fp8) {
+    auto held = [&](const std::string& p, int din, int dout) {
+      return hold_fp8(ck.get(p + ".weight", {dout, din}), ck.get(p + ".bias", {dout}));
+    };
+    m.dense8 = held(L + ".attention.dense", 768, 768);
+    m.ffn8 = held(L + ".ffn", 768, 2048);
+    m.ffn_out8 = held(L + ".ffn_output", 2048, 768);
+  } else {
+    m.dense = load_linear(ck, L + ".attention.dense", 768, 768);
+    m.ffn = load_linear(ck, L + ".ffn", 768, 2048);
+    m.ffn_out = load_linear(ck, L + ".ffn_output", 2048, 768);
+  }
   m.attn_g = up(ck.get(L + ".attention.LayerNorm.weight", {768}));
   m.attn_b = up(ck.get(L + ".attention.LayerNorm.bias", {768}));
-  m.ffn = load_linear(ck, L + ".ffn", 768, 2048);
-  m.ffn_out = load_linear(ck, L + ".ffn_output", 2048, 768);
   m.full_g = up(ck.get(L + ".full_layer_layer_norm.weight", {768}));
   m.full_b = up(ck.get(L + ".full_layer_layer_norm.bias", {768}));
   m.bert_enc = load_linear(ck, "bert_encoder", 768, 512);
-  if (text_fp8) {
-    m.dense8 = hold_fp8(ck.get(L + ".attention.dense.weight", {768, 768}), m.dense);
-    m.ffn8 = hold_fp8(ck.get(L + ".ffn.weight", {2048, 768}), m.ffn);
-    m.ffn_out8 = hold_fp8(ck.get(L + ".ffn_output.weight", {768, 2048}), m.ffn_out);
-  }
   // ---- predictor (src/model.rs:60-86)
   for (int i = 0; i < 3; i++) {
     m.dur_lstm[i] = load_lstm(ck, "predictor.text_encoder.lstms." + std::to_string(2 * i), 640);
@@ -1595,7 +1601,7 @@ void Engine::forward(int B, const int64_t* ids, const int32_t* ids_len, const fl
       t.ypre = yp, t.ypre_rows = pre_rows;
       return t;
     };
-    if (precision == KK_PRECISION_BF16 && tc_ok) {
+    if (precision == KK_PRECISION_BF16 && tc_ok && !text_fp8) {
       hpre = ar.get<uint8_t>(planes768);
       ctxpre = ar.get<uint8_t>(planes768);
       apre = ar.get<uint8_t>(planes768);
@@ -1613,10 +1619,10 @@ void Engine::forward(int B, const int64_t* ids, const int32_t* ids_len, const fl
     // GELU layer as they finish them (the attention's rows by the quantiser); the residual rows stay in 32 bits
     Fp8Store hq{}, cq{}, aq{}, fq{};
     if (text_fp8) {
-      planes = false;
       hq = fp8_rows(LT, 768), cq = fp8_rows(LT, 768), aq = fp8_rows(LT, 768), fq = fp8_rows(LT, 2048);
+    } else if (!planes) {
+      f = ar.get<float>((size_t)LT * 2048);
     }
-    if (!planes && !text_fp8) f = ar.get<float>((size_t)LT * 2048);
     linear(m.map_in, emb, 128, LT, h, 768);
     int max_t = 0;
     for (int b = 0; b < B; b++) max_t = std::max(max_t, ids_len[b]);

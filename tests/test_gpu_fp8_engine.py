@@ -143,3 +143,22 @@ def test_fp8_identity_and_vocoder(kk, ckpt_path, eng8):
                               e16.decode_batch([asr], [f0], [nc], s, seeds=[3])[0])
     finally:
         e16.close()
+
+
+def test_fp8_mode_holds_its_layers_in_8_bits_alone(kk, ckpt_path, cases):
+    """The four layers' weights take a byte each and a scale for each 128 x 128, where the BF16 mode has 4 bytes (f32) and
+    at least 2 (bf16 tiles); and a forward's buffers are no larger."""
+    layers = ((2304, 768), (768, 768), (2048, 768), (768, 2048))
+    values = sum(n * k for n, k in layers)
+    scales = sum(-(-n // 128) * -(-k // 512) * 4 for n, k in layers)
+    fresh, after = {}, {}
+    for mode in ("bf16", "fp8"):
+        e = kk.GpuKokoro(ckpt_path, 0, mode)
+        try:
+            fresh[mode] = e.device_bytes()
+            e.forward_batch(cases)
+            after[mode] = e.device_bytes()
+        finally:
+            e.close()
+    assert fresh["bf16"] - fresh["fp8"] >= (4 + 2 - 1) * values - scales
+    assert after["fp8"] - fresh["fp8"] <= after["bf16"] - fresh["bf16"]
