@@ -162,3 +162,77 @@ def test_fp8_mode_holds_its_layers_in_8_bits_alone(kk, ckpt_path, cases):
             e.close()
     assert fresh["bf16"] - fresh["fp8"] >= (4 + 2 - 1) * values - scales
     assert after["fp8"] - fresh["fp8"] <= after["bf16"] - fresh["bf16"]
+
+
+def test_fp8_canary_audio_is_the_same(kk, eng8, cases):
+    """With every buffer NaN before it is written, the audio too has the same bits."""
+    want = eng8.forward_batch(cases)
+    eng8.set_option(kk.engine.KK_OPT_GAP_CANARY, 1)
+    try:
+        got = eng8.forward_batch(cases)
+    finally:
+        eng8.set_option(kk.engine.KK_OPT_GAP_CANARY, 0)
+    for a, b in zip(want, got):
+        assert np.array_equal(a.audio, b.audio)
+
+
+@pytest.fixture(scope="module")
+def large(kk):
+    """13 items of 511 tokens, 6,669 rows with their gaps: 53 tiles of 128 rows, at which every layer is past the small
+    layers' kernel. That takes more than 2 x 148 tiles of 128 x 128 (QKV, 18 tiles wide; the output projection and the
+    down projection, 6 wide: 318), more than 148 for the 8-bit result of the GELU layer (16 wide)."""
+    rng = np.random.default_rng(33)
+    items = []
+    for i in range(13):
+        ids, ref_s = synth_item(rng, 509)
+        items.append(kk.BatchItem(ids, ref_s, 1.0, kk.ItemNoise(seed=300 + i)))
+    return items
+
+
+LOOKED_AT = (0, 6, 12)  # of the large batch, against the oracles
+
+
+def test_fp8_encoder_rows_of_a_large_batch(eng8, large, oracle, oracle8):
+    """The bounds of the small batches hold for the large layers' kernels and their rows for the attention."""
+    d = tempfile.mkdtemp()
+    os.environ["KK_DEBUG_DUMP_DIR"] = d
+    try:
+        eng8.forward_batch(large, forced_dur=[np.arange(511) < 4] * len(large))
+    finally:
+        del os.environ["KK_DEBUG_DUMP_DIR"]
+    bert = np.fromfile(os.path.join(d, "bert.f32"), np.float32).reshape(-1, 768)
+    for i in LOOKED_AT:
+        ids = np.asarray(large[i].ids)
+        p, p8 = oracle.albert(ids).numpy(), oracle8.albert(ids).numpy()
+        got = bert[i * 513:i * 513 + 511]
+        far = np.linalg.norm(p8 - p) / np.linalg.norm(p)
+        off = np.linalg.norm(got - p8) / np.linalg.norm(p8)
+        worst = (np.linalg.norm(got - p8, axis=1) / np.linalg.norm(p8, axis=1)).max()
+        print(f"item {i}: 8-bit oracle {far:.3g} off the plain one, engine {off:.3g} off the 8-bit one, worst row {worst:.3g}")
+        assert far <= 0.25 and off <= 0.6 * far
+        # no row is lost among the others: a wrong one would be 1 or more off, the rounding errors of 768 columns average
+        assert worst <= 3 * 0.6 * far
+
+
+def test_fp8_durations_of_a_large_batch(kk, ckpt_path, eng8, large, oracle, oracle8):
+    """What the mode says of its durations: some differ, by a frame, from the BF16 mode's and from the plain oracle's.
+
+    How many: a duration is a rounded sum, so it changes with a probability that goes with how far the sum moves. The
+    engine's rows are at most 0.6 as far from the 8-bit oracle's as those are from the plain ones, so at most 1.6 times as
+    far from the plain ones, and 1.6 times as many durations may change as between the two oracles, give or take four
+    standard deviations of a count."""
+    outs = eng8.forward_batch(large, fetch=False)
+    e16 = kk.GpuKokoro(ckpt_path, 0, "bf16")
+    try:
+        outs16 = e16.forward_batch(large, fetch=False)
+    finally:
+        e16.close()
+    assert all(np.abs(a.pred_dur - b.pred_dur).max() <= 1 for a, b in zip(outs, outs16))
+    n = moved = moved8 = 0
+    for i in LOOKED_AT:
+        it, got = large[i], outs[i].pred_dur
+        plain, eight = (o.durations(it.ids, it.ref_s)[0] for o in (oracle, oracle8))
+        assert np.abs(got - eight).max() <= 1 and np.abs(got - plain).max() <= 1
+        n, moved, moved8 = n + len(got), moved + int((got != plain).sum()), moved8 + int((eight != plain).sum())
+    print(f"{moved} of {n} durations differ from the plain oracle's, {moved8} between the oracles")
+    assert 0 < moved <= 1.6 * moved8 + 4 * np.sqrt(1.6 * moved8) + 4
