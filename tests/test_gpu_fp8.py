@@ -821,3 +821,58 @@ def test_top_of_the_range_read_back(kk, block_rows):
         y = fp8.linear(q, fp8.quantize(w, block_rows=128)).double().cpu().numpy()
         # 2^-100 is below the smallest step at the scale of the block's 2^-3: it is held as 0
         assert np.array_equal(y, held[:, :1] * np.array([[2.0 ** -3, -3 * 2.0 ** -20, 0.0]]))
+
+
+@pytest.mark.parametrize("m", [1, 66, 513, 5000])
+def test_feed_forward_block_by_its_middle_store(kk, m):
+    """The block's two layers each against the definition, the second on the codes that the first left: every element of
+    both within its own layer's bound."""
+    rng = np.random.default_rng(m + 1)
+    fp8 = kk.fp8
+    x = torch.from_numpy(rng.standard_normal((m, 768)).astype(np.float32)).cuda()
+    W = [(rng.uniform(-1, 1, s) / np.sqrt(s[1])).astype(np.float32) for s in ((2048, 768), (768, 2048))]
+    B = [(rng.uniform(-1, 1, s) * 0.03).astype(np.float32) for s in (2048, 768)]
+    w1, w2 = (fp8.quantize(torch.from_numpy(w).cuda(), block_rows=128) for w in W)
+    b1, b2 = (torch.from_numpy(b).cuda() for b in B)
+    d1, d2 = (ref.dequantize(bits(w.values), w.exps.cpu().numpy(), 128) for w in (w1, w2))
+    xq = fp8.quantize(x)
+    xd = ref.dequantize(bits(xq.values), xq.exps.cpu().numpy())
+    h = fp8.linear(xq, w1, b1, act="gelu", out_dtype=E4M3)
+    want, S = ref.linear(xd, d1, B[0], "gelu")
+    check_linear(h, want, S, None, 768, "gelu", E4M3)
+    hd = ref.dequantize(bits(h.values), h.exps.cpu().numpy())
+    for dtype in (torch.float32, torch.bfloat16):
+        r = x.to(dtype)
+        y, S2 = ref.linear(hd, d2, B[1], None, r.double().cpu().numpy())
+        rms = np.sqrt((hd ** 2) @ (d2 ** 2).T + y ** 2)
+        got = fp8.linear(h, w2, b2, residual=r, out_dtype=dtype)
+        check_linear(got, y, S2, rms, 2048, None, dtype)
+        if dtype == torch.float32:
+            assert torch.equal(got, feed_forward(fp8, x, w1, b1, w2, b2, x))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("m, n, k", [(66, 2048, 768), (700, 640, 520), (4800, 1000, 384), (5003, 1157, 2100), (2600, 2304, 768)])
+def test_rounded_results_as_a_whole(kk, m, n, k, dtype):
+    """The norm of what rounding leaves, beside check_linear's bound on each element. A value falls anywhere between two
+    neighbours, so its rounding error has 1 / sqrt(3) of the most it can be (root mean square): 2^-8 |y| in bf16, 2^-4 |y| or
+    half of the smallest step in e4m3, four standard deviations of the mean of N squares (each at most 1 where their mean
+    is 1/3) above that; and the additions' part as for 32-bit results."""
+    rng = np.random.default_rng(m + n + k)
+    fp8 = kk.fp8
+    xq, wq, xd, wd = make(rng, m, n, k, fp8)
+    bias = rng.standard_normal(n).astype(np.float32) * 0.1
+    res = torch.from_numpy(rng.standard_normal((m, n)).astype(np.float32)).cuda().to(dtype) if dtype != E4M3 else None
+    for act, r in ((None, None), ("gelu", None), (None, res), ("gelu", res)) if dtype != E4M3 else ((None, None), ("gelu", None)):
+        y, S = ref.linear(xd, wd, bias, act, None if r is None else r.double().cpu().numpy())
+        got = fp8.linear(xq, wq, torch.from_numpy(bias).cuda(), act=act, residual=r, out_dtype=dtype)
+        if dtype == E4M3:
+            g = ref.dequantize(bits(got.values), got.exps.cpu().numpy())
+            amax = np.stack([np.abs(y[:, b:b + 128]).max(1) for b in range(0, n, 128)], 1)
+            most = np.maximum(2.0 ** -4 * np.abs(y), 2.0 ** -10 / 224 * np.repeat(amax, 128, 1)[:, :n])
+        else:
+            g, most = got.double().cpu().numpy(), 2.0 ** -8 * np.abs(y)
+        rms = np.sqrt((xd ** 2) @ (wd ** 2).T + y ** 2)
+        added = 4 * (k / 32 + 8) * 2.0 ** -23 * (1.13 if act else 1.0) + 2.0 ** -20 * (act is not None)
+        rounded = np.sqrt((1 / 3 + 4 * 0.5 / np.sqrt(y.size)) * (most ** 2).sum())
+        assert np.linalg.norm(g - y) <= added * np.linalg.norm(rms) + rounded
