@@ -176,12 +176,24 @@ __device__ __forceinline__ void pause_1ms() {
 
 constexpr int SF_RING = 4;  // scale groups (4 blocks of K each) of a pair, in shared memory and TMEM
 
+// Waits until what used a ring's places last is done, from place s on, with the parity of its loop's next wait (which a place
+// that was never used passes). The commits of a pair's MMAs arrive on barriers of both CTAs, the second CTA's from the
+// first: none may still be on its way there when its shared memory goes.
+template <int RING>
+__device__ __forceinline__ void last_uses(uint64_t* done, uint32_t s, uint32_t ph, volatile int* abort_flag, int* err) {
+#pragma unroll 1
+  for (int i = 0; i < RING; i++) {
+    if (!warp_wait(done + s, ph, abort_flag, err)) return;
+    if (++s == RING) s = 0, ph ^= 1;
+  }
+}
+
 // ---- scales
 // One warp brings the scales of a CTA's tiles, a group (four blocks of K: a word for each row of x and of W) at a
 // time, into a ring of shared-memory slots in the layout of the TMEM copy. A word waits behind the TMA's boxes on its
 // way from L2 (about 2000 cycles, as long as the MMAs of two or three groups), so the words of the next AHEAD groups
 // are always on their way, in registers; waiting for each group in turn held the MMAs up by half.
-template <int RING, int ROWS_W>
+template <int RING, int ROWS_W, bool PAIR>
 struct ScaleFeed {
   static constexpr int NB = (ROWS_W + 127) / 128, BYTES = 512 * (1 + NB), AHEAD = 4;
   const Fp8Linear& a;
@@ -227,7 +239,10 @@ struct ScaleFeed {
     while (true) {
 #pragma unroll
       for (int i = 0; i < AHEAD; i++) {
-        if (left-- == 0) return;
+        if (left-- == 0) {
+          if (PAIR) last_uses<RING>(empty, slot, ph, abort_flag, err);
+          return;
+        }
         if (used && !warp_wait(empty + slot, ph, abort_flag, err)) return;
         const uint32_t dst = ring + slot * BYTES + lane * 16;
 #pragma unroll
@@ -558,6 +573,7 @@ struct PairLoop {
         if (++s == S::STAGES) s = 0, ph ^= 1;
       }
     }
+    if (ok) last_uses<S::STAGES>(empty, s, ph, abort_flag, err);
     // After an expired wait, loads still in flight land before the shared memory goes: the first CTA sees them
     // complete, the second, whose loads complete there, waits far longer than a load takes.
     if (!ok) {
@@ -617,7 +633,7 @@ struct PairLoop {
   }
 
   __device__ __forceinline__ void scales() {
-    ScaleFeed<SF_RING, S::N> feed{p.a, smem_u32(smem + S::OFF_SF), sf_full, sf_empty, abort_flag, err, lane};
+    ScaleFeed<SF_RING, S::N, true> feed{p.a, smem_u32(smem + S::OFF_SF), sf_full, sf_empty, abort_flag, err, lane};
     feed.run(first, step, tiles, 0, p.kb, [&](int t, long* m0, long* n0) {
       int mt, nt;
       tile_at(p, t, &mt, &nt);
@@ -1162,7 +1178,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     if (ok && lead) mma_commit(&acc_full);
     if (!ok && last >= 0) mbar_drain(empty + last, last_ph);  // MMAs in flight end before their operands and TMEM go
   } else if (warp == 2) {
-    ScaleFeed<SPLIT_RING, NT> feed{a, smem_u32(sf_s), sf_full, sf_empty, abort_flag, err, lane};
+    ScaleFeed<SPLIT_RING, NT, false> feed{a, smem_u32(sf_s), sf_full, sf_empty, abort_flag, err, lane};
     feed.run(0, 1, 1, b_lo & ~3, b_hi, [&](int, long* m, long* n) { *m = m0, *n = n0; });
   } else if (warp >= 4) {
     const bool ok = warp_wait(&acc_full, 0, abort_flag, err);

@@ -876,3 +876,30 @@ def test_rounded_results_as_a_whole(kk, m, n, k, dtype):
         added = 4 * (k / 32 + 8) * 2.0 ** -23 * (1.13 if act else 1.0) + 2.0 ** -20 * (act is not None)
         rounded = np.sqrt((1 / 3 + 4 * 0.5 / np.sqrt(y.size)) * (most ** 2).sum())
         assert np.linalg.norm(g - y) <= added * np.linalg.norm(rms) + rounded
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, E4M3])
+def test_short_kernels_of_pairs_in_a_row(kk, dtype):
+    """One block of K and a tile or two a pair, hundreds of times in a row on two streams: blocks that begin in the shared
+    memory of blocks that just ended."""
+    rng = np.random.default_rng(23)
+    fp8 = kk.fp8
+    xq, wq, _, _ = make(rng, 25000, 300, 100, fp8)
+    res = torch.randn(25000, 300, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+
+    def call(r):
+        y = fp8.linear(xq, wq, residual=r if dtype != E4M3 else None, out_dtype=dtype)
+        return y.values.view(torch.uint8) if dtype == E4M3 else y
+
+    for r in (None, res):
+        want = call(r)
+        wrong = [torch.zeros((), device="cuda", dtype=torch.int64) for _ in streams]
+        torch.cuda.synchronize()
+        for _ in range(200):
+            for s, bad in zip(streams, wrong):
+                with torch.cuda.stream(s):
+                    bad += (call(r) != want).sum()
+        torch.cuda.synchronize()
+        assert not any(bad.item() for bad in wrong)
+    fp8.check()
