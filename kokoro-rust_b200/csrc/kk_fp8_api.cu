@@ -127,6 +127,7 @@ kk_status run(int ordinal, const char* what, cudaError_t (*f)(const void*, cudaS
   if (kind == 2) return fail(KK_ERR_CUDA, "device is not compute capability 10.x (sm_100a)");
   DeviceGuard g(ordinal);
   if (g.err != cudaSuccess) return fail(KK_ERR_CUDA, what, cudaGetErrorString(g.err));
+  cudaGetLastError();  // (what an earlier call of this thread left is not this one's)
   const cudaError_t e = f(arg, (cudaStream_t)stream);
   if (e == cudaSuccess) return KK_OK;
   cudaGetLastError();

@@ -903,3 +903,27 @@ def test_short_kernels_of_pairs_in_a_row(kk, dtype):
         torch.cuda.synchronize()
         assert not any(bad.item() for bad in wrong)
     fp8.check()
+
+
+def test_an_earlier_failure_is_not_this_calls(kk):
+    """A call that the library refused with a CUDA error, on this thread, before each of the operators."""
+    import ctypes
+    fp8, lib = kk.fp8, kk.load_library()
+    x = torch.randn(6000, 768, device="cuda")
+    w = fp8.quantize(torch.randn(768, 768, device="cuda"), block_rows=128)
+    n, buf = np.array([1], np.int32), np.zeros(2304, np.float32)
+
+    def fail():
+        assert lib.kk_attention_selftest(99, 1, n.ctypes.data_as(ctypes.c_void_p), buf.ctypes.data_as(ctypes.c_void_p),
+                                         buf.ctypes.data_as(ctypes.c_void_p)) == kk.engine.KK_ERR_CUDA
+
+    fail()
+    q = fp8.quantize(x)
+    fail()
+    fp8.linear(q, w)
+    fail()
+    fp8.linear(q[:5], w, residual=x[:5])
+    fail()
+    assert torch.equal(fp8.dequantize(q), fp8.dequantize(q))
+    fail()
+    fp8.check()
