@@ -19,6 +19,7 @@ from typing import Optional, Union
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from .engine import KK_ERR_INVALID_ARG, KokoroError, load_library
 
@@ -183,6 +184,7 @@ def dequantize(q: Fp8Tensor, dtype: torch.dtype = torch.float32, out: Optional[t
         if out.shape != q.shape:
             _refuse("out: the store's shape is wanted")
         _one_device(dev, out.device)
+        increment_version(out)  # (a backward pass that saved it says so, as for any operator in place)
     _run(load_library().kk_fp8_call(1, _args12(dev.index, _stream(dev.index), *q._args, q.block_rows, rows, k,
                                                out.data_ptr(), _TYPES[dtype], ld), 12))
     return out
@@ -235,6 +237,8 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
             out = Fp8Tensor.empty(m, n, 1, dev)
         elif not isinstance(out, Fp8Tensor) or out.block_rows != 1 or out.shape != (m, n):
             _refuse(f"out: a store [{m}, {n}] with block_rows 1 is wanted")
+        elif out.device != dev:
+            _one_device(dev, out.device)
         y = out._args
     elif out is None:
         out = torch.empty(m, n, dtype=out_dtype, device=dev)
@@ -243,9 +247,10 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
         ldy = _rows(out, "out", (out_dtype,))[2]
         if out.shape != (m, n):
             _refuse(f"out: [{m}, {n}] is wanted")
+        if out.device != dev:
+            _one_device(dev, out.device)
+        increment_version(out)
         y = (out.data_ptr(), ldy, 0, 0)
-    if out.device != dev:
-        _one_device(dev, out.device)
     _run(load_library().kk_fp8_call(2, _args22(dev.index, _stream(dev.index), m, n, k, *x._args, *w._args, b, _ACTS[act],
                                                res, ldr, _TYPES[out_dtype], *y), 22))
     return out

@@ -927,3 +927,20 @@ def test_an_earlier_failure_is_not_this_calls(kk):
     assert torch.equal(fp8.dequantize(q), fp8.dequantize(q))
     fail()
     fp8.check()
+
+
+def test_results_over_what_a_backward_pass_saved(kk):
+    """A tensor that autograd keeps for its backward pass and that is then given as `out`: the backward pass says so."""
+    fp8 = kk.fp8
+    x = fp8.quantize(torch.randn(4, 256, device="cuda"))
+    w = fp8.quantize(torch.randn(256, 256, device="cuda"), block_rows=128)
+    for f in (lambda y: fp8.linear(x, w, out=y), lambda y: fp8.linear(x, w, residual=y, out=y), lambda y: fp8.dequantize(x, out=y)):
+        a = torch.randn(4, 256, device="cuda", requires_grad=True)
+        y = torch.randn(4, 256, device="cuda")
+        z = (a * y).sum()
+        f(y)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.backward()
+    with torch.inference_mode():
+        y = torch.empty(4, 256, device="cuda")
+        assert torch.equal(fp8.linear(x, w, out=y), fp8.linear(x, w))
