@@ -1013,6 +1013,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TileShape<OUT>::THRE
 // nothing is waited for twice: K is split over the CTAs of a cluster until the tiles fill the machine, each CTA
 // starts its loads before anything else, and the shares are summed through the cluster's shared memory (in the
 // order of the shares, so the result does not vary).
+//
+// Two CTAs fit an SM (114 registers of 256 threads, of which a third has no room) and its 512 TMEM columns: no allocation
+// waits, which in a cluster could be for a CTA that waits for its own cluster.
 constexpr int SPLIT_THREADS = 256;
 constexpr int SPLIT_RING = 8;          // scale groups held
 constexpr int SPLIT_STAGES = 8;        // at most
