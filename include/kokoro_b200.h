@@ -374,17 +374,17 @@ KK_API const char* kk_conv_selftest_error(void);
  * byte per 128 columns): a block stands for value * 2^(E - 127). block_rows is 1 for activations (one
  * row of exps per row) and 128 for weights (one row of exps per 128 rows). ldv is a multiple of 16 and
  * lde of 4; values are 16-byte and exps 4-byte aligned. A block's E is the smallest integer >= 0 with
- * max |x| <= 448 * 2^(E - 127) over its finite values; values are rounded to nearest even (off by at most 2^-4 of
- * the value, or by 2^-10 * 2^(E - 127) where that is more); infinities and
- * NaN are held as NaN, which e4m3 has, and so reach every result that reads them. Magnitudes from 248 * 2^120 =
- * 3.2965e38 on are held as 2^128, which reads back as infinity (a linear layer multiplies by 2^128). Nothing but the rows x k
- * values and their exps is written: not the bytes between k and ldv, nor rows behind the last. (kk_fp8_linear
- * reads exps by whole 4-byte words.)
+ * max |x| <= 448 * 2^(E - 127) over its finite values; values are rounded to nearest even (off by at most 2^-4
+ * of the value, or by 2^-10 * 2^(E - 127) where that is more); infinities and NaN are held as NaN, which e4m3
+ * has, and so reach every result that reads them. Magnitudes from 248 * 2^120 = 3.2965e38 on are held as 2^128,
+ * which reads back as infinity (a linear layer multiplies by 2^128). Nothing but the rows x k values and their
+ * exps is written: not the bytes between k and ldv, nor rows behind the last. (kk_fp8_linear reads exps by whole
+ * 4-byte words.)
  *
  * All pointers are device pointers of device `cuda_ordinal`; `stream` is a cudaStream_t of that device
  * (NULL: its legacy default stream). The calls only enqueue work (they may be captured into a graph),
  * allocate nothing, keep nothing, and may run at once on several streams and host threads. The caller's
- * current device is left as it was. rows / m = 0 is a no-op. Rows and blocks stay below 2^31, columns below 2^30.
+ * current device is left as it was. rows / m = 0 is a no-op. Rows and blocks stay below 2^31, columns below 2^30 (one at least).
  * What a call writes may not overlap what it reads, but for a residual that is the result itself: such calls are
  * refused, as are those whose rows of two pitches lie in one range of addresses.
  */

@@ -4,9 +4,10 @@
 // Block of 128 columns of one row (activations) or 128 x 128 (weights), a = max |x| over its finite
 // values: E is the smallest integer >= 0 with a <= 448 * 2^(E - 127) (448 is e4m3's largest value), and
 // the block is held as e4m3(x * 2^(127 - E)), rounded to nearest even (off by at most 2^-4 of the value, or by
-// 2^-10 * 2^(E - 127), half of e4m3's smallest step, where that is more); infinities and NaN are held as NaN. A power of two scales exactly, so a value is rounded once and does not
-// depend on the order or precision of anything; against a scale of a / 448 it gives up at most one binade of
-// e4m3's 17, and it is the scale format the tensor core applies by itself.
+// 2^-10 * 2^(E - 127), half of e4m3's smallest step, where that is more); infinities and NaN are held as NaN.
+// A power of two scales exactly, so a value is rounded once and does not depend on the order or precision of
+// anything; against a scale of a / 448 it gives up at most one binade of e4m3's 17, and it is the scale format
+// the tensor core applies by itself.
 //
 // All of it is bound by HBM: each kernel reads and writes each byte once, 16 bytes a lane on its 16- or 32-bit
 // side, with several loads in flight before the first is used.

@@ -72,7 +72,8 @@ def _rows(t: torch.Tensor, name: str, dtypes, unit: int = 1):
 class Fp8Tensor:
     """A store of ``rows`` x ``k`` values: ``values`` (float8_e4m3fn [rows, k], rows a multiple of 16
     bytes apart) and ``exps`` (uint8 [ceil(rows / block_rows), ceil(k / 128)], rows a multiple of 4
-    bytes apart): a block stands for value * 2^(E - 127). block_rows is 1 (activations) or 128 (weights)."""
+    bytes apart): a block stands for value * 2^(E - 127). block_rows is 1 (activations) or 128 (weights).
+    It is a view of the tensors' memory and keeps it, but not over a storage's own ``resize_``."""
 
     __slots__ = ("shape", "block_rows", "device", "_values", "_exps", "_buf", "_args")
 
