@@ -2079,6 +2079,7 @@ static thread_local std::string g_create_error;
 
 template <class F>
 static kk_status guarded(kk_engine* h, F&& f) {
+  cudaGetLastError();  // (what an earlier call of this thread left is not this one's)
   try {
     f();
     if (h) h->e->err.clear();

@@ -236,3 +236,25 @@ def test_fp8_durations_of_a_large_batch(kk, ckpt_path, eng8, large, oracle, orac
         n, moved, moved8 = n + len(got), moved + int((got != plain).sum()), moved8 + int((eight != plain).sum())
     print(f"{moved} of {n} durations differ from the plain oracle's, {moved8} between the oracles")
     assert 0 < moved <= 1.6 * moved8 + 4 * np.sqrt(1.6 * moved8) + 4
+
+
+def test_an_earlier_failure_is_not_the_engines(kk, ckpt_path, eng8, cases):
+    """A call that the library refused with a CUDA error, on this thread, before an engine is made (the FP8 mode launches
+    kernels as it loads) and before a forward."""
+    import ctypes
+    lib = kk.load_library()
+    n, buf = np.array([1], np.int32), np.zeros(2304, np.float32)
+    want = eng8.forward_batch(cases[:1])[0]
+
+    def fail():
+        assert lib.kk_attention_selftest(99, 1, n.ctypes.data_as(ctypes.c_void_p), buf.ctypes.data_as(ctypes.c_void_p),
+                                         buf.ctypes.data_as(ctypes.c_void_p)) == kk.engine.KK_ERR_CUDA
+
+    fail()
+    e = kk.GpuKokoro(ckpt_path, 0, "fp8")
+    try:
+        fail()
+        got = e.forward_batch(cases[:1])[0]
+    finally:
+        e.close()
+    assert np.array_equal(got.pred_dur, want.pred_dur) and np.array_equal(got.audio, want.audio)
