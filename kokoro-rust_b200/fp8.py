@@ -42,10 +42,11 @@ _stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
 
 
 def _no_gradient(t: torch.Tensor, name: str):
+    """For a tensor that requires a gradient, or while a dual level is open (tangents live inside one; -1 is outside of all):
+    asked for beforehand, which is 0.03 us where unpacking is 0.5."""
     if t.requires_grad and torch.is_grad_enabled():
         _refuse(f"{name}: the 8-bit operators have no gradient")
-    # (a tangent lives inside a dual level, -1 outside of all: looking there first is 0.03 us instead of 0.5)
-    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+    if forward_ad.unpack_dual(t).tangent is not None:
         _refuse(f"{name}: the 8-bit operators have no gradient, in forward mode either")
 
 
@@ -63,7 +64,8 @@ def _rows(t: torch.Tensor, name: str, dtypes, unit: int = 1):
         _refuse(f"{name}: a row's columns must be adjacent")
     if k == 1 and t.is_neg():  # (the imaginary part of a conjugate, whose columns are never adjacent)
         _refuse(f"{name}: its negation is still to be done (resolve_neg)")
-    _no_gradient(t, name)
+    if t.requires_grad or forward_ad._current_level >= 0:
+        _no_gradient(t, name)
     if not t.is_cuda:
         _refuse(f"{name}: a CUDA tensor is wanted")
     return rows, k, ld if rows > 1 else -(-k // unit) * unit
@@ -217,7 +219,8 @@ def linear(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, a
     if bias is not None:
         if not isinstance(bias, torch.Tensor) or bias.dtype is not _F32 or bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
             _refuse(f"bias: adjacent float32 [{n}] is wanted")
-        _no_gradient(bias, "bias")
+        if bias.requires_grad or forward_ad._current_level >= 0:
+            _no_gradient(bias, "bias")
         if n == 1 and bias.is_neg():
             _refuse("bias: its negation is still to be done (resolve_neg)")
         if bias.device != dev:
