@@ -944,3 +944,48 @@ def test_results_over_what_a_backward_pass_saved(kk):
     with torch.inference_mode():
         y = torch.empty(4, 256, device="cuda")
         assert torch.equal(fp8.linear(x, w, out=y), fp8.linear(x, w))
+
+
+FIRST_LARGE_CALLS_IN_A_CAPTURE = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+import conftest
+fp8 = conftest.import_package().fp8
+E4M3, BF16 = torch.float8_e4m3fn, torch.bfloat16
+m, n, k = 5000, 1040, 520
+x, w = torch.randn(m, k, device="cuda"), torch.randn(n, k, device="cuda") / 25
+b, r = torch.randn(n, device="cuda"), torch.randn(m, n, device="cuda")
+
+def layers(y):
+    xq, wq = fp8.quantize(x), fp8.quantize(w, 128)
+    fp8.linear(xq, wq, b, residual=y, out=y)
+    return [y, fp8.linear(xq, wq, b), fp8.linear(xq, wq, b, out_dtype=BF16),
+            fp8.linear(xq, wq, b, residual=r.to(BF16), out_dtype=BF16),
+            fp8.dequantize(fp8.linear(xq, wq, b, act="gelu", out_dtype=E4M3), BF16)]
+
+y = r.clone()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = layers(y)
+for seed in (1, 2):
+    torch.manual_seed(seed)
+    x.copy_(torch.randn(m, k, device="cuda"))
+    y.copy_(r)
+    g.replay()
+    want = layers(r.clone())
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+fp8.check()
+print("fine")
+"""
+
+
+def test_first_large_calls_of_a_process_may_be_captured():
+    """The kernels of pairs, with and without a residual, in each result type: their first launches inside a capture, and
+    replayed on new inputs."""
+    import os
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", FIRST_LARGE_CALLS_IN_A_CAPTURE, os.path.dirname(os.path.abspath(__file__))],
+                       capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
